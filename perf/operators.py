@@ -245,13 +245,18 @@ def run(state):
 
 # ------------------------------------------------------------------------------------------------ 64 bits
 
+def _pow2(e):
+    """2^e for whole numbers, exactly (from the bits of a double)."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
 def _exact_mx(x):
     """The values that the 4-bit form of x [r, k] stands for, by nearest neighbour on the E2M1 grid."""
     v = x.double().view(x.shape[0], -1, 32)
     v = torch.where(v.isfinite(), v, 0.0)
     grid = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64, device=v.device)
     _, e = torch.frexp(v.abs().amax(-1, keepdim=True))      # max = m * 2^e with m in [0.5, 1)
-    unit = torch.pow(torch.full_like(v[..., :1], 2.0), (e - 3).clamp(min=-127).double())
+    unit = _pow2((e - 3).clamp(min=-127))
     a = v.abs() / unit
     low = (torch.searchsorted(grid, a.contiguous(), right=True) - 1).clamp(0, 7)
     high = (low + 1).clamp(max=7)
@@ -281,7 +286,7 @@ def exact(case, seed):
         w = torch.tensor(grid + [-v for v in grid], dtype=torch.float64, device=c.device)[c]
         row, blk = torch.arange(r, device=c.device)[:, None], torch.arange(k // 32, device=c.device)[None, :]
         at = (row // 128 * -(-k // 128) + blk // 4) * 512 + row % 32 * 16 + row % 128 // 32 * 4 + blk % 4
-        w = w.view(r, -1, 32) * torch.pow(2.0, s["scales"].long()[at].double() - 127).unsqueeze(-1)
+        w = w.view(r, -1, 32) * _pow2(s["scales"].long()[at] - 127).unsqueeze(-1)
         y = _exact_mx(s["x"]) @ w.view(r, k).t()
         return y if s["b"] is None else y + s["b"].double()
     if op == "linear":
