@@ -168,6 +168,44 @@ TCB_API int tcb_decompress_sym(const int8_t* q, const uint16_t* scales, uint16_t
                                void* stream);
 
 /*
+ * Microscaled 4-bit floating point (MXFP4): blocks of 32 values of a row, E2M1 codes, one
+ * power-of-two scale byte (E8M0) per block.  No counterpart in the reference.
+ *   byte  = max(fp32 exponent field of the block's max|x| - 2, 0); the scale is 2^(byte - 127)
+ *   code  = E2M1 nearest to x / scale, ties to even, magnitudes above 6 become 6;
+ *           values that are not finite count as 0 (as in the int8 codecs)
+ *   x       [rows, cols] of `dtype`       codes  [rows, cols / 2], element 2i in the low half
+ *   scales  [ceil(rows / 128) * ceil(cols / 128) * 512] bytes, tiles of 128 rows x 4 blocks:
+ *           block b of row r is byte (r / 128 * ceil(cols / 128) + b / 4) * 512
+ *                                    + r % 32 * 16 + r % 128 / 32 * 4 + b % 4;
+ *           padding is written as 0
+ *   out     [rows, cols] bf16 bits = code * scale, exact; a scale byte of 255 decodes to NaN
+ * cols must be a multiple of 32; all arrays 16-byte aligned.
+ */
+TCB_API int tcb_quantize_mxfp4(const void* x, int dtype, int64_t rows, int64_t cols, uint8_t* codes, uint8_t* scales,
+                               void* stream);
+TCB_API int tcb_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, uint16_t* out,
+                                 void* stream);
+
+/*
+ * Rows of a device-resident cache of symmetric int8 codes, quantised as they are written and
+ * decoded as they are read (the device counterpart of FeatureCacheWriter.append,
+ * src/tensorcache/feature_cache.py:342-424, and of the row gather of
+ * FeatureCacheDataset.iter_batches, feature_cache.py:1018-1078).  Codes, scales and decoded
+ * bits are those of tcb_compress_sym (n_cand == 0) and tcb_decompress_sym of the row.
+ *   codes   [num_rows, width]                scales  [num_rows, width / G] bf16 bits
+ *   indices [n] device array; row t of x / out belongs to cache row indices[t].  An index
+ *           outside [0, num_rows) leaves the cache alone (write) or yields zeros (read).
+ *           An index that occurs more than once in one write: the last occurrence stays.
+ *   claims  [num_rows + 1] device array of the cache, zeroed once when the cache is made
+ * width must be a multiple of G (8, 16, 24, 32, 48, 64 or 128); x, out and codes 16-byte
+ * aligned; n < 2^31.  Writes to one cache must be ordered by the caller (one stream).
+ */
+TCB_API int tcb_cache_write(const void* x, int dtype, const int64_t* indices, int64_t n, int8_t* codes, uint16_t* scales,
+                            int64_t num_rows, int64_t width, int group_size, int64_t* claims, void* stream);
+TCB_API int tcb_cache_read(const int8_t* codes, const uint16_t* scales, int64_t num_rows, int64_t width, int group_size,
+                           const int64_t* indices, int64_t n, uint16_t* out, void* stream);
+
+/*
  * Fused dequantise + GEMM on the tcgen05 tensor cores:
  *     out[m, n] = bf16( sum_k dense[m, k] * deq(q)[n, k]  + bias )
  * with deq(q)[n, k] = (q[n, k] - zp[n, k / G]) * scale[n, k / G]   (zp != NULL, uint8 codes)

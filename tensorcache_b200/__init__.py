@@ -11,8 +11,10 @@ compute calls raise.
 """
 from .codec import (AMO_BQ_PRESETS, BlockwiseInt8Codec, dequantize_int8_amo_bq, dequantize_int8_g32,
                     quantize_int8_adaptive, quantize_int8_amo_bq, quantize_int8_g32)
+from .device_cache import DeviceFeatureCache
 from .feature_cache import FeatureCacheDataset, FeatureCacheWriter
 from .fused_linear import FusedDequantLinear, fused_dequant_matmul
+from .mxfp4 import dequantize_mxfp4, mxfp4_scales_from_rows, mxfp4_scales_to_rows, quantize_mxfp4
 from .streamer import ZeroCopyTensorStreamer
 from .utils import auto_select_mode, benchmark_tensor, compress, decompress, estimate_compression, selftest_sum_order
 
@@ -22,5 +24,6 @@ __all__ = [
     "quantize_int8_g32", "quantize_int8_adaptive", "dequantize_int8_g32",
     "compress", "decompress", "estimate_compression", "benchmark_tensor", "auto_select_mode", "selftest_sum_order",
     "FusedDequantLinear", "fused_dequant_matmul",
-    "FeatureCacheWriter", "FeatureCacheDataset", "ZeroCopyTensorStreamer",
+    "quantize_mxfp4", "dequantize_mxfp4", "mxfp4_scales_to_rows", "mxfp4_scales_from_rows",
+    "DeviceFeatureCache", "FeatureCacheWriter", "FeatureCacheDataset", "ZeroCopyTensorStreamer",
 ]

@@ -31,6 +31,8 @@ SOURCES = [
     ("streamer.cpp", []),
     ("fused_linear.cu", []),
     ("noalloc.cu", []),
+    ("mxfp4.cu", []),
+    ("row_cache.cu", []),
 ]
 
 

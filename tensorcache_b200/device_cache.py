@@ -1,0 +1,116 @@
+"""``DeviceFeatureCache``: feature rows kept in GPU memory as symmetric int8 codes.
+
+The device-resident counterpart of ``FeatureCacheWriter`` / ``FeatureCacheDataset``: rows are quantised as
+they are written and decoded as they are read, at any row index, with the codec of ``quantize_int8_g32``
+(codes, bf16 scales and decoded values have its bits).  A row takes ``1 + 2 / group_size`` bytes a value, so a
+180 GB GPU holds about twice the rows that bf16 would.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+from .codec import _DTYPES, _check_group_size, _ptr
+from .fused_linear import _aligned
+
+Indices = Union[torch.Tensor, Sequence[int]]
+
+
+class DeviceFeatureCache:
+    """``num_rows`` rows of ``row_shape`` values (an int, or a tuple such as ``(seq_len, dim)``) on one GPU.
+
+    ``codes`` (int8 ``[num_rows, width]``) and ``scales`` (bf16 ``[num_rows, width / group_size]``) are plain
+    tensors that start as zeros; rows that were never written read as zeros.  The number of values of a row must be
+    a multiple of ``group_size``.
+
+    Calls only enqueue work on the current stream of the cache's device (index tensors on the GPU are not looked
+    at by the host), so they can be captured in a CUDA graph.  As with any tensor, calls on different streams need
+    an order from the caller.
+    """
+
+    def __init__(self, num_rows: int, row_shape: Union[int, Tuple[int, ...]], group_size: int = 32,
+                 device: Optional[Union[str, torch.device]] = None):
+        _check_group_size(group_size)
+        self.row_shape = (int(row_shape),) if isinstance(row_shape, int) else tuple(int(v) for v in row_shape)
+        if num_rows < 0 or any(v < 0 for v in self.row_shape):
+            raise ValueError(f"negative size: {num_rows} rows of {self.row_shape}")
+        self.num_rows, self.group_size = int(num_rows), group_size
+        self.width = math.prod(self.row_shape)
+        if self.width % group_size != 0:
+            raise ValueError(f"{self.width} values a row is not a multiple of the group size {group_size}")
+        if not torch.cuda.is_available():
+            raise RuntimeError("DeviceFeatureCache keeps its rows on a CUDA device (no CPU fallback) and none is available")
+        dev = torch.device("cuda" if device is None else device)
+        if dev.type != "cuda":
+            raise ValueError(f"DeviceFeatureCache keeps its rows on a CUDA device, got {dev}")
+        self.device = torch.device("cuda", torch.cuda.current_device() if dev.index is None else dev.index)
+        self.codes = torch.zeros((self.num_rows, self.width), dtype=torch.int8, device=self.device)
+        self.scales = torch.zeros((self.num_rows, self.width // group_size), dtype=torch.bfloat16, device=self.device)
+        # per row: which call wrote it last and from where in the call's list (settles an index that occurs twice);
+        # the last word counts calls
+        self._claims = torch.zeros(self.num_rows + 1, dtype=torch.int64, device=self.device)
+
+    def __len__(self) -> int:
+        return self.num_rows
+
+    def __repr__(self):
+        return f"DeviceFeatureCache({self.num_rows} x {self.row_shape}, G={self.group_size}, {self.device})"
+
+    def _indices(self, indices: Indices) -> torch.Tensor:
+        idx = torch.as_tensor(indices)
+        if idx.numel() == 0:
+            idx = idx.long()
+        if idx.dim() != 1 or idx.dtype not in (torch.int64, torch.int32):
+            raise ValueError(f"indices must be one-dimensional int64 or int32, got {tuple(idx.shape)} of {idx.dtype}")
+        if idx.is_cuda:
+            if idx.device != self.device:
+                raise ValueError(f"indices are on {idx.device}, the cache is on {self.device}")
+        elif idx.numel() and int(idx.max()) >= self.num_rows:
+            raise IndexError(f"row {int(idx.max())} in a cache of {self.num_rows} rows")
+        return idx.to(device=self.device, dtype=torch.int64).contiguous()
+
+    def write(self, indices: Indices, x: torch.Tensor) -> None:
+        """Quantises row ``t`` of ``x`` (``[n, *row_shape]`` or ``[n, width]``) into row ``indices[t]``.
+
+        A negative index leaves its row out (padding); so does, in an index tensor on the GPU, one past the end --
+        given on the host that raises ``IndexError``.  Of an index that occurs more than once the last occurrence stays.  Values that are
+        not finite are stored as 0.  bf16, fp16 and fp32 are read as they are, other types are converted to fp32.
+        """
+        with torch.cuda.device(self.device):
+            idx = self._indices(indices)
+            n = idx.numel()
+            if tuple(x.shape) not in ((n, *self.row_shape), (n, self.width)):
+                raise ValueError(f"expected {n} rows of {self.row_shape}, got {tuple(x.shape)}")
+            if x.is_cuda and x.device != self.device:
+                raise ValueError(f"x is on {x.device}, the cache is on {self.device}")
+            if x.dtype not in _DTYPES:
+                x = x.float()
+            xd = _aligned(x.detach().to(self.device).reshape(n, self.width).contiguous())
+            stream = ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+            _lib.check(_lib.lib().tcb_cache_write(_ptr(xd), _DTYPES[xd.dtype], _ptr(idx), n, _ptr(self.codes), _ptr(self.scales),
+                                                  self.num_rows, self.width, self.group_size, _ptr(self._claims), stream))
+
+    def read(self, indices: Indices, out_buffer: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """bf16 ``[n, *row_shape]``: row ``indices[t]`` decoded; a row that ``write`` would leave out is zeros.
+        If ``out_buffer`` is given it is written in place and returned."""
+        with torch.cuda.device(self.device):
+            idx = self._indices(indices)
+            n = idx.numel()
+            if out_buffer is None:
+                out_buffer = torch.empty((n, *self.row_shape), dtype=torch.bfloat16, device=self.device)
+            if out_buffer.numel() != n * self.width or out_buffer.dtype != torch.bfloat16:
+                raise ValueError(f"out_buffer must be a bf16 tensor of {n} rows of {self.width} values")
+            if out_buffer.numel() == 0:
+                return out_buffer
+            direct = out_buffer.device == self.device and out_buffer.is_contiguous() and out_buffer.data_ptr() % 16 == 0
+            od = out_buffer if direct else torch.empty(n * self.width, dtype=torch.bfloat16, device=self.device)
+            stream = ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+            _lib.check(_lib.lib().tcb_cache_read(_ptr(self.codes), _ptr(self.scales), self.num_rows, self.width, self.group_size,
+                                                 _ptr(idx), n, _ptr(od), stream))
+            if not direct:
+                out_buffer.copy_(od.view(out_buffer.shape))
+        return out_buffer

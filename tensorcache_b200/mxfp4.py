@@ -1,0 +1,125 @@
+"""Microscaled 4-bit floating point (MXFP4): codec and matrix product.
+
+Blocks of 32 values along the last dimension, E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+negatives) and one power-of-two scale byte per block: 4.25 bits a value, a quarter of bf16.  The 8-bit
+codecs next door (``compress`` / ``decompress``) have no 4-bit counterpart in the reference that keeps its
+scales as powers of two, so there is nothing to mirror here; argument checks, staging of CPU tensors and
+errors follow ``codec.py``.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .codec import _DTYPES, _compute_device, _ptr
+from .fused_linear import _aligned
+
+BLOCK = 32          # values that share a scale
+_TILE_ROWS = 128    # a scale tile covers 128 rows x 4 blocks
+_TILE_BLOCKS = 4
+
+
+def _rows_cols(shape) -> Tuple[int, int]:
+    if len(shape) == 0:
+        raise ValueError("MXFP4 blocks run along the last dimension: a 0-dimensional tensor has none")
+    cols = int(shape[-1])
+    if cols % BLOCK != 0:
+        raise ValueError(f"the last dimension ({cols}) must be a multiple of {BLOCK}")
+    return math.prod(shape[:-1]), cols
+
+
+def mxfp4_scale_bytes(rows: int, cols: int) -> int:
+    """Number of scale bytes of a ``[rows, cols]`` tensor: whole tiles of 128 rows x 128 values."""
+    return -(-rows // _TILE_ROWS) * -(-cols // (BLOCK * _TILE_BLOCKS)) * 512
+
+
+def mxfp4_scales_to_rows(scales: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """Scale bytes in tile order -> uint8 ``[rows, cols / 32]`` (one row of scales per row of codes)."""
+    _rows_cols((rows, cols))
+    if scales.dtype != torch.uint8 or scales.numel() != mxfp4_scale_bytes(rows, cols):
+        raise ValueError(f"expected {mxfp4_scale_bytes(rows, cols)} uint8 scales, got {scales.numel()} of {scales.dtype}")
+    tr, tk = -(-rows // _TILE_ROWS), -(-cols // (BLOCK * _TILE_BLOCKS))
+    t = scales.reshape(tr, tk, 32, 4, _TILE_BLOCKS).permute(0, 3, 2, 1, 4)
+    return t.reshape(tr * _TILE_ROWS, tk * _TILE_BLOCKS)[:rows, :cols // BLOCK].contiguous()
+
+
+def mxfp4_scales_from_rows(row_scales: torch.Tensor) -> torch.Tensor:
+    """uint8 ``[rows, cols / 32]`` -> scale bytes in the tile order the kernels read (padding 0)."""
+    if row_scales.dim() != 2 or row_scales.dtype != torch.uint8:
+        raise ValueError("row scales are a uint8 tensor [rows, cols / 32]")
+    rows, blocks = row_scales.shape
+    tr, tk = -(-rows // _TILE_ROWS), -(-blocks // _TILE_BLOCKS)
+    t = torch.zeros((tr * _TILE_ROWS, tk * _TILE_BLOCKS), dtype=torch.uint8, device=row_scales.device)
+    t[:rows, :blocks] = row_scales
+    return t.view(tr, 4, 32, tk, _TILE_BLOCKS).permute(0, 3, 2, 1, 4).reshape(-1)
+
+
+def _quantize_on_device(x2: torch.Tensor, rows: int, cols: int):
+    """Contiguous CUDA ``[rows, cols]`` -> codes ``[rows, cols / 2]`` and scales, on the current device."""
+    codes = torch.empty((rows, cols // 2), dtype=torch.uint8, device=x2.device)
+    scales = torch.empty(mxfp4_scale_bytes(rows, cols), dtype=torch.uint8, device=x2.device)
+    if codes.numel():
+        x2 = _aligned(x2)
+        stream = ctypes.c_void_p(torch.cuda.current_stream(x2.device).cuda_stream)
+        _lib.check(_lib.lib().tcb_quantize_mxfp4(_ptr(x2), _DTYPES[x2.dtype], rows, cols, _ptr(codes), _ptr(scales), stream))
+    return codes, scales
+
+
+def quantize_mxfp4(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, Tuple[int, ...]]:
+    """Encode -> ``(codes uint8 [..., K / 2], scales uint8 [...], orig_shape)`` on ``x.device``.
+
+    The last dimension K is a multiple of 32.  Element 2i of a row is the low half of byte i; the scales
+    are in tile order (``mxfp4_scales_to_rows`` gives them per row).  A block's scale is
+    ``2^(floor(log2 max|x|) - 2)``, codes round to nearest even and saturate at 6, values that are not
+    finite become 0.  Inputs other than bf16, fp16 and fp32 are converted to fp32.  For CUDA inputs nothing
+    synchronises with the host, so the call can be captured in a CUDA graph.
+    """
+    rows, cols = _rows_cols(x.shape)
+    if x.dtype not in _DTYPES:
+        x = x.float()
+    dev = _compute_device(x)
+    with torch.cuda.device(dev):
+        codes, scales = _quantize_on_device(x.detach().reshape(rows, cols).contiguous().to(dev), rows, cols)
+    codes = codes.view(*x.shape[:-1], cols // 2)
+    if not x.is_cuda:
+        codes, scales = codes.cpu(), scales.cpu()
+    return codes, scales, x.shape
+
+
+def _check_codes(codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int) -> None:
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError("MXFP4 operands are uint8 codes with uint8 scales")
+    if codes.numel() * 2 != rows * cols:
+        raise ValueError(f"expected {rows * cols // 2} bytes of codes for [{rows}, {cols}], got {codes.numel()}")
+    if scales.numel() != mxfp4_scale_bytes(rows, cols):
+        raise ValueError(f"expected {mxfp4_scale_bytes(rows, cols)} scales in tile order for [{rows}, {cols}], got {scales.numel()}")
+    if codes.device != scales.device:
+        raise ValueError(f"codes and scales are on different devices ({codes.device}, {scales.device})")
+
+
+def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, orig_shape: Tuple[int, ...],
+                     out_buffer: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Decode to bf16 of ``orig_shape`` (exact: a code has two significant bits).  If ``out_buffer`` is given
+    it is written in place and returned.  A scale byte of 255 decodes to NaN."""
+    rows, cols = _rows_cols(orig_shape)
+    _check_codes(codes, scales, rows, cols)
+    dev = _compute_device(codes)
+    if out_buffer is None:
+        out_buffer = torch.empty(tuple(orig_shape), dtype=torch.bfloat16, device=codes.device)
+    if out_buffer.numel() != rows * cols or out_buffer.dtype != torch.bfloat16:
+        raise ValueError("out_buffer must be a bf16 tensor of the decoded size")
+    if out_buffer.numel() == 0:
+        return out_buffer
+    with torch.cuda.device(dev):
+        cd, sd = _aligned(codes.contiguous().to(dev)), _aligned(scales.contiguous().to(dev))
+        direct = out_buffer.device == dev and out_buffer.is_contiguous() and out_buffer.data_ptr() % 16 == 0
+        od = out_buffer if direct else torch.empty(rows * cols, dtype=torch.bfloat16, device=dev)
+        stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+        _lib.check(_lib.lib().tcb_dequantize_mxfp4(_ptr(cd), _ptr(sd), rows, cols, _ptr(od), stream))
+        if not direct:
+            out_buffer.copy_(od.view(out_buffer.shape))
+    return out_buffer

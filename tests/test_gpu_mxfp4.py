@@ -1,0 +1,130 @@
+"""MXFP4 codec against a 64-bit restatement.  Codes, scale bytes and decoded bf16 values are compared exactly: the
+scale is a power of two, so the quotient and the decoded product have no rounding but the one to the E2M1 grid."""
+import pytest
+import torch
+
+import tensorcache_b200 as tc
+from tests import low_bit_plain as plain
+from tests import synth
+from tests.util import bits
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def check_codec(x):
+    """Codes, scales, padding and decoded values of a 2-D tensor."""
+    rows, cols = x.shape
+    codes, scales, shape = tc.quantize_mxfp4(x)
+    assert codes.shape == (rows, cols // 2) and codes.dtype == torch.uint8 and tuple(shape) == (rows, cols)
+    ref_code, ref_byte = plain.mx_encode(x)
+    assert torch.equal(codes, plain.mx_pack(ref_code))
+    per_row = tc.mxfp4_scales_to_rows(scales, rows, cols)
+    assert torch.equal(per_row.long(), ref_byte)
+    assert torch.equal(tc.mxfp4_scales_from_rows(per_row), scales)      # padding is 0
+    out = tc.dequantize_mxfp4(codes, scales, shape)
+    assert out.dtype == torch.bfloat16 and out.shape == x.shape
+    assert torch.equal(out.double(), plain.mx_values(ref_code, ref_byte))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 32), (1, 4096), (3, 96), (127, 128), (128, 160), (129, 992), (446, 768), (1000, 4128)])
+def test_codec_matches_the_restatement(rows, cols, dtype):
+    g = torch.Generator(device=DEV).manual_seed(rows + cols)
+    x = torch.randn(rows, cols, generator=g, device=DEV) * torch.exp(2 * torch.randn(rows, 1, generator=g, device=DEV))
+    check_codec(x.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_grid_point_tie_and_neighbour(dtype):
+    """All E2M1 values, the midpoints between them and values just beside both, in blocks whose maximum pins the scale."""
+    mid = (plain.GRID[1:] + plain.GRID[:-1]) / 2
+    base = torch.cat([plain.GRID, mid, torch.tensor([6.5, 7.0, 7.5], dtype=torch.float64)])
+    eps = 2.0 ** (-7 if dtype == torch.bfloat16 else -10)
+    v = torch.cat([base, base * (1 + eps), base * (1 - eps)])
+    v = torch.cat([v, -v])
+    v = v[v.abs() < 8]
+    blocks = v[:v.numel() // 31 * 31].view(-1, 31)
+    x = torch.cat([torch.full((blocks.shape[0], 1), 4.0, dtype=torch.float64), blocks], 1)   # max in [4, 8): scale 1
+    for scale in (1.0, 2.0 ** -9, 2.0 ** 8):
+        check_codec((x * scale).to(dtype).to(DEV))
+
+
+def test_extremes_of_the_exponent_and_values_that_are_not_finite():
+    x = synth.edge_values().view(8, 512).clone()
+    x[7, :32] = torch.tensor([float("nan"), float("inf"), float("-inf"), 5.0] * 8)
+    x[7, 32:64] = 3.4028e38
+    x[7, 64:96] = 1.1754944e-38     # smallest normal fp32
+    x[7, 96:128] = 1e-45            # smallest subnormal
+    x[7, 128:160] = -0.0
+    check_codec(x.to(DEV))
+    check_codec(x.to(torch.bfloat16).to(DEV))
+    check_codec(x.to(torch.float16).to(DEV))
+
+
+def test_all_codes_and_scale_bytes_decode():
+    """Every scale byte (as another program may have written them) with every code."""
+    code = torch.arange(16, device=DEV).repeat(256, 2)
+    byte = torch.arange(256, device=DEV).view(256, 1)
+    out = tc.dequantize_mxfp4(plain.mx_pack(code), tc.mxfp4_scales_from_rows(byte.to(torch.uint8)), (256, 32))
+    ref = plain.mx_values(code, byte).to(torch.bfloat16)
+    assert bool(out[255].isnan().all())
+    assert torch.equal(out[:255].float(), ref[:255].float())
+
+
+def test_leading_dimensions_strides_alignment_buffers_and_host_tensors():
+    x = synth.config0_style(3, (3, 5, 64)).to(DEV)
+    codes, scales, shape = tc.quantize_mxfp4(x)
+    assert codes.shape == (3, 5, 32) and tuple(shape) == (3, 5, 64)
+    ref = tc.dequantize_mxfp4(codes, scales, shape)
+    wide = torch.zeros(3, 5, 200, dtype=torch.bfloat16, device=DEV)
+    wide[..., 7:71] = x
+    for view in (wide[..., 7:71], x.transpose(0, 1).contiguous().transpose(0, 1)):
+        c2, s2, _ = tc.quantize_mxfp4(view)
+        assert torch.equal(c2, codes) and torch.equal(s2, scales)
+    odd = torch.empty(15 * 64 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(3, 5, 64)     # 2-byte aligned
+    odd.copy_(x)
+    c2, s2, _ = tc.quantize_mxfp4(odd)
+    assert torch.equal(c2, codes) and torch.equal(s2, scales)
+    buf = torch.full((15 * 64 + 8,), 7.0, dtype=torch.bfloat16, device=DEV)
+    assert tc.dequantize_mxfp4(codes, scales, shape, out_buffer=buf[1:961].view(3, 5, 64)) is not None
+    assert torch.equal(buf[1:961].view(3, 5, 64), ref) and bool((buf[961:] == 7).all()) and float(buf[0]) == 7
+    cc, cs, _ = tc.quantize_mxfp4(x.cpu())
+    assert not cc.is_cuda and torch.equal(cc, codes.cpu()) and torch.equal(cs, scales.cpu())
+    assert (bits(tc.dequantize_mxfp4(cc, cs, shape)) == bits(ref)).all()
+    c64, s64, _ = tc.quantize_mxfp4(x.double())
+    assert torch.equal(c64, codes) and torch.equal(s64, scales)
+
+
+def test_empty_tensors():
+    for shape in ((0, 64), (4, 0), (0,), (2, 0, 32)):
+        codes, scales, s = tc.quantize_mxfp4(torch.empty(shape, device=DEV))
+        assert codes.numel() == 0 and tc.dequantize_mxfp4(codes, scales, s).shape == shape
+
+
+def test_capture_and_replay_on_another_stream():
+    x = torch.randn(200, 96, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        tc.dequantize_mxfp4(*tc.quantize_mxfp4(x))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = tc.dequantize_mxfp4(*tc.quantize_mxfp4(x))
+    for seed in (1, 2):
+        x.copy_(torch.randn(200, 96, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV))
+        graph.replay()
+        assert torch.equal(out.double(), plain.mx_values(*plain.mx_encode(x)))
+
+
+def test_more_than_2_31_values():
+    rows, cols = (1 << 20) + 3, 2080
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device=DEV)
+    tail = torch.randn(131, cols, device=DEV).to(torch.bfloat16)
+    x[-131:] = tail
+    codes, scales, shape = tc.quantize_mxfp4(x)
+    out = tc.dequantize_mxfp4(codes, scales, shape)
+    assert torch.equal(out[-131:].double(), plain.mx_values(*plain.mx_encode(tail)))
+    assert not bool(out[:1000].any()) and not bool(codes[:-131].any())
