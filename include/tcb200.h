@@ -228,8 +228,33 @@ TCB_API int tcb_fused_dequant_linear(const uint16_t* dense, const uint8_t* q, co
                              int64_t R_d, int64_t R_q, int64_t K, int group_size, int quant_is_rhs,
                              void* stream);
 
-/* Reads (and clears) the per-device status word the fused GEMM writes when a
- * bounded wait runs out.  Synchronises `stream`.  Returns TCB_OK or TCB_ERR_TIMEOUT. */
+/*
+ * Training step of a linear layer whose input is kept as 8-bit codes (tcgen05; fp32 sums, bf16
+ * results).  The reference's FusedDequantLinear has no backward pass.
+ *   forward      y  [M, N] = x [M, K] . w [N, K]^T (+ bias [N])
+ *   grad_input   dx [M, K] = dy [M, N] . w [N, K]
+ *   grad_weight  dw [N, K] = dy [M, N]^T . deq(q) [M, K]       db [N] = column sums of dy
+ * deq(q) is the bf16 number tcb_decompress_amo / tcb_decompress_sym gives for the codes
+ * (zp != NULL: uint8 codes, else signed).  Either of dw and db may be NULL.  All bf16.
+ *   ld_dy      elements between rows of dy: a multiple of 8, at least N
+ *   workspace  tcb_linear_workspace(M, N, K) bytes on the current device, 32-byte aligned,
+ *              enough for any of the three; used by the call's own work on `stream` only
+ * Requirements: K a positive multiple of 8 (forward, grad_input) or of G in {16, 32, 64, 128}
+ * (grad_weight); x, w, dy and q 16-byte aligned; M, N arbitrary.  With M == 0 or N == 0 nothing
+ * is written.  A contraction that is split over the GPU is added up in a fixed order.
+ */
+TCB_API int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K);
+TCB_API int tcb_linear_forward(const uint16_t* x, const uint16_t* w, const uint16_t* bias_or_null, uint16_t* y, int64_t M,
+                               int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+TCB_API int tcb_linear_grad_input(const uint16_t* dy, int64_t ld_dy, const uint16_t* w, uint16_t* dx, int64_t M, int64_t N,
+                                  int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+TCB_API int tcb_linear_grad_weight(const uint16_t* dy, int64_t ld_dy, const uint8_t* q, const uint16_t* scales,
+                                   const uint8_t* zp_or_null, uint16_t* dw_or_null, uint16_t* db_or_null, int64_t M,
+                                   int64_t N, int64_t K, int group_size, void* workspace, int64_t workspace_bytes,
+                                   void* stream);
+
+/* Reads (and clears) the per-device status words the fused GEMM and the tcb_linear_*
+ * kernels write when a bounded wait runs out.  Synchronises `stream`.  Returns TCB_OK or TCB_ERR_TIMEOUT. */
 TCB_API int tcb_fused_dequant_linear_check(void* stream);
 
 /* Launches a tiny kernel whose only work is a bounded wait on a barrier that nothing

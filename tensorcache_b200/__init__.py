@@ -9,6 +9,7 @@ Drop-in for the reference's API on that path -- ``compress`` / ``decompress``,
 and no CPU implementation: without the built library or a CUDA device the
 compute calls raise.
 """
+from .checkpoint import Int8CheckpointLinear, fused_dequant_linear, int8_checkpoint_linear
 from .codec import (AMO_BQ_PRESETS, BlockwiseInt8Codec, dequantize_int8_amo_bq, dequantize_int8_g32,
                     quantize_int8_adaptive, quantize_int8_amo_bq, quantize_int8_g32)
 from .device_cache import DeviceFeatureCache
@@ -24,6 +25,7 @@ __all__ = [
     "quantize_int8_g32", "quantize_int8_adaptive", "dequantize_int8_g32",
     "compress", "decompress", "estimate_compression", "benchmark_tensor", "auto_select_mode", "selftest_sum_order",
     "FusedDequantLinear", "fused_dequant_matmul",
+    "fused_dequant_linear", "int8_checkpoint_linear", "Int8CheckpointLinear",
     "quantize_mxfp4", "dequantize_mxfp4", "mxfp4_scales_to_rows", "mxfp4_scales_from_rows",
     "DeviceFeatureCache", "FeatureCacheWriter", "FeatureCacheDataset", "ZeroCopyTensorStreamer",
 ]

@@ -63,6 +63,10 @@ SIGNATURES = {
     "tcb_cache_write": (_i32, [_vp, _i32, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp, _vp]),
     "tcb_cache_read": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp]),
     "tcb_fused_dequant_linear": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
+    "tcb_linear_workspace": (_i64, [_i64, _i64, _i64]),
+    "tcb_linear_forward": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "tcb_linear_grad_input": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "tcb_linear_grad_weight": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
     "tcb_fused_dequant_linear_check": (_i32, [_vp]),
     "tcb_selftest_bounded_wait": (_i32, [_i32, _vp]),
     "tcb_gather_rows": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64, _i32]),

@@ -31,6 +31,7 @@ SOURCES = [
     ("streamer.cpp", []),
     ("fused_linear.cu", []),
     ("noalloc.cu", []),
+    ("linear_train.cu", []),
     ("mxfp4.cu", []),
     ("row_cache.cu", []),
 ]

@@ -1,0 +1,208 @@
+"""Linear layers that train with their input kept in 8 bits.
+
+* ``int8_checkpoint_linear(x, weight, bias)`` / ``Int8CheckpointLinear``: ``x @ weight.T + bias`` whose graph
+  keeps ``quantize_int8_g32(x)`` instead of ``x`` (``1 + 2 / group_size`` bytes a value instead of 2).
+* ``fused_dequant_linear(q, scales, weight, bias, zero_points)``: the product of ``FusedDequantLinear`` on codes
+  that come out of a feature cache, differentiable in ``weight`` and ``bias``.
+
+The weight gradient is computed from the codes: the kernel decodes them in shared memory, so the bf16 input never
+exists again.  Products run on the tensor cores with fp32 sums and one rounding to bf16; a long sum over few output
+tiles is split over the GPU and added in a fixed order, so results do not change from run to run.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .codec import _ptr, quantize_int8_g32
+from .fused_linear import SUPPORTED_GROUP_SIZES, _aligned, _check_common, _launch
+
+
+def _check_dense(name: str, t: torch.Tensor, device: torch.device) -> None:
+    if t.dtype != torch.bfloat16:
+        raise ValueError(f"{name} must be bf16, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the input is on {device}")
+
+
+def _check_layer(weight: torch.Tensor, bias: Optional[torch.Tensor], K: int, device: torch.device) -> None:
+    if weight.dim() != 2 or weight.shape[1] != K:
+        raise ValueError(f"weight must be [out_features, {K}], got {tuple(weight.shape)}")
+    _check_dense("weight", weight, device)
+    if bias is not None:
+        if tuple(bias.shape) != (weight.shape[0],):
+            raise ValueError(f"bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
+        _check_dense("bias", bias, device)
+
+
+def _operand(t: torch.Tensor) -> torch.Tensor:
+    return _aligned(t.detach().contiguous())
+
+
+class _Workspace:
+    """Scratch of one call's kernels (split sums), from the caching allocator of the current stream."""
+
+    def __init__(self, M: int, N: int, K: int, device: torch.device):
+        self.bytes = _lib.lib().tcb_linear_workspace(M, N, K)
+        self.buffer = torch.empty(self.bytes, dtype=torch.uint8, device=device)
+
+    def args(self):
+        return _ptr(self.buffer), self.bytes
+
+
+def _dy_operand(dy: torch.Tensor):
+    """``[M, N]`` contiguous, 16-byte aligned, with rows a multiple of 8 elements apart (a copy only if N is not)."""
+    N = dy.shape[1]
+    if N % 8 == 0:
+        return _operand(dy), N
+    ld = -(-N // 8) * 8
+    padded = torch.zeros((dy.shape[0], ld), dtype=dy.dtype, device=dy.device)
+    padded[:, :N] = dy
+    return padded, ld
+
+
+def _grad_weight(dy: torch.Tensor, ld: int, q: Optional[torch.Tensor], scales: Optional[torch.Tensor], zp: Optional[torch.Tensor],
+                 sizes, group_size: int, need_dw: bool, need_db: bool, ws: _Workspace, stream):
+    """``(dw or None, db or None)`` from a padded ``dy`` and the kept codes."""
+    M, N, K = sizes
+    make = torch.empty if M else torch.zeros
+    dw = make((N, K), dtype=torch.bfloat16, device=dy.device) if need_dw else None
+    db = make(N, dtype=torch.bfloat16, device=dy.device) if need_db else None
+    if M and N and (need_dw or need_db):
+        _lib.check(_lib.lib().tcb_linear_grad_weight(_ptr(dy), ld, _ptr(q), _ptr(scales), _ptr(zp), _ptr(dw), _ptr(db), M, N, K,
+                                                     group_size, *ws.args(), stream))
+    return dw, db
+
+
+class _CheckpointLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, group_size):
+        N, K = weight.shape
+        x2 = _operand(x.reshape(-1, K))
+        M = x2.shape[0]
+        y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+        q = scales = None
+        with torch.cuda.device(x.device):
+            if M and N:
+                w, b = _operand(weight), None if bias is None else bias.detach().contiguous()
+                ws = _Workspace(M, N, K, x.device)
+                stream = ctypes.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)
+                _lib.check(_lib.lib().tcb_linear_forward(_ptr(x2), _ptr(w), _ptr(b), _ptr(y), M, N, K, *ws.args(), stream))
+            if ctx.needs_input_grad[1]:
+                q, scales, _ = quantize_int8_g32(x2, group_size)
+        ctx.save_for_backward(q, scales, weight if ctx.needs_input_grad[0] else None)
+        ctx.x_shape, ctx.sizes, ctx.group_size = x.shape, (M, N, K), group_size
+        return y.view(*x.shape[:-1], N)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        q, scales, weight = ctx.saved_tensors
+        (M, N, K), dev = ctx.sizes, dy.device
+        need_dx, need_dw, need_db, _ = ctx.needs_input_grad
+        dx = None
+        with torch.cuda.device(dev):
+            dy2, ld = _dy_operand(dy.reshape(M, N))
+            ws = _Workspace(M, N, K, dev)
+            stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+            if need_dx:
+                dx = (torch.empty if N else torch.zeros)((M, K), dtype=torch.bfloat16, device=dev)
+                if M and N:
+                    w = _operand(weight)
+                    _lib.check(_lib.lib().tcb_linear_grad_input(_ptr(dy2), ld, _ptr(w), _ptr(dx), M, N, K, *ws.args(), stream))
+                dx = dx.view(ctx.x_shape)
+            dw, db = _grad_weight(dy2, ld, q, scales, None, ctx.sizes, ctx.group_size, need_dw, need_db, ws, stream)
+        return dx, dw, db, None
+
+
+class _FusedDequantLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, bias, q, scales, zp, group_size):
+        N, K = weight.shape
+        M = q.shape[0]
+        y = torch.empty((M, N), dtype=torch.bfloat16, device=q.device)
+        if M and N:
+            _launch(weight.detach().contiguous(), q, scales, zp, None if bias is None else bias.detach().contiguous(), y, N, M, K, group_size, False)
+        ctx.save_for_backward(q, scales, zp)
+        ctx.sizes, ctx.group_size = (M, N, K), group_size
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        q, scales, zp = ctx.saved_tensors
+        with torch.cuda.device(dy.device):
+            dy2, ld = _dy_operand(dy)
+            ws = _Workspace(*ctx.sizes, dy.device)
+            stream = ctypes.c_void_p(torch.cuda.current_stream(dy.device).cuda_stream)
+            dw, db = _grad_weight(dy2, ld, _aligned(q), scales, zp, ctx.sizes, ctx.group_size, ctx.needs_input_grad[0], ctx.needs_input_grad[1], ws, stream)
+        return dw, db, None, None, None, None
+
+
+def int8_checkpoint_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, group_size: int = 32) -> torch.Tensor:
+    """``x @ weight.T + bias`` (bf16 ``[..., K]`` -> ``[..., N]``) that keeps ``x`` in 8 bits for the backward pass.
+
+    The forward product and the gradients of ``x`` and ``bias`` use the bf16 values; the gradient of ``weight`` is
+    ``dy.T @ dequantize_int8_g32(quantize_int8_g32(x))``.  K is a multiple of ``group_size`` (16, 32, 64 or 128).
+    Values of ``x`` that are not finite enter the weight gradient as 0, as the codec stores them.  CUDA tensors
+    only; gradients of gradients are not available.  A training step can be captured in a CUDA graph under torch's own
+    condition: no eager graph of the same leaves is alive during the capture (``del`` the outputs of warm-up steps).
+    """
+    if x.dim() == 0 or weight.dim() != 2:
+        raise ValueError(f"x must be [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    K = x.shape[-1]
+    if group_size not in SUPPORTED_GROUP_SIZES:
+        raise ValueError(f"group_size {group_size} is not supported, choose from {SUPPORTED_GROUP_SIZES}")
+    if K <= 0 or K % group_size != 0:
+        raise ValueError(f"the inner dimension ({K}) must be a positive multiple of the group size {group_size}")
+    _check_dense("x", x, x.device)
+    _check_layer(weight, bias, K, x.device)
+    if not x.is_cuda:
+        raise RuntimeError("int8_checkpoint_linear runs on CUDA tensors only (no CPU fallback)")
+    return _CheckpointLinear.apply(x, weight, bias, group_size)
+
+
+def fused_dequant_linear(q: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                         zero_points: Optional[torch.Tensor] = None, group_size: int = 32) -> torch.Tensor:
+    """``dequant(q) @ weight.T + bias`` for codes ``[..., K]`` (int8, or uint8 with zero points), differentiable in
+    ``weight`` and ``bias``: ``dweight = dy.T @ dequant(q)``, straight from the codes.  The values are those of
+    ``FusedDequantLinear``, which has no gradient; K is a multiple of ``group_size`` (16, 32, 64 or 128)."""
+    if q.dim() == 0:
+        raise ValueError("q must be [..., K]")
+    K = q.shape[-1]
+    q2 = q.reshape(-1, K).contiguous() if K else q.reshape(0, 0)
+    _check_common(q2, scales, zero_points, K, q2.shape[0], group_size)
+    _check_layer(weight, bias, K, q.device)
+    for name, t in (("scales", scales), ("zero_points", zero_points)):
+        if t is not None and t.device != q.device:
+            raise ValueError(f"{name} is on {t.device}, q is on {q.device}")
+    y = _FusedDequantLinear.apply(weight, bias, q2, scales.contiguous().view(-1), None if zero_points is None else zero_points.contiguous().view(-1),
+                                  group_size)
+    return y.view(*q.shape[:-1], weight.shape[0])
+
+
+class Int8CheckpointLinear(nn.Module):
+    """``nn.Linear`` in bf16 whose input is kept in 8 bits between the forward and the backward pass."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, group_size: int = 32):
+        super().__init__()
+        self.in_features = in_features
+        self.out_features = out_features
+        self.group_size = group_size
+        self.weight = nn.Parameter(torch.empty((out_features, in_features), dtype=torch.bfloat16))
+        if bias:
+            self.bias = nn.Parameter(torch.empty(out_features, dtype=torch.bfloat16))
+        else:
+            self.register_parameter("bias", None)
+        nn.init.kaiming_uniform_(self.weight, a=math.sqrt(5))
+        if self.bias is not None:
+            nn.init.zeros_(self.bias)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return int8_checkpoint_linear(x, self.weight, self.bias, self.group_size)

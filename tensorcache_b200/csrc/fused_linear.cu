@@ -70,6 +70,10 @@
 
 #include "tcb_tcgen05.h"
 
+namespace tcb {
+int take_linear_status(int* status);
+}
+
 namespace {
 
 constexpr int kTileRows = 128;   // rows of each operand per CTA and tile
@@ -185,36 +189,6 @@ __device__ __forceinline__ void table_spill(uint8_t* dst, const TableRegs& c) {
     }
 #pragma unroll
     for (int v = 0; v < 4; ++v) reinterpret_cast<uint4*>(dst)[v] = make_uint4(m[4 * v], m[4 * v + 1], m[4 * v + 2], m[4 * v + 3]);
-}
-
-// 16 codes of one row -> 16 bf16 values, written as two 16-byte pieces of the 128-byte-swizzled operand row.
-// Per code: one byte permute (the byte into the mantissa of 2^15), one FMA, half a cvt.rn.bf16x2.f32.
-template <bool HAS_ZP>
-__device__ __forceinline__ void convert16(uint4 c, uint32_t sz_word, uint8_t* piece0, uint8_t* piece1) {
-    uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    const float scale = __uint_as_float(sz_word & 0xFFFF0000u);
-    float base;
-    if (HAS_ZP) {
-        base = __uint_as_float(__byte_perm(sz_word, 0x47000000u, 0x7604));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] ^= 0x80808080u;
-        base = __uint_as_float(0x47008000u);
-    }
-    const float cc = -__fmul_rn(base, scale);
-    const uint32_t magic = 0x47000000u;
-    uint32_t o[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float f0 = __fmaf_rn(__uint_as_float(__byte_perm(w[i], magic, 0x7604)), scale, cc);
-        const float f1 = __fmaf_rn(__uint_as_float(__byte_perm(w[i], magic, 0x7614)), scale, cc);
-        const float f2 = __fmaf_rn(__uint_as_float(__byte_perm(w[i], magic, 0x7624)), scale, cc);
-        const float f3 = __fmaf_rn(__uint_as_float(__byte_perm(w[i], magic, 0x7634)), scale, cc);
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[2 * i]) : "f"(f1), "f"(f0));
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[2 * i + 1]) : "f"(f3), "f"(f2));
-    }
-    *reinterpret_cast<uint4*>(piece0) = make_uint4(o[0], o[1], o[2], o[3]);
-    *reinterpret_cast<uint4*>(piece1) = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
 struct Tile {
@@ -657,11 +631,16 @@ extern "C" int tcb_selftest_bounded_wait(int budget_ms, void* stream) {
 
 extern "C" int tcb_fused_dequant_linear_check(void* stream) {
     TCB_CUDA_TRY(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
-    int status = 0;
+    int status = 0, linear = 0;
+    const int rc = tcb::take_linear_status(&linear);
+    if (rc != TCB_OK) return rc;
     TCB_CUDA_TRY(cudaMemcpyFromSymbol(&status, g_status, sizeof(int)));
-    if (status == 0) return TCB_OK;
-    const int zero = 0;
-    TCB_CUDA_TRY(cudaMemcpyToSymbol(g_status, &zero, sizeof(int)));
-    return tcb::fail(TCB_ERR_TIMEOUT, "tcb_fused_dequant_linear: a bounded wait ran out (role %d, barrier %d)", status >> 8, status & 0xff);
+    if (status != 0) {
+        const int zero = 0;
+        TCB_CUDA_TRY(cudaMemcpyToSymbol(g_status, &zero, sizeof(int)));
+        return tcb::fail(TCB_ERR_TIMEOUT, "tcb_fused_dequant_linear: a bounded wait ran out (role %d, barrier %d)", status >> 8, status & 0xff);
+    }
+    if (linear != 0)
+        return tcb::fail(TCB_ERR_TIMEOUT, "tcb_linear_*: a bounded wait ran out (role %d, barrier %d)", linear >> 8, linear & 0xff);
+    return TCB_OK;
 }
-

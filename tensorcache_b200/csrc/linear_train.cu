@@ -1,0 +1,655 @@
+// Training step of a linear layer whose input is kept in 8 bits: three products on the tcgen05 tensor cores.
+//
+//     forward       y[m, n]  = sum_k x[m, k] w[n, k] + b[n]
+//     input grad    dx[m, k] = sum_n dy[m, n] w[n, k]
+//     weight grad   dw[n, k] = sum_m dy[m, n] deq(q)[m, k]          db[n] = sum_m dy[m, n]
+//
+// x, w, dy, y and the gradients are bf16, sums are fp32 (TMEM accumulators, fp32 partial sums) and rounded once.  The
+// kept input exists as int8 / uint8 codes and group scales only; deq(q) is the bf16 number the decode kernels
+// produce, made in shared memory by producer warps, and never goes to global memory.
+//
+// One kernel serves all three: D[a, b] = sum_c A[a, c] B[b, c] on tiles of 256 x 256 per pair of CTAs
+// (tcgen05.mma.cta_group::2; each CTA stages 128 rows of A and 128 of B), 64 of the contraction per stage.  What
+// differs is which way the operands lie in memory:
+//     forward       A = x  (contraction contiguous)        B = w   (contraction contiguous)
+//     input grad    A = dy (contraction contiguous)        B = w   (rows contiguous)
+//     weight grad   A = dy (rows contiguous)               B = q   (rows contiguous, dequantised)
+// An operand whose contraction is contiguous is staged as 128 rows x 64 (128-byte rows, 128-byte swizzle), one whose
+// rows are contiguous as two boxes of 64 contraction steps x 64 rows, in the same swizzle: the tensor core reads either
+// (the "major" bits of the instruction descriptor), so nothing is transposed by anyone.
+//
+// Warps per CTA: 0 TMA, 1 MMA issue (leader CTA) and TMEM, 2-5 epilogue, 6-13 dequantising producers (weight
+// gradient only).  The two 256-column accumulators alternate between tiles, so a tile's epilogue runs under the next
+// one's products.  Where the output has too few tiles to fill the GPU the contraction is split: each part leaves fp32
+// sums in a workspace and a second kernel adds them in a fixed order (results do not depend on timing).
+//
+// Waits are bounded as in the fused dequantising product; the status word is read by tcb_fused_dequant_linear_check().
+#include <type_traits>
+
+#include "tcb_tcgen05.h"
+
+namespace {
+
+constexpr int kTileRows = 128;                       // rows of each operand per CTA
+constexpr int kPairRows = 256;                       // per pair
+constexpr int kBlockK = 64;                          // contraction per stage
+constexpr uint32_t kOperandBytes = 128 * 64 * 2;     // 16 KB: one operand, one CTA, one stage
+constexpr uint32_t kCodeBytes = 128 * 64;            // 8 KB of raw codes
+constexpr uint32_t kBoxBytes = 64 * 64 * 2;          // 8 KB: 64 contraction steps x 64 rows
+constexpr int kEpilogueWarps = 4, kProducerWarps = 8;
+constexpr int kFirstEpilogueWarp = 2, kFirstProducerWarp = kFirstEpilogueWarp + kEpilogueWarps;
+constexpr uint32_t kMaxSmem = 232448;
+
+enum Source { kContraction, kRows, kCodes };         // how an operand lies in memory (kCodes: rows contiguous, 8-bit codes)
+
+template <Source B>
+struct Config {
+    static constexpr bool kDeq = B == kCodes;
+    static constexpr int kThreads = 32 * (kFirstProducerWarp + (kDeq ? kProducerWarps : 0));
+    static constexpr int kStages = kDeq ? 5 : 6;
+    static constexpr uint32_t kTiles = kStages * (2 * kOperandBytes + (kDeq ? kCodeBytes : 0));
+    static constexpr uint32_t kSmem = kTiles + 1024 /* alignment */ + 256 /* barriers */;
+    static_assert(kSmem <= kMaxSmem, "shared memory");
+};
+
+struct Params {
+    int64_t rows_a, rows_b;     // output rows and columns
+    const uint16_t* bias;       // null, or one per column (only without a split)
+    uint16_t* out;              // [rows_a, rows_b]
+    float* partial;             // split: [splits][rows_a][ld_partial]
+    int64_t ld_partial;
+    const uint16_t* scales;     // codes: [contraction, rows_b / G]
+    const uint8_t* zp;
+    int64_t contraction;
+    int tiles_a, tiles_b, tiles;    // tiles = tiles_a * tiles_b
+    int num_kb, kb_per_split, items;
+};
+
+struct Item {
+    int ta, tb, split, kb0, kb1;
+};
+
+// Work items: the tiles of split 0, then those of split 1, ...  Tiles run in bands of 8 tile rows, down the band first,
+// so that the tiles in flight share their operands in L2.
+__device__ __forceinline__ Item decode_item(const Params& p, int item) {
+    Item r;
+    r.split = item / p.tiles;
+    const int t = item - r.split * p.tiles;
+    const int band = t / (8 * p.tiles_b), first = band * 8;
+    const int height = p.tiles_a - first < 8 ? p.tiles_a - first : 8;
+    const int u = t - first * p.tiles_b;
+    r.ta = first + u % height;
+    r.tb = u / height;
+    r.kb0 = r.split * p.kb_per_split;
+    r.kb1 = r.kb0 + p.kb_per_split < p.num_kb ? r.kb0 + p.kb_per_split : p.num_kb;
+    return r;
+}
+
+// Leading byte offset (in 16-byte units) of an operand's descriptor: contraction contiguous -- unused, 1; rows
+// contiguous -- from one box of 64 rows to the next.  The stride (1024 bytes: 8 rows of 128 bytes) is the same.
+template <bool ROWS>
+__device__ __forceinline__ uint32_t operand_lo(uint32_t smem_addr) {
+    return ((smem_addr & 0x3FFFFu) >> 4) | ((ROWS ? kBoxBytes >> 4 : 1u) << 16);
+}
+
+// The four MMAs (16 of the contraction each) of a stage.
+template <uint32_t STEP_A, uint32_t STEP_B>
+__device__ __forceinline__ void umma_x4(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate_first) {
+    asm volatile(
+        "{\n\t.reg .pred p, t;\n\t.reg .b64 a, b;\n\t.reg .b32 al, bl;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "setp.eq.b32 t, %5, %5;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n\t"
+        "add.u32 al, %1, %6;\n\tadd.u32 bl, %2, %7;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, t;\n\t"
+        "add.u32 al, al, %6;\n\tadd.u32 bl, bl, %7;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, t;\n\t"
+        "add.u32 al, al, %6;\n\tadd.u32 bl, bl, %7;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, t;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate_first), "n"(STEP_A), "n"(STEP_B)
+        : "memory");
+}
+
+// One CTA's part of an operand for one stage: rows [row, row + 128), contraction [c, c + 64).
+template <Source S>
+__device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* map, int row, int c, uint32_t bar) {
+    if constexpr (S == kContraction) {
+        tma_load_2d_pair(dst, map, c, row, bar);
+    } else {
+        tma_load_2d_pair(dst, map, row, c, bar);
+        tma_load_2d_pair(dst + kBoxBytes, map, row + 64, c, bar);
+    }
+}
+
+template <Source A, Source B, int LOG2_G, bool HAS_ZP>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<B>::kThreads, 1)
+linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
+    using C = Config<B>;
+    constexpr int S = C::kStages;
+    // bf16 x bf16 -> fp32, M = N = 256; bits 15 / 16: rows contiguous
+    constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((A != kContraction ? 1u : 0u) << 15) |
+                                ((B != kContraction ? 1u : 0u) << 16) | (uint32_t(kPairRows >> 3) << 17) | (uint32_t(kPairRows >> 4) << 24);
+    // 16 of the contraction in the descriptor's 16-byte units: 32 bytes along a row, or 16 rows of 128 bytes
+    constexpr uint32_t kStepA = A == kContraction ? 2 : 128, kStepB = B == kContraction ? 2 : 128;
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* smem_a = smem;
+    uint8_t* smem_b = smem + S * kOperandBytes;
+    uint8_t* smem_c = smem + 2 * S * kOperandBytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kTiles);
+    // barriers: full (leader), empty, full_c (raw codes), accumulator full [2], accumulator empty [2] (leader)
+    constexpr int FULL = 0, EMPTY = S, FULL_C = 2 * S, TFULL = 3 * S, TEMPTY = 3 * S + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * S + 4);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const uint32_t bar0 = smem_u32(bars);
+    auto bar = [&](int id) { return bar0 + 8u * uint32_t(id); };
+    auto leader_bar = [&](int id) { return map_to_cta(bar(id), 0); };
+    const uint32_t abort_peer = map_to_cta(smem_u32(const_cast<int*>(abort_flag)), rank ^ 1);
+
+    cluster_sync_all();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(bar(FULL + s), 2 + (C::kDeq ? 2 * kProducerWarps : 0));
+            mbar_init(bar(EMPTY + s), 1);
+            mbar_init(bar(FULL_C + s), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(TFULL + i), 1);
+            mbar_init(bar(TEMPTY + i), 2 * kEpilogueWarps);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(tmem_slot), 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int first = int(blockIdx.x >> 1), step = int(gridDim.x >> 1);
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- TMA
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int item = first; ok && item < p.items; item += step) {
+                const Item t = decode_item(p, item);
+                const int row_a = t.ta * kPairRows + int(rank) * kTileRows, row_b = t.tb * kPairRows + int(rank) * kTileRows;
+                for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                    ok = mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag, abort_peer, (1 << 8) | (EMPTY + s));
+                    if (!ok) break;
+                    const uint32_t full = leader_bar(FULL + s);
+                    load_operand<A>(smem_u32(smem_a + s * kOperandBytes), &map_a, row_a, kb * kBlockK, full);
+                    if constexpr (C::kDeq) {
+                        mbar_arrive_expect_tx(bar(FULL_C + s), kCodeBytes);
+                        tma_load_2d(smem_u32(smem_c + s * kCodeBytes), &map_b, row_b, kb * kBlockK, bar(FULL_C + s));
+                    } else {
+                        load_operand<B>(smem_u32(smem_b + s * kOperandBytes), &map_b, row_b, kb * kBlockK, full);
+                    }
+                    if (leader) mbar_arrive_expect_tx(bar(FULL + s), (C::kDeq ? 2 : 4) * kOperandBytes);
+                    else mbar_arrive_cluster(full);
+                    if (++s == S) { s = 0; ph ^= 1; }
+                }
+            }
+            if (!ok) {   // aborting: copies still in flight land in this CTA's shared memory within microseconds
+                const long long t0 = clock64();
+                while (clock64() - t0 < 4000000LL) __nanosleep(1000);
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issue
+        if (lane == 0 && leader) {
+            int s = 0, local = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            const uint32_t a0 = operand_lo<A != kContraction>(smem_u32(smem_a)), b0 = operand_lo<B != kContraction>(smem_u32(smem_b));
+            for (int item = first; ok && item < p.items; item += step, ++local) {
+                const Item t = decode_item(p, item);
+                const int buf = local & 1;
+                ok = mbar_wait(bar(TEMPTY + buf), ((local >> 1) & 1) ^ 1, abort_flag, abort_peer, (2 << 8) | (TEMPTY + buf));
+                if (!ok) break;
+                tc_fence_after();
+                for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                    ok = mbar_wait(bar(FULL + s), ph, abort_flag, abort_peer, (2 << 8) | (FULL + s));
+                    if (!ok) break;
+                    tc_fence_after();
+                    umma_x4<kStepA, kStepB>(tmem_base + uint32_t(buf * kPairRows), a0 + uint32_t(s) * (kOperandBytes >> 4),
+                                            b0 + uint32_t(s) * (kOperandBytes >> 4), kIdesc, kb > t.kb0 ? 1u : 0u);
+                    umma_commit_both(bar(EMPTY + s));
+                    if (++s == S) { s = 0; ph ^= 1; }
+                }
+                if (ok) umma_commit_both(bar(TFULL + buf));
+            }
+        }
+    } else if (warp < kFirstProducerWarp) {
+        // ---------------------------------------------------------------- epilogue
+        const int quad = warp & 3;   // the TMEM lanes this warp may read
+        const bool vec = (p.rows_b % 16 == 0) && ((reinterpret_cast<uintptr_t>(p.out) & 31) == 0) &&
+                         ((reinterpret_cast<uintptr_t>(p.bias) & 3) == 0);
+        int local = 0;
+        bool ok = true;
+        for (int item = first; ok && item < p.items; item += step, ++local) {
+            const Item t = decode_item(p, item);
+            const int buf = local & 1;
+            ok = __all_sync(0xffffffffu, mbar_wait(bar(TFULL + buf), (local >> 1) & 1, abort_flag, abort_peer, (4 << 8) | (TFULL + buf)));
+            if (!ok) break;
+            tc_fence_after();
+            const int64_t row = int64_t(t.ta) * kPairRows + int64_t(rank) * kTileRows + quad * 32 + lane;
+            const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(buf * kPairRows);
+#pragma unroll 1
+            for (int c = 0; c < kPairRows / 32; ++c) {
+                const int64_t col0 = int64_t(t.tb) * kPairRows + c * 32;
+                if (col0 >= p.rows_b) break;   // warp-uniform
+                uint32_t v[32];
+                tmem_ld32(taddr + uint32_t(c * 32), v);
+                tmem_ld_wait();
+                if (row >= p.rows_a) continue;
+                if (p.partial) {
+                    // ld_partial is a multiple of 8 and padded columns may be written
+                    float* dst = p.partial + (int64_t(t.split) * p.rows_a + row) * p.ld_partial + col0;
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+                        if (col0 + 8 * h < p.rows_b) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) w[i] = v[8 * h + i];
+                            st_global_v8(dst + 8 * h, w);
+                        }
+                    continue;
+                }
+                uint16_t* dst = p.out + row * p.rows_b + col0;
+                if (vec) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (col0 + 16 * h >= p.rows_b) continue;
+                        uint32_t w[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float x = __uint_as_float(v[16 * h + 2 * i]), y = __uint_as_float(v[16 * h + 2 * i + 1]);
+                            if (p.bias) {
+                                const uint32_t bb = __ldg(reinterpret_cast<const uint32_t*>(p.bias + col0) + 8 * h + i);
+                                x += __uint_as_float(bb << 16);
+                                y += __uint_as_float(bb & 0xffff0000u);
+                            }
+                            w[i] = pack_bf16(x, y);
+                        }
+                        st_global_v8(dst + 16 * h, w);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (col0 + i < p.rows_b) {
+                            float x = __uint_as_float(v[i]);
+                            if (p.bias) x += __uint_as_float(uint32_t(p.bias[col0 + i]) << 16);
+                            dst[i] = f32_to_bf16_bits(x);
+                        }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(leader_bar(TEMPTY + buf));
+        }
+    } else if constexpr (C::kDeq) {
+        // ---------------------------------------------------------------- dequantising producers
+        // Warp pw takes contraction rows [8 pw, 8 pw + 8) of the stage, a lane 2 x 16 codes of one row: columns
+        // 16 kq + 64 h of the CTA's 128 (h = 0, 1).  Rows of odd number read their upper half first, so that neither the
+        // reads of codes nor the writes of operand pieces meet in a bank.
+        const int pw = warp - kFirstProducerWarp, r = pw * 8 + (lane >> 2), kq = lane & 3, h0 = r & 1;
+        const uint32_t piece0 = uint32_t(((2 * kq) ^ (r & 7)) * 16), piece1 = piece0 ^ 16u;
+        const int64_t gpr = p.rows_b >> LOG2_G;
+        // scale and zero point of the lane's two pieces, fetched two stages ahead
+        int pf_item = first, pf_kb = 0;
+        Item pf = decode_item(p, pf_item < p.items ? pf_item : 0);
+        pf_kb = pf.kb0;
+        auto fetch = [&](uint32_t (&sz)[2]) {
+            sz[0] = sz[1] = 0;
+            if (pf_item >= p.items) return;
+            const int64_t m = int64_t(pf_kb) * kBlockK + r;
+            const int64_t col = int64_t(pf.tb) * kPairRows + int64_t(rank) * kTileRows + 16 * kq;
+            if (m < p.contraction) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int64_t k = col + 64 * (h0 ^ i);
+                    if (k < p.rows_b) {
+                        const int64_t g = m * gpr + (k >> LOG2_G);
+                        sz[i] = uint32_t(__ldg(p.scales + g)) << 16;
+                        if (HAS_ZP) sz[i] |= __ldg(p.zp + g);
+                    }
+                }
+            }
+            if (++pf_kb == pf.kb1) {
+                pf_item += step;
+                if (pf_item < p.items) {
+                    pf = decode_item(p, pf_item);
+                    pf_kb = pf.kb0;
+                }
+            }
+        };
+        uint32_t ahead0[2], ahead1[2];
+        fetch(ahead0);
+        fetch(ahead1);
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int item = first; ok && item < p.items; item += step) {
+            const Item t = decode_item(p, item);
+            for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                const uint32_t sz0 = ahead0[0], sz1 = ahead0[1];
+                ahead0[0] = ahead1[0];
+                ahead0[1] = ahead1[1];
+                fetch(ahead1);
+                // warp-uniform verdict: the warp-level sync below needs every lane
+                ok = __all_sync(0xffffffffu, mbar_wait(bar(FULL_C + s), ph, abort_flag, abort_peer, (3 << 8) | (FULL_C + s)));
+                if (!ok) break;
+                const uint8_t* c = smem_c + s * kCodeBytes + r * 128 + kq * 16;
+                const uint4 c0 = *reinterpret_cast<const uint4*>(c + 64 * h0), c1 = *reinterpret_cast<const uint4*>(c + 64 * (h0 ^ 1));
+                uint8_t* d = smem_b + s * kOperandBytes + r * 128;
+                uint8_t *d0 = d + h0 * kBoxBytes, *d1 = d + (h0 ^ 1) * kBoxBytes;
+                convert16<HAS_ZP>(c0, sz0, d0 + piece0, d0 + piece1);
+                convert16<HAS_ZP>(c1, sz1, d1 + piece0, d1 + piece1);
+                fence_proxy_async();   // the stores above become visible to the tensor cores
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(leader_bar(FULL + s));
+                if (++s == S) { s = 0; ph ^= 1; }
+            }
+        }
+    }
+
+    // Neither CTA leaves while the other may still arrive on its barriers or read its shared memory.
+    tc_fence_before();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+// out[a, b] = bf16(sum over the splits, in order, + bias[b]); four columns per thread.
+__global__ void __launch_bounds__(256) add_parts_kernel(const float* __restrict__ partial, int splits, int64_t rows, int64_t cols, int64_t ld,
+                                                        const uint16_t* __restrict__ bias, uint16_t* __restrict__ out) {
+    const int64_t quads = ld / 4, total = rows * quads;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+        const int64_t row = i / quads, col = (i - row * quads) * 4;
+        if (col >= cols) continue;
+        float4 sum = __ldcs(reinterpret_cast<const float4*>(partial + row * ld + col));
+        for (int s = 1; s < splits; ++s) {
+            const float4 v = __ldcs(reinterpret_cast<const float4*>(partial + (int64_t(s) * rows + row) * ld + col));
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (col + j < cols) {
+                const float b = bias ? __uint_as_float(uint32_t(bias[col + j]) << 16) : 0.0f;
+                out[row * cols + col + j] = f32_to_bf16_bits(f[j] + b);
+            }
+    }
+}
+
+// Column sums of dy: block (x, y) adds rows y, y + gridDim.y, ... (8 at a time) of 256 columns and leaves fp32 sums.
+__global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __restrict__ dy, int64_t rows, int64_t cols, int64_t ld,
+                                                          float* __restrict__ partial) {
+    __shared__ float acc[8][256];
+    const int r = threadIdx.x >> 5, c = (threadIdx.x & 31) * 8;
+    const int64_t col = int64_t(blockIdx.x) * 256 + c;
+    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (col < cols)   // ld is a multiple of 8: a whole 16-byte piece is there
+        for (int64_t row = int64_t(blockIdx.y) * 8 + r; row < rows; row += int64_t(gridDim.y) * 8) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(dy + row * ld + col));
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[2 * i] += __uint_as_float(w[i] << 16);
+                s[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[r][c + i] = s[i];
+    __syncthreads();
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += acc[i][threadIdx.x];
+    const int64_t out_col = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (out_col < cols) partial[int64_t(blockIdx.y) * cols + out_col] = sum;
+}
+
+__global__ void __launch_bounds__(256) add_column_sums_kernel(const float* __restrict__ partial, int parts, int64_t cols, uint16_t* __restrict__ out) {
+    const int64_t col = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (col >= cols) return;
+    float sum = 0.0f;
+    for (int i = 0; i < parts; ++i) sum += partial[int64_t(i) * cols + col];
+    out[col] = f32_to_bf16_bits(sum);
+}
+
+// ------------------------------------------------------------------------ host
+
+struct Plan {
+    int64_t tiles_a, tiles_b, num_kb;
+    int splits, kb_per_split;
+    int64_t ld_partial;
+    int64_t partial_bytes(int64_t rows_a) const { return splits > 1 ? int64_t(splits) * rows_a * ld_partial * 4 : 0; }
+};
+
+// Splits the contraction while tiles leave pairs of CTAs idle, but not into parts of fewer than 8 stages.
+Plan make_plan(int64_t rows_a, int64_t rows_b, int64_t contraction) {
+    Plan p;
+    p.tiles_a = (rows_a + kPairRows - 1) / kPairRows;
+    p.tiles_b = (rows_b + kPairRows - 1) / kPairRows;
+    p.num_kb = (contraction + kBlockK - 1) / kBlockK;
+    const int64_t pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1;
+    int64_t splits = pairs / (p.tiles_a * p.tiles_b);
+    if (splits > p.num_kb / 8) splits = p.num_kb / 8;
+    if (splits < 1) splits = 1;
+    p.kb_per_split = int((p.num_kb + splits - 1) / splits);
+    p.splits = int((p.num_kb + p.kb_per_split - 1) / p.kb_per_split);
+    p.ld_partial = (rows_b + 7) / 8 * 8;
+    return p;
+}
+
+int column_parts(int64_t rows, int64_t cols) {
+    const int64_t across = (cols + 255) / 256, most = (rows + 63) / 64;
+    int64_t parts = (2 * int64_t(tcb::sm_count()) + across - 1) / across;
+    if (parts > most) parts = most;
+    return int(parts < 1 ? 1 : parts);
+}
+
+// A tensor map over a row-major [outer, inner] array with rows of `ld` elements.
+int encode_map(const char* who, CUtensorMap* map, bool bytes, const void* base, int64_t inner, int64_t outer, int64_t ld, int box_inner,
+               int box_outer) {
+    EncodeTiledFn encode = encode_tiled_fn();
+    if (!encode) return tcb::fail(TCB_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available from the driver", who);
+    const cuuint64_t dims[2] = {cuuint64_t(inner), cuuint64_t(outer)};
+    const cuuint64_t strides[1] = {cuuint64_t(ld) * (bytes ? 1 : 2)};
+    const cuuint32_t box[2] = {cuuint32_t(box_inner), cuuint32_t(box_outer)}, estr[2] = {1, 1};
+    const CUresult cr = encode(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
+                               strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               bytes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return cr == CUDA_SUCCESS ? TCB_OK : tcb::fail(TCB_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed with %d", who, int(cr));
+}
+
+struct Operand {
+    const void* base;
+    int64_t rows, contraction, ld;
+};
+
+template <Source S>
+int operand_map(const char* who, CUtensorMap* map, const Operand& o) {
+    if (S == kContraction) return encode_map(who, map, false, o.base, o.contraction, o.rows, o.ld, kBlockK, kTileRows);
+    if (S == kRows) return encode_map(who, map, false, o.base, o.rows, o.contraction, o.ld, 64, kBlockK);
+    return encode_map(who, map, true, o.base, o.rows, o.contraction, o.ld, kTileRows, kBlockK);
+}
+
+template <Source A, Source B, int LOG2_G, bool HAS_ZP>
+int launch(const char* who, const Operand& a, const Operand& b, const uint16_t* scales, const uint8_t* zp, const uint16_t* bias, uint16_t* out,
+           void* workspace, int64_t workspace_bytes, cudaStream_t st) {
+    const Plan plan = make_plan(a.rows, b.rows, a.contraction);
+    if (plan.tiles_a * plan.tiles_b * plan.splits > (int64_t(1) << 30)) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: too many output tiles", who);
+    if (plan.partial_bytes(a.rows) > workspace_bytes)
+        return tcb::fail(TCB_ERR_BAD_ARG, "%s: the workspace holds %lld bytes, %lld are needed", who, (long long)workspace_bytes,
+                         (long long)plan.partial_bytes(a.rows));
+    CUtensorMap map_a, map_b;
+    int rc = operand_map<A>(who, &map_a, a);
+    if (rc == TCB_OK) rc = operand_map<B>(who, &map_b, b);
+    if (rc != TCB_OK) return rc;
+    const auto kernel = linear_kernel<A, B, LOG2_G, HAS_ZP>;
+    static std::atomic<bool> attr_set[64] = {};
+    int dev = 0;
+    TCB_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
+        TCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Config<B>::kSmem)));
+        if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
+    }
+    Params p;
+    p.rows_a = a.rows;
+    p.rows_b = b.rows;
+    p.bias = plan.splits > 1 ? nullptr : bias;
+    p.out = out;
+    p.partial = plan.splits > 1 ? static_cast<float*>(workspace) : nullptr;
+    p.ld_partial = plan.ld_partial;
+    p.scales = scales;
+    p.zp = zp;
+    p.contraction = a.contraction;
+    p.tiles_a = int(plan.tiles_a);
+    p.tiles_b = int(plan.tiles_b);
+    p.tiles = p.tiles_a * p.tiles_b;
+    p.num_kb = int(plan.num_kb);
+    p.kb_per_split = plan.kb_per_split;
+    p.items = p.tiles * plan.splits;
+    const int pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1;
+    kernel<<<2 * (p.items < pairs ? p.items : pairs), Config<B>::kThreads, Config<B>::kSmem, st>>>(map_a, map_b, p);
+    TCB_CUDA_TRY(cudaGetLastError());
+    if (plan.splits > 1) {
+        const int64_t blocks = (a.rows * (plan.ld_partial / 4) + 255) / 256, most = int64_t(tcb::sm_count()) * 8;
+        add_parts_kernel<<<unsigned(blocks < most ? blocks : most), 256, 0, st>>>(p.partial, plan.splits, a.rows, b.rows, plan.ld_partial, bias, out);
+        TCB_CUDA_TRY(cudaGetLastError());
+    }
+    return TCB_OK;
+}
+
+int check_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
+    const int64_t limit = (int64_t(1) << 31) - 1;
+    if (M < 0 || N < 0 || K < 0) return tcb::fail(TCB_ERR_BAD_ARG, "%s: negative size", who);
+    if (M > limit || N > limit || K > limit) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: dimension beyond 2^31 - 1", who);
+    if (M > 0 && N > 0 && (K <= 0 || K % 8 != 0)) return tcb::fail(TCB_ERR_BAD_ARG, "%s: K = %lld must be a positive multiple of 8", who, (long long)K);
+    return TCB_OK;
+}
+
+int check_operands(const char* who, const void* a, const void* b, const void* out, const void* bias, const void* workspace) {
+    if (!a || !b || !out) return tcb::fail(TCB_ERR_BAD_ARG, "%s: null pointer", who);
+    if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15)
+        return tcb::fail(TCB_ERR_ALIGNMENT, "%s: operands must be 16-byte aligned", who);
+    if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 1)
+        return tcb::fail(TCB_ERR_ALIGNMENT, "%s: bias and output must be 2-byte aligned", who);
+    if (reinterpret_cast<uintptr_t>(workspace) & 31) return tcb::fail(TCB_ERR_ALIGNMENT, "%s: the workspace must be 32-byte aligned", who);
+    return TCB_OK;
+}
+
+int check_ld(const char* who, int64_t ld, int64_t N) {
+    if (ld < N || ld % 8 != 0)
+        return tcb::fail(TCB_ERR_BAD_ARG, "%s: rows of dy are %lld elements apart: a multiple of 8, at least N = %lld, is needed", who,
+                         (long long)ld, (long long)N);
+    return TCB_OK;
+}
+
+}  // namespace
+
+namespace tcb {
+// Reads and clears this file's status word (the stream has been synchronised).
+int take_linear_status(int* status) {
+    *status = 0;
+    TCB_CUDA_TRY(cudaMemcpyFromSymbol(status, g_status, sizeof(int)));
+    if (*status) {
+        const int zero = 0;
+        TCB_CUDA_TRY(cudaMemcpyToSymbol(g_status, &zero, sizeof(int)));
+    }
+    return TCB_OK;
+}
+}  // namespace tcb
+
+extern "C" int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    const int64_t sizes[3] = {make_plan(M, N, K).partial_bytes(M), make_plan(M, K, N).partial_bytes(M),
+                              (make_plan(N, K, M).partial_bytes(N) + 31) / 32 * 32 + column_parts(M, N) * N * 4};
+    int64_t most = sizes[0];
+    for (int i = 1; i < 3; ++i) most = sizes[i] > most ? sizes[i] : most;
+    return most;
+}
+
+extern "C" int tcb_linear_forward(const uint16_t* x, const uint16_t* w, const uint16_t* bias_or_null, uint16_t* y, int64_t M, int64_t N, int64_t K,
+                                  void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* who = "tcb_linear_forward";
+    int rc = check_sizes(who, M, N, K);
+    if (rc != TCB_OK || M == 0 || N == 0) return rc;
+    rc = check_operands(who, x, w, y, bias_or_null, workspace);
+    if (rc != TCB_OK) return rc;
+    return launch<kContraction, kContraction, 0, false>(who, Operand{x, M, K, K}, Operand{w, N, K, K}, nullptr, nullptr, bias_or_null, y, workspace,
+                                                        workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int tcb_linear_grad_input(const uint16_t* dy, int64_t ld_dy, const uint16_t* w, uint16_t* dx, int64_t M, int64_t N, int64_t K,
+                                     void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* who = "tcb_linear_grad_input";
+    int rc = check_sizes(who, M, N, K);
+    if (rc == TCB_OK) rc = check_ld(who, ld_dy, N);
+    if (rc != TCB_OK || M == 0 || N == 0) return rc;
+    rc = check_operands(who, dy, w, dx, nullptr, workspace);
+    if (rc != TCB_OK) return rc;
+    return launch<kContraction, kRows, 0, false>(who, Operand{dy, M, N, ld_dy}, Operand{w, K, N, K}, nullptr, nullptr, nullptr, dx, workspace,
+                                                 workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int tcb_linear_grad_weight(const uint16_t* dy, int64_t ld_dy, const uint8_t* q, const uint16_t* scales, const uint8_t* zp_or_null,
+                                      uint16_t* dw_or_null, uint16_t* db_or_null, int64_t M, int64_t N, int64_t K, int group_size, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+    const char* who = "tcb_linear_grad_weight";
+    int rc = check_sizes(who, M, N, K);
+    if (rc == TCB_OK) rc = check_ld(who, ld_dy, N);
+    if (rc != TCB_OK) return rc;
+    if (dw_or_null && !tcb::core_group_size_ok(group_size) && group_size != 128)
+        return tcb::fail(TCB_ERR_GROUP_SIZE, "%s: group_size %d not in {16, 32, 64, 128}", who, group_size);
+    if (M == 0 || N == 0) return TCB_OK;
+    if (dw_or_null && K % group_size != 0)
+        return tcb::fail(TCB_ERR_BAD_ARG, "%s: K = %lld must be a multiple of the group size %d", who, (long long)K, group_size);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!dy || (reinterpret_cast<uintptr_t>(dy) & 15)) return tcb::fail(TCB_ERR_BAD_ARG, "%s: dy is null or not 16-byte aligned", who);
+    if (dw_or_null) {
+        if (!scales) return tcb::fail(TCB_ERR_BAD_ARG, "%s: null pointer", who);
+        rc = check_operands(who, dy, q, dw_or_null, scales, workspace);
+        if (rc != TCB_OK) return rc;
+    }
+    const int64_t dw_bytes = (make_plan(N, K, M).partial_bytes(N) + 31) / 32 * 32;
+    if (db_or_null) {
+        const int parts = column_parts(M, N);
+        if (!workspace || workspace_bytes < dw_bytes + parts * N * 4 || (reinterpret_cast<uintptr_t>(workspace) & 31))
+            return tcb::fail(TCB_ERR_BAD_ARG, "%s: the workspace is too small or not 32-byte aligned", who);
+        float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + dw_bytes);
+        column_sums_kernel<<<dim3(unsigned((N + 255) / 256), unsigned(parts)), 256, 0, st>>>(dy, M, N, ld_dy, partial);
+        add_column_sums_kernel<<<unsigned((N + 255) / 256), 256, 0, st>>>(partial, parts, N, db_or_null);
+        TCB_CUDA_TRY(cudaGetLastError());
+    }
+    if (!dw_or_null) return TCB_OK;
+    const Operand a{dy, N, M, ld_dy}, b{q, K, M, K};
+    uint16_t* dw = dw_or_null;
+    const uint8_t* zp = zp_or_null;
+    switch (group_size) {
+    case 16: return zp ? launch<kRows, kCodes, 4, true>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st)
+                       : launch<kRows, kCodes, 4, false>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st);
+    case 32: return zp ? launch<kRows, kCodes, 5, true>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st)
+                       : launch<kRows, kCodes, 5, false>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st);
+    case 64: return zp ? launch<kRows, kCodes, 6, true>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st)
+                       : launch<kRows, kCodes, 6, false>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st);
+    default: return zp ? launch<kRows, kCodes, 7, true>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st)
+                       : launch<kRows, kCodes, 7, false>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st);
+    }
+}

@@ -141,6 +141,36 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&w)[8]) {
 constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t smem_desc_lo(uint32_t smem_addr) { return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16); }
 
+// 16 codes of one group -> 16 bf16 values, the numbers the decode kernels produce, written as two 16-byte pieces of the 128-byte-swizzled operand row.
+// Per code: one byte permute (the byte into the mantissa of 2^15), one FMA, half a cvt.rn.bf16x2.f32.
+template <bool HAS_ZP>
+__device__ __forceinline__ void convert16(uint4 c, uint32_t sz_word, uint8_t* piece0, uint8_t* piece1) {
+    uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    const float scale = __uint_as_float(sz_word & 0xFFFF0000u);
+    float base;
+    if (HAS_ZP) {
+        base = __uint_as_float(__byte_perm(sz_word, 0x47000000u, 0x7604));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] ^= 0x80808080u;
+        base = __uint_as_float(0x47008000u);
+    }
+    const float cc = -__fmul_rn(base, scale);
+    const uint32_t magic = 0x47000000u;
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f0 = __fmaf_rn(__uint_as_float(__byte_perm(w[i], magic, 0x7604)), scale, cc);
+        const float f1 = __fmaf_rn(__uint_as_float(__byte_perm(w[i], magic, 0x7614)), scale, cc);
+        const float f2 = __fmaf_rn(__uint_as_float(__byte_perm(w[i], magic, 0x7624)), scale, cc);
+        const float f3 = __fmaf_rn(__uint_as_float(__byte_perm(w[i], magic, 0x7634)), scale, cc);
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[2 * i]) : "f"(f1), "f"(f0));
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[2 * i + 1]) : "f"(f3), "f"(f2));
+    }
+    *reinterpret_cast<uint4*>(piece0) = make_uint4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<uint4*>(piece1) = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
@@ -157,8 +187,12 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// The encoder, with the current device's context bound to this thread: the encoder is a driver call, and a thread that
+// has made no CUDA call of its own yet (a backward pass runs on one of the autograd engine's) has no context.
 EncodeTiledFn encode_tiled_fn() {
     static std::atomic<EncodeTiledFn> cached{nullptr};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return nullptr;
     EncodeTiledFn fn = cached.load(std::memory_order_acquire);
     if (!fn) {
         void* sym = nullptr;

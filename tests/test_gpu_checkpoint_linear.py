@@ -1,0 +1,282 @@
+"""Linear layers whose input is kept in 8 bits, against 64-bit products.
+
+Tolerances.  A result is rounded once to bf16: 2^-8 of its magnitude.  The sums behind it are fp32 over bf16 x bf16
+products (exact in fp32): adding n terms in fp32 in any order is off by at most n 2^-24 times the sum of magnitudes.
+The weight gradient multiplies the codec's decoded values, which are bf16 roundings of code * scale: the reference
+rounds them too.  With bound = |a| @ |b| that gives, per element,
+    |got - ref| <= 2^-8 |ref| + (1 + 2^-8) n 2^-24 bound + smallest bf16 subnormal."""
+import pytest
+import torch
+
+import tensorcache_b200 as tc
+from tensorcache_b200.fused_linear import check_device_status
+from tests import low_bit_plain as plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def close(got, a, b, add=None):
+    """got ~ a @ b (+ add) for fp64 a [r, n], b [n, c]."""
+    ref, bound = a @ b, a.abs() @ b.abs()
+    if add is not None:
+        ref, bound = ref + add, bound + add.abs()
+    n = a.shape[1] + 1
+    tol = 2.0 ** -8 * ref.abs() + 1.01 * n * 2.0 ** -24 * bound + 2.0 ** -133
+    assert got.dtype == torch.bfloat16 and got.shape == ref.shape
+    off = (got.double() - ref).abs()
+    assert bool((off <= tol).all()), (float((off / tol).nan_to_num(0).max()), tuple(got.shape))
+
+
+def layer(M, N, K, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(M, K, generator=g, device=DEV) * torch.exp(torch.randn(K, generator=g, device=DEV))
+    w = torch.randn(N, K, generator=g, device=DEV) * K ** -0.5
+    return (x.to(torch.bfloat16), w.to(torch.bfloat16), torch.randn(N, generator=g, device=DEV).to(torch.bfloat16),
+            torch.randn(M, N, generator=g, device=DEV).to(torch.bfloat16))
+
+
+def decoded(q, s, G, zp=None):
+    return plain.int8_values(q, s, G, zp).to(torch.bfloat16).double()
+
+
+SIZES = [(1, 1, 16, 16), (1, 768, 768, 32), (3, 17, 96, 32), (64, 64, 64, 64), (65, 130, 80, 16), (129, 257, 384, 128), (256, 256, 256, 32),
+         (257, 1000, 768, 32), (446, 768, 768, 16), (1000, 33, 2048, 64), (4000, 40, 128, 128), (20011, 100, 192, 32), (300, 2049, 1024, 32)]
+
+
+@pytest.mark.parametrize("M,N,K,G", SIZES)
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_checkpoint_linear(M, N, K, G, with_bias):
+    x, w, b, dy = layer(M, N, K, M + N + K)
+    x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)
+    y = tc.int8_checkpoint_linear(x, w, b if with_bias else None, group_size=G)
+    grads = torch.autograd.grad(y, [x, w] + ([b] if with_bias else []), dy)
+    check_device_status()
+    X, W, D = x.detach().double(), w.detach().double(), dy.double()
+    close(y.detach(), X, W.t(), b.detach().double() if with_bias else None)
+    close(grads[0], D, W)
+    close(grads[1], D.t(), decoded(*plain.int8_encode(x.detach(), G), G))
+    if with_bias:
+        close(grads[2].view(1, -1), torch.ones(1, M, dtype=torch.float64, device=DEV), D)
+
+
+@pytest.mark.parametrize("M,N,K,G", SIZES)
+@pytest.mark.parametrize("zp", [False, True])
+def test_gradient_from_cached_codes(M, N, K, G, zp):
+    x, w, b, dy = layer(M, N, K, M + N)
+    w.requires_grad_(True), b.requires_grad_(True)
+    if zp:
+        q, s, z, _ = tc.compress(x, "fast", G)
+    else:
+        (q, s, _), z = tc.quantize_int8_g32(x, G), None
+    q = q.view(M, K)
+    y = tc.fused_dequant_linear(q, s, w, b, zero_points=z, group_size=G)
+    dw, db = torch.autograd.grad(y, [w, b], dy)
+    check_device_status()
+    X = decoded(q, s, G, z)
+    close(y.detach(), X, w.detach().double().t(), b.detach().double())
+    close(dw, dy.double().t(), X)
+    close(db.view(1, -1), torch.ones(1, M, dtype=torch.float64, device=DEV), dy.double())
+    # the values of the module without gradients
+    module = tc.FusedDequantLinear(K, N, group_size=G).to(DEV)
+    with torch.no_grad():
+        module.weight.copy_(w), module.bias.copy_(b)
+    assert torch.equal(module(q, s, z), y.detach())
+
+
+def test_wide_layer():
+    """Many tiles per pair of CTAs (both accumulators, several bands of tiles) in all three products."""
+    M, N, K, G = 4360, 2312, 2560, 32
+    x, w, _, dy = layer(M, N, K)
+    x.requires_grad_(True), w.requires_grad_(True)
+    y = tc.int8_checkpoint_linear(x, w, None, group_size=G)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    X, W, D = x.detach().double(), w.detach().double(), dy.double()
+    close(y.detach(), X, W.t())
+    close(dx, D, W)
+    close(dw, D.t(), decoded(*plain.int8_encode(x.detach(), G), G))
+
+
+def test_gradients_against_differences():
+    """Directional differences of the layer's own outputs.  The loss is linear in w and in x, so a difference over a
+    finite step is exact but for the bf16 roundings of the two outputs: half a step, 2^-8 of each at most per element,
+    times |dy|, summed over all elements, and of the gradient (2^-8 of each term)."""
+    M, N, K = 96, 48, 64
+    x, w, b, dy = layer(M, N, K, 5)
+    x = (x.float() / x.float().abs().amax(-1, keepdim=True).clamp(min=1e-3) * 127).round().to(torch.bfloat16)   # codes of scale 1: exact
+    x[:, ::32] = 127.0
+    x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)
+    y = tc.int8_checkpoint_linear(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y, [x, w, b], dy)
+    for grad, which in ((gx, 0), (gw, 1), (gb, 2)):
+        args = [x.detach(), w.detach(), b.detach()]
+        step = torch.randn_like(args[which].float()).to(torch.bfloat16)
+        moved = (args[which].double() + step.double()).to(torch.bfloat16)
+        real = moved.double() - args[which].double()          # the step that was taken after rounding
+        args[which] = moved
+        y2 = tc.int8_checkpoint_linear(*args)
+        change = ((y2.double() - y.detach().double()) * dy.double()).sum()
+        slope = (grad.double() * real).sum()
+        tol = (2.0 ** -8 * (y2.double().abs() + y.detach().double().abs()) * dy.double().abs()).sum() + (2.0 ** -8 * (grad.double() * real).abs()).sum()
+        assert abs(float(change - slope)) <= float(tol)
+
+
+def test_graph_keeps_codes_and_not_the_input():
+    x, w, _, _ = layer(4096, 64, 1024)
+    w.requires_grad_(True)
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        tc.int8_checkpoint_linear(x, w)
+    assert sum(t.numel() * t.element_size() for t in kept) == 4096 * 1024 * (1 + 2 / 32)
+    kept.clear()
+    with torch.no_grad(), torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        tc.int8_checkpoint_linear(x, w)
+    assert not kept
+
+
+def test_shapes_strides_partial_gradients_and_expanded_dy():
+    x, w, b, dy = layer(24, 40, 64, 9)
+    ref = tc.int8_checkpoint_linear(x, w, b)
+    x3 = x.view(2, 3, 4, 64)
+    assert torch.equal(tc.int8_checkpoint_linear(x3, w, b), ref.view(2, 3, 4, 40))
+    assert torch.equal(tc.int8_checkpoint_linear(x.t().contiguous().t(), w.t().contiguous().t(), b), ref)
+    shifted = torch.empty(24 * 64 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(24, 64)
+    shifted.copy_(x)
+    assert torch.equal(tc.int8_checkpoint_linear(shifted, w, b), ref)
+    assert tc.int8_checkpoint_linear(x[0], w, b).shape == (40,)
+    for which in range(3):       # one leaf at a time, a dy without memory of its own
+        leaves = [x.clone(), w.clone(), b.clone()]
+        leaves[which].requires_grad_(True)
+        tc.int8_checkpoint_linear(*leaves).sum().backward()
+        ones = torch.ones(24, 40, dtype=torch.float64, device=DEV)
+        if which == 0:
+            close(leaves[0].grad, ones, w.double())
+        elif which == 1:
+            close(leaves[1].grad, ones.t(), decoded(*plain.int8_encode(x, 32), 32))
+        else:
+            assert torch.equal(leaves[2].grad, torch.full_like(b, 24))
+    x.requires_grad_(True), w.requires_grad_(True)
+    dyt = dy.t().contiguous().t()
+    a = torch.autograd.grad(tc.int8_checkpoint_linear(x, w), [x, w], dy)
+    c = torch.autograd.grad(tc.int8_checkpoint_linear(x, w), [x, w], dyt)
+    assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
+
+
+def test_empty_batches_and_layers():
+    w, b = (torch.randn(s, device=DEV).to(torch.bfloat16).requires_grad_(True) for s in ((8, 32), (8,)))
+    x = torch.empty(0, 32, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    y = tc.int8_checkpoint_linear(x, w, b)
+    assert y.shape == (0, 8)
+    gx, gw, gb = torch.autograd.grad(y, [x, w, b], torch.empty_like(y))
+    assert gx.shape == (0, 32) and not bool(gw.any()) and not bool(gb.any()) and gw.shape == (8, 32)
+    x = torch.randn(4, 32, device=DEV).to(torch.bfloat16).requires_grad_(True)
+    w0 = torch.empty(0, 32, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    y = tc.int8_checkpoint_linear(x, w0)
+    gx, gw = torch.autograd.grad(y, [x, w0], torch.empty_like(y))
+    assert y.shape == (4, 0) and not bool(gx.any()) and gw.shape == (0, 32)
+    q, s, _ = tc.quantize_int8_g32(x[:0])
+    y = tc.fused_dequant_linear(q.view(0, 32), s, w, b)
+    gw, gb = torch.autograd.grad(y, [w, b], torch.empty_like(y))
+    assert not bool(gw.any()) and not bool(gb.any())
+
+
+def test_repeated_calls_give_the_same_bits():
+    x, w, b, dy = layer(20011, 100, 192, 1)
+    x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)
+    runs = [torch.autograd.grad(tc.int8_checkpoint_linear(x, w, b), [x, w, b], dy) for _ in range(3)]
+    for other in runs[1:]:
+        assert all(torch.equal(a, c) for a, c in zip(runs[0], other))
+
+
+def test_training_step_captured_and_replayed():
+    M, N, K = 3000, 72, 128
+    x, w, b, dy = layer(M, N, K, 3)
+    x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)
+
+    def step():
+        y = tc.int8_checkpoint_linear(x, w, b)
+        return (y.detach(), *torch.autograd.grad(y, [x, w, b], dy))
+
+    # no eager graph of the same leaves is alive here: torch ties a leaf's gradient node to the stream of the first graph
+    # that is still alive, and refuses a capture that would have to wait for that stream (for its own operators as well)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (11, 12):
+        nx, nw, nb, ndy = layer(M, N, K, seed)
+        with torch.no_grad():
+            x.copy_(nx), w.copy_(nw), b.copy_(nb), dy.copy_(ndy)
+        graph.replay()
+        assert all(torch.equal(a, c) for a, c in zip(out, step()))
+
+
+def test_weight_changed_in_place_before_the_backward_pass_is_reported():
+    x, w, _, dy = layer(16, 8, 32)
+    x.requires_grad_(True)
+    y = tc.int8_checkpoint_linear(x, w)
+    w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, [x], dy)
+
+
+def test_calls_from_threads_that_have_made_no_cuda_call():
+    """A fresh host thread has no CUDA context of its own until a call binds one (the memory comes from a cache)."""
+    import threading
+
+    x, w, b, dy = layer(64, 32, 64)
+    q, s, _ = tc.quantize_int8_g32(x)
+    calls = [lambda: tc.int8_checkpoint_linear(x, w, b), lambda: tc.fused_dequant_linear(q.view(64, 64), s, w, b),
+             lambda: tc.fused_dequant_matmul(x, q.view(64, 64), s)]
+    want = [c() for c in calls]
+    got, errors = [None] * len(calls), []
+
+    def work(i):
+        try:
+            got[i] = calls[i]()
+        except Exception as e:  # noqa: BLE001 -- reported below
+            errors.append(e)
+
+    for i in range(len(calls)):
+        t = threading.Thread(target=work, args=(i,))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors and all(torch.equal(a, c) for a, c in zip(want, got))
+
+
+def test_module_trains_in_a_stack():
+    """Input gradient through two layers and a non-linearity between them, against the same stack in 64 bits on the
+    bf16 intermediates (so that each product is checked on its own)."""
+    torch.manual_seed(0)
+    l1, l2 = tc.Int8CheckpointLinear(64, 96).to(DEV), tc.Int8CheckpointLinear(96, 8, bias=False).to(DEV)
+    x = torch.randn(50, 64, device=DEV).to(torch.bfloat16).requires_grad_(True)
+    h = l1(x)
+    h.retain_grad()
+    a = torch.relu(h)
+    y = l2(a)
+    dy = torch.randn_like(y)
+    y.backward(dy)
+    close(l2.weight.grad, dy.double().t(), decoded(*plain.int8_encode(a.detach(), 32), 32))
+    close(l1.weight.grad, h.grad.double().t(), decoded(*plain.int8_encode(x.detach(), 32), 32))
+    close(x.grad, h.grad.double(), l1.weight.detach().double())
+    close(l1.bias.grad.view(1, -1), torch.ones(1, 50, dtype=torch.float64, device=DEV), h.grad.double())
+
+
+def test_device_cache_feeds_a_head():
+    """Rows written into a device cache, gathered as codes, and a head trained on them: the gradient is that of the
+    decoded rows."""
+    cache = tc.DeviceFeatureCache(500, 128, 32, DEV)
+    cache.write(torch.randperm(500, device=DEV), torch.randn(500, 128, device=DEV))
+    pick = torch.randint(0, 500, (77,), device=DEV)
+    w = torch.randn(10, 128, device=DEV).to(torch.bfloat16).requires_grad_(True)
+    dy = torch.randn(77, 10, device=DEV).to(torch.bfloat16)
+    y = tc.fused_dequant_linear(cache.codes[pick], cache.scales[pick], w)
+    (dw,) = torch.autograd.grad(y, [w], dy)
+    rows = cache.read(pick).double()
+    close(y.detach(), rows, w.detach().double().t())
+    close(dw, dy.double().t(), rows)

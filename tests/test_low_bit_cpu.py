@@ -95,3 +95,46 @@ def test_device_cache_refusals():
     else:
         with pytest.raises(RuntimeError, match="CUDA device"):
             tc.DeviceFeatureCache(4, 64)
+
+
+def test_linear_entry_points_refuse_bad_arguments(built_lib):
+    from tensorcache_b200 import _lib
+
+    L, p = built_lib, 1 << 20
+    fwd = lambda *a: L.tcb_linear_forward(*a, None)  # noqa: E731
+    assert fwd(None, None, None, None, 0, 8, 32, None, 0) == _lib.TCB_OK
+    assert fwd(p, p, None, p, 4, 8, 12, p, 0) == _lib.ERR_BAD_ARG            # K % 8
+    assert fwd(p, p, None, p, 4, -8, 16, p, 0) == _lib.ERR_BAD_ARG
+    assert fwd(None, p, None, p, 4, 8, 16, p, 0) == _lib.ERR_BAD_ARG
+    assert fwd(p + 2, p, None, p, 4, 8, 16, p, 0) == _lib.ERR_ALIGNMENT
+    assert fwd(p, p, p + 1, p, 4, 8, 16, p, 0) == _lib.ERR_ALIGNMENT
+    assert fwd(p, p, None, p, 1 << 31, 8, 16, p, 0) == _lib.ERR_TOO_LARGE
+    gi = lambda *a: L.tcb_linear_grad_input(*a, None)  # noqa: E731
+    assert gi(p, 8, p, p, 4, 16, 32, p, 0) == _lib.ERR_BAD_ARG               # ld < N
+    assert gi(p, 20, p, p, 4, 16, 32, p, 0) == _lib.ERR_BAD_ARG              # ld % 8
+    gw = lambda *a: L.tcb_linear_grad_weight(*a, None)  # noqa: E731
+    assert gw(p, 8, p, p, None, p, None, 4, 8, 32, 24, p, 0) == _lib.ERR_GROUP_SIZE
+    assert gw(p, 8, p, p, None, p, None, 4, 8, 48, 32, p, 0) == _lib.ERR_BAD_ARG
+    assert gw(p, 8, p, None, None, p, None, 4, 8, 32, 32, p, 0) == _lib.ERR_BAD_ARG
+    assert gw(p, 8, p, p, None, None, p, 4, 8, 32, 32, p, 4) == _lib.ERR_BAD_ARG   # workspace too small
+    assert L.tcb_linear_workspace(0, 8, 32) == 0 and L.tcb_linear_workspace(4, 8, 32) > 0
+
+
+def test_linear_layer_refusals():
+    bf = torch.bfloat16
+    x, w, b = torch.zeros(4, 64, dtype=bf), torch.zeros(8, 64, dtype=bf), torch.zeros(8, dtype=bf)
+    for bad, match in (((x.float(), w, b), "bf16"), ((x, w.float(), b), "bf16"), ((x, w, b.float()), "bf16"), ((x, w[:, :32], b), "weight"),
+                       ((x, w, b[:4]), "bias"), ((x, w[0], b), "weight"), ((x[:, :24], w[:, :24], b), "multiple")):
+        with pytest.raises(ValueError, match=match):
+            tc.int8_checkpoint_linear(*bad)
+    with pytest.raises(ValueError, match="group_size"):
+        tc.int8_checkpoint_linear(x, w, b, group_size=24)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        tc.int8_checkpoint_linear(x, w, b)
+    q, s = torch.zeros(4, 64, dtype=torch.int8), torch.zeros(8, dtype=bf)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        tc.fused_dequant_linear(q, s, w, b)
+    with pytest.raises(ValueError, match="scales"):
+        tc.fused_dequant_linear(q, s[:-1], w, b)
+    with pytest.raises(ValueError, match="int8"):
+        tc.fused_dequant_linear(q.to(torch.uint8), s, w, b)
