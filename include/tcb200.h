@@ -187,6 +187,21 @@ TCB_API int tcb_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, in
                                  void* stream);
 
 /*
+ * Product of MXFP4 operands on the block-scaled tensor-core path:
+ *     out[m, n] = bf16( sum_k X[m, k] W[n, k] + bias[n] )          (fp32 sums)
+ * with X = the MXFP4 values of x (quantised by the call, as tcb_quantize_mxfp4 does) and W the
+ * values of wq [N, K / 2], w_scales (tile order; no padding byte may be 255: it would be a NaN).
+ * No counterpart in the reference.
+ *   x [M, K] of `dtype`, 16-byte aligned like wq and w_scales; bias bf16 [N] or NULL;
+ *   out [M, N] bf16; workspace: tcb_mxfp4_linear_workspace(M, K) bytes, 16-byte aligned, used by
+ *   the call's own work on `stream` only.  K a positive multiple of 32; M, N arbitrary.
+ */
+TCB_API int64_t tcb_mxfp4_linear_workspace(int64_t M, int64_t K);
+TCB_API int tcb_mxfp4_linear(const void* x, int dtype, const uint8_t* wq, const uint8_t* w_scales,
+                             const uint16_t* bias_or_null, uint16_t* out, int64_t M, int64_t N, int64_t K,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Rows of a device-resident cache of symmetric int8 codes, quantised as they are written and
  * decoded as they are read (the device counterpart of FeatureCacheWriter.append,
  * src/tensorcache/feature_cache.py:342-424, and of the row gather of
@@ -253,8 +268,8 @@ TCB_API int tcb_linear_grad_weight(const uint16_t* dy, int64_t ld_dy, const uint
                                    int64_t N, int64_t K, int group_size, void* workspace, int64_t workspace_bytes,
                                    void* stream);
 
-/* Reads (and clears) the per-device status words the fused GEMM and the tcb_linear_*
- * kernels write when a bounded wait runs out.  Synchronises `stream`.  Returns TCB_OK or TCB_ERR_TIMEOUT. */
+/* Reads (and clears) the per-device status words the fused GEMM, the tcb_linear_*
+ * and the MXFP4 product kernels write when a bounded wait runs out.  Synchronises `stream`.  Returns TCB_OK or TCB_ERR_TIMEOUT. */
 TCB_API int tcb_fused_dequant_linear_check(void* stream);
 
 /* Launches a tiny kernel whose only work is a bounded wait on a barrier that nothing

@@ -15,7 +15,7 @@ from .codec import (AMO_BQ_PRESETS, BlockwiseInt8Codec, dequantize_int8_amo_bq, 
 from .device_cache import DeviceFeatureCache
 from .feature_cache import FeatureCacheDataset, FeatureCacheWriter
 from .fused_linear import FusedDequantLinear, fused_dequant_matmul
-from .mxfp4 import dequantize_mxfp4, mxfp4_scales_from_rows, mxfp4_scales_to_rows, quantize_mxfp4
+from .mxfp4 import dequantize_mxfp4, mxfp4_matmul, mxfp4_scales_from_rows, mxfp4_scales_to_rows, quantize_mxfp4
 from .streamer import ZeroCopyTensorStreamer
 from .utils import auto_select_mode, benchmark_tensor, compress, decompress, estimate_compression, selftest_sum_order
 
@@ -26,6 +26,6 @@ __all__ = [
     "compress", "decompress", "estimate_compression", "benchmark_tensor", "auto_select_mode", "selftest_sum_order",
     "FusedDequantLinear", "fused_dequant_matmul",
     "fused_dequant_linear", "int8_checkpoint_linear", "Int8CheckpointLinear",
-    "quantize_mxfp4", "dequantize_mxfp4", "mxfp4_scales_to_rows", "mxfp4_scales_from_rows",
+    "quantize_mxfp4", "dequantize_mxfp4", "mxfp4_matmul", "mxfp4_scales_to_rows", "mxfp4_scales_from_rows",
     "DeviceFeatureCache", "FeatureCacheWriter", "FeatureCacheDataset", "ZeroCopyTensorStreamer",
 ]

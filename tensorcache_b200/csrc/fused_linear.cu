@@ -72,6 +72,7 @@
 
 namespace tcb {
 int take_linear_status(int* status);
+int take_mxfp4_status(int* status);
 }
 
 namespace {
@@ -631,8 +632,9 @@ extern "C" int tcb_selftest_bounded_wait(int budget_ms, void* stream) {
 
 extern "C" int tcb_fused_dequant_linear_check(void* stream) {
     TCB_CUDA_TRY(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
-    int status = 0, linear = 0;
-    const int rc = tcb::take_linear_status(&linear);
+    int status = 0, linear = 0, mxfp4 = 0;
+    int rc = tcb::take_linear_status(&linear);
+    if (rc == TCB_OK) rc = tcb::take_mxfp4_status(&mxfp4);
     if (rc != TCB_OK) return rc;
     TCB_CUDA_TRY(cudaMemcpyFromSymbol(&status, g_status, sizeof(int)));
     if (status != 0) {
@@ -642,5 +644,7 @@ extern "C" int tcb_fused_dequant_linear_check(void* stream) {
     }
     if (linear != 0)
         return tcb::fail(TCB_ERR_TIMEOUT, "tcb_linear_*: a bounded wait ran out (role %d, barrier %d)", linear >> 8, linear & 0xff);
+    if (mxfp4 != 0)
+        return tcb::fail(TCB_ERR_TIMEOUT, "tcb_mxfp4_linear: a bounded wait ran out (role %d, barrier %d)", mxfp4 >> 8, mxfp4 & 0xff);
     return TCB_OK;
 }

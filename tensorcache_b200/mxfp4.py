@@ -123,3 +123,42 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, orig_shape: Tupl
         if not direct:
             out_buffer.copy_(od.view(out_buffer.shape))
     return out_buffer
+
+
+def mxfp4_matmul(x: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``mxfp4(x) @ dequant(W).T (+ bias)`` on the 4-bit tensor cores, with W stored as MXFP4 (``wq`` uint8 ``[N, K / 2]``,
+    ``w_scales`` in tile order, both as ``quantize_mxfp4`` returns them for ``[N, K]``).
+
+    ``x`` is bf16, fp16 or fp32 ``[..., K]`` and is quantised by the call, each row in blocks of 32; the result is bf16
+    ``[..., N]``, summed in fp32 and rounded once.  The counterpart of ``fused_dequant_matmul`` for 4-bit weights, and
+    like it without a gradient: an ``x`` that requires one is refused.  CUDA tensors only.
+    """
+    if wq.dim() != 2 or x.dim() == 0:
+        raise ValueError(f"x must be [..., K] and wq [N, K / 2], got {tuple(x.shape)} and {tuple(wq.shape)}")
+    N, K = wq.shape[0], wq.shape[1] * 2
+    if K <= 0 or K % BLOCK != 0 or x.shape[-1] != K:
+        raise ValueError(f"the inner dimensions must agree and be a positive multiple of {BLOCK}, got {x.shape[-1]} and {K}")
+    _check_codes(wq, w_scales, N, K)
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
+    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype != torch.bfloat16 or bias.device != x.device):
+        raise ValueError(f"bias must be bf16 [{N}] on {x.device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
+    if wq.device != x.device:
+        raise ValueError(f"x is on {x.device}, the weight on {wq.device}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("mxfp4_matmul has no gradient: call it under torch.no_grad() or detach x")
+    if not x.is_cuda:
+        raise RuntimeError("mxfp4_matmul runs on CUDA tensors only (no CPU fallback)")
+    x2 = x.detach().reshape(-1, K)
+    M = x2.shape[0]
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    if M and N:
+        with torch.cuda.device(x.device):
+            x2, cd, sd = _aligned(x2.contiguous()), _aligned(wq.contiguous()), _aligned(w_scales.contiguous())
+            b = None if bias is None else bias.detach().contiguous()
+            L = _lib.lib()
+            nbytes = L.tcb_mxfp4_linear_workspace(M, K)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            stream = ctypes.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)
+            _lib.check(L.tcb_mxfp4_linear(_ptr(x2), _DTYPES[x2.dtype], _ptr(cd), _ptr(sd), _ptr(b), _ptr(out), M, N, K, _ptr(ws), nbytes, stream))
+    return out.view(*x.shape[:-1], N)

@@ -1,9 +1,10 @@
-"""MXFP4 codec against a 64-bit restatement.  Codes, scale bytes and decoded bf16 values are compared exactly: the
+"""MXFP4 codec and product against a 64-bit restatement.  Codes, scale bytes and decoded bf16 values are compared exactly: the
 scale is a power of two, so the quotient and the decoded product have no rounding but the one to the E2M1 grid."""
 import pytest
 import torch
 
 import tensorcache_b200 as tc
+from tensorcache_b200.fused_linear import check_device_status
 from tests import low_bit_plain as plain
 from tests import synth
 from tests.util import bits
@@ -128,3 +129,132 @@ def test_more_than_2_31_values():
     out = tc.dequantize_mxfp4(codes, scales, shape)
     assert torch.equal(out[-131:].double(), plain.mx_values(*plain.mx_encode(tail)))
     assert not bool(out[:1000].any()) and not bool(codes[:-131].any())
+
+
+# ------------------------------------------------------------------------------------------------ product
+#
+# Tolerance: code products times powers of two are exact in fp32; adding K of them in fp32, in any order and even with
+# truncation, is off by at most K 2^-23 times the sum of magnitudes; the result is rounded once to bf16 (2^-8 of it).
+
+
+def product_close(got, x, w, bias=None):
+    """x, w: fp64 values of the two operands."""
+    ref, bound = x @ w.t(), x.abs() @ w.abs().t()
+    if bias is not None:
+        ref, bound = ref + bias.double(), bound + bias.double().abs()
+    tol = 2.0 ** -8 * ref.abs() + 1.01 * (x.shape[1] + 1) * 2.0 ** -23 * bound + 2.0 ** -133
+    assert got.dtype == torch.bfloat16 and got.shape == ref.shape
+    off = (got.double() - ref).abs()
+    assert bool((off <= tol).all()), float((off / tol).nan_to_num(0).max())
+
+
+def product_inputs(M, N, K, dtype=torch.bfloat16, seed=0):
+    """Rows and blocks of very different sizes, so that a scale applied to the wrong row or block shows."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(M, K, generator=g, device=DEV) * torch.exp2(torch.randint(-4, 5, (M, K // 32, 1), generator=g, device=DEV).expand(-1, -1, 32).reshape(M, K))
+    w = torch.randn(N, K, generator=g, device=DEV) * torch.exp2(torch.randint(-6, 3, (N, K // 32, 1), generator=g, device=DEV).expand(-1, -1, 32).reshape(N, K))
+    return x.to(dtype), w.to(torch.bfloat16), torch.randn(N, generator=g, device=DEV).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 32), (1, 256, 64), (1, 1000, 4096), (2, 33, 96), (7, 130, 160), (16, 512, 256), (17, 257, 288), (33, 64, 1024),
+                                   (64, 4096, 512), (100, 300, 992), (128, 128, 128), (129, 255, 768), (256, 256, 256), (257, 513, 4128),
+                                   (446, 1001, 768), (1000, 2000, 544)])
+def test_product(M, N, K, dtype):
+    x, w, b = product_inputs(M, N, K, dtype, M + N + K)
+    wq, ws, _ = tc.quantize_mxfp4(w)
+    X, W = plain.mx_values(*plain.mx_encode(x)), plain.mx_values(*plain.mx_encode(w))
+    y = tc.mxfp4_matmul(x, wq, ws)
+    check_device_status()
+    product_close(y, X, W)
+    product_close(tc.mxfp4_matmul(x, wq, ws, bias=b), X, W, b)
+
+
+def test_product_of_the_identity_returns_the_weight():
+    """One non-zero code per row of x, with its own scale: every weight and every scale comes back where it belongs."""
+    K, N = 1024, 700
+    _, w, _ = product_inputs(1, N, K, seed=3)
+    wq, ws, shape = tc.quantize_mxfp4(w)
+    scale = torch.exp2(torch.arange(K, device=DEV) % 13 - 6)
+    y = tc.mxfp4_matmul(torch.diag(scale).to(torch.bfloat16), wq, ws)
+    assert torch.equal(y.double(), (tc.dequantize_mxfp4(wq, ws, shape).double() * scale).t())
+
+
+def test_product_with_many_tiles_per_pair():
+    M, N, K = 5000, 6000, 640
+    x, w, _ = product_inputs(M, N, K, seed=4)
+    wq, ws, _ = tc.quantize_mxfp4(w)
+    y = tc.mxfp4_matmul(x, wq, ws)
+    check_device_status()
+    product_close(y, plain.mx_values(*plain.mx_encode(x)), plain.mx_values(*plain.mx_encode(w)))
+
+
+def test_product_leading_dimensions_strides_empty_and_zero_rows():
+    x, w, b = product_inputs(12, 40, 96, seed=5)
+    wq, ws, _ = tc.quantize_mxfp4(w)
+    ref = tc.mxfp4_matmul(x, wq, ws, b)
+    assert torch.equal(tc.mxfp4_matmul(x.view(2, 3, 2, 96), wq, ws, b), ref.view(2, 3, 2, 40))
+    assert torch.equal(tc.mxfp4_matmul(x.t().contiguous().t(), wq, ws, b), ref)
+    assert tc.mxfp4_matmul(x[0], wq, ws, b).shape == (40,) and torch.equal(tc.mxfp4_matmul(x[0], wq, ws, b), ref[0])
+    shifted = torch.empty(12 * 96 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(12, 96)
+    shifted.copy_(x)
+    odd = [torch.empty(t.numel() + 3, dtype=torch.uint8, device=DEV)[3:] for t in (wq, ws)]
+    odd[0].copy_(wq.view(-1)), odd[1].copy_(ws)
+    assert torch.equal(tc.mxfp4_matmul(shifted, odd[0].view_as(wq), odd[1], b), ref)
+    assert tc.mxfp4_matmul(x[:0], wq, ws, b).shape == (0, 40)
+    assert tc.mxfp4_matmul(x, wq[:0], ws[:0]).shape == (12, 0)
+    x[3] = 0
+    x[4, 5] = float("nan")
+    x[5, 6] = float("inf")
+    y = tc.mxfp4_matmul(x, wq, ws)
+    assert not bool(y[3].any()) and bool(y.isfinite().all())
+    product_close(y, plain.mx_values(*plain.mx_encode(x)), plain.mx_values(*plain.mx_encode(w)))
+
+
+def test_product_captured_and_replayed():
+    x, w, b = product_inputs(40, 300, 512, seed=6)
+    wq, ws, _ = tc.quantize_mxfp4(w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        tc.mxfp4_matmul(x, wq, ws, b)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(tc.mxfp4_matmul(x, wq, ws, b))
+    for seed in (7, 8):
+        x.copy_(product_inputs(40, 300, 512, seed=seed)[0])
+        want = tc.mxfp4_matmul(x, wq, ws, b)
+        for graph in graphs:
+            graph.replay()
+        assert all(torch.equal(o, want) for o in outs)
+
+
+def test_product_refusals_on_the_gpu():
+    x, w, b = product_inputs(4, 8, 64)
+    wq, ws, _ = tc.quantize_mxfp4(w)
+    with pytest.raises(ValueError, match="no gradient"):
+        tc.mxfp4_matmul(x.clone().requires_grad_(True), wq, ws)
+    with torch.no_grad():
+        tc.mxfp4_matmul(x.clone().requires_grad_(True), wq, ws)
+    with pytest.raises(ValueError, match="x is on"):
+        tc.mxfp4_matmul(x.cpu(), wq, ws)
+    with pytest.raises(ValueError, match="bias"):
+        tc.mxfp4_matmul(x, wq, ws, b.cpu())
+
+
+def test_features_through_4_and_8_bits_together():
+    """The operators as a program strings them: rows into the device cache, gathered, a head trained on their codes, the
+    trained head stored in 4 bits and applied to the decoded rows."""
+    cache = tc.DeviceFeatureCache(256, 64, 32, DEV)
+    cache.write(torch.arange(256, device=DEV), torch.randn(256, 64, device=DEV))
+    pick = torch.randperm(256, device=DEV)[:100]
+    w = torch.randn(16, 64, device=DEV).to(torch.bfloat16).requires_grad_(True)
+    y = tc.fused_dequant_linear(cache.codes[pick], cache.scales[pick], w)
+    (dw,) = torch.autograd.grad(y, [w], y.detach())
+    trained = (w - 0.01 * dw).detach()
+    wq, ws, _ = tc.quantize_mxfp4(trained)
+    rows = cache.read(pick)
+    product_close(tc.mxfp4_matmul(rows, wq, ws), plain.mx_values(*plain.mx_encode(rows)), plain.mx_values(*plain.mx_encode(trained)))

@@ -36,6 +36,32 @@ def test_library_refuses_bad_arguments_before_any_device_work(built_lib):
     assert L.tcb_cache_read(p, p, 10, 64, 32, p, 0, p, None) == _lib.TCB_OK
 
 
+def test_mxfp4_product_refusals(built_lib):
+    from tensorcache_b200 import _lib
+
+    L, p = built_lib, 1 << 20
+    need = L.tcb_mxfp4_linear_workspace(4, 64)
+    assert need == 512 + 512 and L.tcb_mxfp4_linear_workspace(0, 64) == 0
+    f = lambda *a: L.tcb_mxfp4_linear(*a, None)  # noqa: E731
+    assert f(None, 0, None, None, None, None, 0, 8, 64, None, 0) == _lib.TCB_OK
+    assert f(p, 3, p, p, None, p, 4, 8, 64, p, need) == _lib.ERR_BAD_ARG            # dtype
+    assert f(p, 0, p, p, None, p, 4, 8, 48, p, need) == _lib.ERR_BAD_ARG            # K % 32
+    assert f(p, 0, p, p, None, p, 4, -8, 64, p, need) == _lib.ERR_BAD_ARG
+    assert f(p, 0, None, p, None, p, 4, 8, 64, p, need) == _lib.ERR_BAD_ARG
+    assert f(p + 8, 0, p, p, None, p, 4, 8, 64, p, need) == _lib.ERR_ALIGNMENT
+    assert f(p, 0, p, p, None, p + 1, 4, 8, 64, p, need) == _lib.ERR_ALIGNMENT
+    assert f(p, 0, p, p, None, p, 4, 8, 64, p, need - 1) == _lib.ERR_BAD_ARG        # workspace
+    assert f(p, 0, p, p, None, p, 1 << 31, 8, 64, p, need) == _lib.ERR_TOO_LARGE
+    x, wq, ws = torch.zeros(4, 64), torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8)
+    for bad, match in (((x[:, :32], wq, ws), "inner dimensions"), ((x, wq.view(-1), ws), "wq"), ((x, wq, ws[:-1]), "scales"),
+                       ((x, wq.to(torch.int8), ws), "uint8"), ((x.double(), wq, ws), "fp32"), ((x, wq, ws, torch.zeros(8)), "bias"),
+                       ((x.clone().requires_grad_(True), wq, ws), "no gradient")):
+        with pytest.raises(ValueError, match=match):
+            tc.mxfp4_matmul(*bad)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        tc.mxfp4_matmul(x, wq, ws)
+
+
 def test_mxfp4_refusals():
     with pytest.raises(ValueError, match="multiple of 32"):
         tc.quantize_mxfp4(torch.zeros(4, 33))
