@@ -246,27 +246,28 @@ TCB_API int tcb_fused_dequant_linear(const uint16_t* dense, const uint8_t* q, co
 /*
  * Training step of a linear layer whose input is kept as 8-bit codes (tcgen05; fp32 sums, bf16
  * results).  The reference's FusedDequantLinear has no backward pass.
- *   forward      y  [M, N] = x [M, K] . w [N, K]^T (+ bias [N])
- *   grad_input   dx [M, K] = dy [M, N] . w [N, K]
- *   grad_weight  dw [N, K] = dy [M, N]^T . deq(q) [M, K]       db [N] = column sums of dy
+ *   forward   y  [M, N] = x [M, K] . w [N, K]^T (+ bias [N]);  if q is given, also the codes and
+ *             scales of x, as tcb_compress_sym (n_cand == 0) writes them
+ *   backward  dx [M, K] = dy [M, N] . w [N, K]                 if dx is given (needs w)
+ *             dw [N, K] = dy [M, N]^T . deq(q) [M, K]          if dw is given (needs q, scales)
+ *             db [N]    = column sums of dy                    if db is given
  * deq(q) is the bf16 number tcb_decompress_amo / tcb_decompress_sym gives for the codes
- * (zp != NULL: uint8 codes, else signed).  Either of dw and db may be NULL.  All bf16.
+ * (zp != NULL: uint8 codes, else signed).  All other arrays are bf16.
  *   ld_dy      elements between rows of dy: a multiple of 8, at least N
  *   workspace  tcb_linear_workspace(M, N, K) bytes on the current device, 32-byte aligned,
- *              enough for any of the three; used by the call's own work on `stream` only
- * Requirements: K a positive multiple of 8 (forward, grad_input) or of G in {16, 32, 64, 128}
- * (grad_weight); x, w, dy and q 16-byte aligned; M, N arbitrary.  With M == 0 or N == 0 nothing
- * is written.  A contraction that is split over the GPU is added up in a fixed order.
+ *              enough for either call; used by the call's own work on `stream` only
+ * Requirements: K a positive multiple of 8, and of G in {16, 32, 64, 128} where codes are written
+ * or read; x, w, dy and q 16-byte aligned; M, N arbitrary.  With M == 0 or N == 0 nothing is
+ * computed.  A contraction that is split over the GPU is added up in a fixed order.
  */
 TCB_API int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K);
-TCB_API int tcb_linear_forward(const uint16_t* x, const uint16_t* w, const uint16_t* bias_or_null, uint16_t* y, int64_t M,
-                               int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
-TCB_API int tcb_linear_grad_input(const uint16_t* dy, int64_t ld_dy, const uint16_t* w, uint16_t* dx, int64_t M, int64_t N,
-                                  int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
-TCB_API int tcb_linear_grad_weight(const uint16_t* dy, int64_t ld_dy, const uint8_t* q, const uint16_t* scales,
-                                   const uint8_t* zp_or_null, uint16_t* dw_or_null, uint16_t* db_or_null, int64_t M,
-                                   int64_t N, int64_t K, int group_size, void* workspace, int64_t workspace_bytes,
-                                   void* stream);
+TCB_API int tcb_linear_forward(const uint16_t* x, const uint16_t* w, const uint16_t* bias_or_null, uint16_t* y,
+                               uint8_t* q_or_null, uint16_t* scales_or_null, int64_t M, int64_t N, int64_t K,
+                               int group_size, void* workspace, int64_t workspace_bytes, void* stream);
+TCB_API int tcb_linear_backward(const uint16_t* dy, int64_t ld_dy, const uint16_t* w_or_null, const uint8_t* q_or_null,
+                                const uint16_t* scales_or_null, const uint8_t* zp_or_null, uint16_t* dx_or_null,
+                                uint16_t* dw_or_null, uint16_t* db_or_null, int64_t M, int64_t N, int64_t K,
+                                int group_size, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Reads (and clears) the per-device status words the fused GEMM, the tcb_linear_*
  * and the MXFP4 product kernels write when a bounded wait runs out.  Synchronises `stream`.  Returns TCB_OK or TCB_ERR_TIMEOUT. */

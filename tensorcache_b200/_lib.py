@@ -6,8 +6,11 @@ library's own message.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from pathlib import Path
+
+import torch
 
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = _PKG / "libtcb200.so"
@@ -66,9 +69,8 @@ SIGNATURES = {
     "tcb_cache_read": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp]),
     "tcb_fused_dequant_linear": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
     "tcb_linear_workspace": (_i64, [_i64, _i64, _i64]),
-    "tcb_linear_forward": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
-    "tcb_linear_grad_input": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
-    "tcb_linear_grad_weight": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
+    "tcb_linear_forward": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
+    "tcb_linear_backward": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
     "tcb_fused_dequant_linear_check": (_i32, [_vp]),
     "tcb_selftest_bounded_wait": (_i32, [_i32, _vp]),
     "tcb_gather_rows": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64, _i32]),
@@ -85,6 +87,24 @@ SIGNATURES = {
 }
 
 _lib = None
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """``torch.cuda.device(device)``, or nothing where that device is the current one already (it nearly always is, and
+    a call of a few microseconds notices the difference)."""
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+def stream_of(device: torch.device) -> int:
+    """Raw handle of the current stream of ``device``."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def address(t):
+    """Data pointer for a ``void*`` argument (None: null)."""
+    return None if t is None else t.data_ptr()
+
 
 
 class TcbError(RuntimeError):

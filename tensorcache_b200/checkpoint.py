@@ -11,8 +11,8 @@ tiles is split over the GPU and added in a fixed order, so results do not change
 """
 from __future__ import annotations
 
-import ctypes
 import math
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -20,7 +20,6 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .codec import _ptr, quantize_int8_g32
 from .fused_linear import SUPPORTED_GROUP_SIZES, _aligned, _check_common, _launch
 
 
@@ -42,61 +41,70 @@ def _check_layer(weight: torch.Tensor, bias: Optional[torch.Tensor], K: int, dev
 
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
-    return _aligned(t.detach().contiguous())
+    return _aligned(t.contiguous())
 
 
-class _Workspace:
-    """Scratch of one call's kernels (split sums), from the caching allocator of the current stream."""
-
-    def __init__(self, M: int, N: int, K: int, device: torch.device):
-        self.bytes = _lib.lib().tcb_linear_workspace(M, N, K)
-        self.buffer = torch.empty(self.bytes, dtype=torch.uint8, device=device)
-
-    def args(self):
-        return _ptr(self.buffer), self.bytes
+@lru_cache(maxsize=1024)
+def _workspace_bytes(M: int, N: int, K: int, device_index: int) -> int:
+    """Scratch bytes of a step of these sizes (they depend on the device's number of SMs)."""
+    return _lib.lib().tcb_linear_workspace(M, N, K)
 
 
-def _dy_operand(dy: torch.Tensor):
-    """``[M, N]`` contiguous, 16-byte aligned, with rows a multiple of 8 elements apart (a copy only if N is not)."""
-    N = dy.shape[1]
-    if N % 8 == 0:
-        return _operand(dy), N
-    ld = -(-N // 8) * 8
-    padded = torch.zeros((dy.shape[0], ld), dtype=dy.dtype, device=dy.device)
-    padded[:, :N] = dy
-    return padded, ld
+def _workspace(M: int, N: int, K: int, device: torch.device):
+    """(buffer or None, bytes): the split sums of one call, from the caching allocator of the current stream."""
+    nbytes = _workspace_bytes(M, N, K, device.index)
+    return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None), nbytes
 
 
-def _grad_weight(dy: torch.Tensor, ld: int, q: Optional[torch.Tensor], scales: Optional[torch.Tensor], zp: Optional[torch.Tensor],
-                 sizes, group_size: int, need_dw: bool, need_db: bool, ws: _Workspace, stream):
-    """``(dw or None, db or None)`` from a padded ``dy`` and the kept codes."""
+def _backward(dy: torch.Tensor, sizes, weight, q, scales, zp, group_size: int, need_dx: bool, need_dw: bool, need_db: bool):
+    """``(dx, dw, db)`` of a layer, None where not needed; ``dx`` is ``[M, K]``."""
     M, N, K = sizes
-    make = torch.empty if M else torch.zeros
-    dw = make((N, K), dtype=torch.bfloat16, device=dy.device) if need_dw else None
-    db = make(N, dtype=torch.bfloat16, device=dy.device) if need_db else None
-    if M and N and (need_dw or need_db):
-        _lib.check(_lib.lib().tcb_linear_grad_weight(_ptr(dy), ld, _ptr(q), _ptr(scales), _ptr(zp), _ptr(dw), _ptr(db), M, N, K,
-                                                     group_size, *ws.args(), stream))
-    return dw, db
+    dev = dy.device
+    bf16 = torch.bfloat16
+    with _lib.on_device(dev):
+        dy = dy.reshape(M, N)
+        if N % 8 == 0:
+            dy, ld = _operand(dy), N
+        else:       # rows of dy must start on 16-byte boundaries
+            ld = -(-N // 8) * 8
+            padded = torch.zeros((M, ld), dtype=bf16, device=dev)
+            padded[:, :N] = dy
+            dy = padded
+        make = torch.empty if M and N else torch.zeros
+        dx = make((M, K), dtype=bf16, device=dev) if need_dx else None
+        dw = make((N, K), dtype=bf16, device=dev) if need_dw else None
+        db = make(N, dtype=bf16, device=dev) if need_db else None
+        if M and N and (need_dx or need_dw or need_db):
+            ws, nbytes = _workspace(M, N, K, dev)
+            w = _operand(weight) if need_dx else None
+            q = _aligned(q) if need_dw else None
+            adr = _lib.address
+            _lib.check(_lib.lib().tcb_linear_backward(adr(dy), ld, adr(w), adr(q), adr(scales), adr(zp), adr(dx), adr(dw), adr(db),
+                                                      M, N, K, group_size, adr(ws), nbytes, _lib.stream_of(dev)))
+    return dx, dw, db
 
 
 class _CheckpointLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, group_size):
         N, K = weight.shape
+        dev = x.device
         x2 = _operand(x.reshape(-1, K))
         M = x2.shape[0]
-        y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+        y = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+        need_dx, need_dw = ctx.needs_input_grad[:2]
         q = scales = None
-        with torch.cuda.device(x.device):
-            if M and N:
-                w, b = _operand(weight), None if bias is None else bias.detach().contiguous()
-                ws = _Workspace(M, N, K, x.device)
-                stream = ctypes.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)
-                _lib.check(_lib.lib().tcb_linear_forward(_ptr(x2), _ptr(w), _ptr(b), _ptr(y), M, N, K, *ws.args(), stream))
-            if ctx.needs_input_grad[1]:
-                q, scales, _ = quantize_int8_g32(x2, group_size)
-        ctx.save_for_backward(q, scales, weight if ctx.needs_input_grad[0] else None)
+        if need_dw:
+            q = torch.empty(M * K, dtype=torch.int8, device=dev)
+            scales = torch.empty(M * K // group_size, dtype=torch.bfloat16, device=dev)
+        if M and N:
+            with _lib.on_device(dev):
+                w, b = _operand(weight), None if bias is None else bias.contiguous()
+                ws, nbytes = _workspace(M, N, K, dev)
+                adr = _lib.address
+                _lib.check(_lib.lib().tcb_linear_forward(adr(x2), adr(w), adr(b), adr(y), adr(q), adr(scales), M, N, K, group_size,
+                                                         adr(ws), nbytes, _lib.stream_of(dev)))
+        ctx.save_for_backward(q, scales, weight if need_dx else None)
         ctx.x_shape, ctx.sizes, ctx.group_size = x.shape, (M, N, K), group_size
         return y.view(*x.shape[:-1], N)
 
@@ -104,21 +112,9 @@ class _CheckpointLinear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         q, scales, weight = ctx.saved_tensors
-        (M, N, K), dev = ctx.sizes, dy.device
         need_dx, need_dw, need_db, _ = ctx.needs_input_grad
-        dx = None
-        with torch.cuda.device(dev):
-            dy2, ld = _dy_operand(dy.reshape(M, N))
-            ws = _Workspace(M, N, K, dev)
-            stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-            if need_dx:
-                dx = (torch.empty if N else torch.zeros)((M, K), dtype=torch.bfloat16, device=dev)
-                if M and N:
-                    w = _operand(weight)
-                    _lib.check(_lib.lib().tcb_linear_grad_input(_ptr(dy2), ld, _ptr(w), _ptr(dx), M, N, K, *ws.args(), stream))
-                dx = dx.view(ctx.x_shape)
-            dw, db = _grad_weight(dy2, ld, q, scales, None, ctx.sizes, ctx.group_size, need_dw, need_db, ws, stream)
-        return dx, dw, db, None
+        dx, dw, db = _backward(dy, ctx.sizes, weight, q, scales, None, ctx.group_size, need_dx, need_dw, need_db)
+        return dx.view(ctx.x_shape) if need_dx else None, dw, db, None
 
 
 class _FusedDequantLinear(torch.autograd.Function):
@@ -128,7 +124,7 @@ class _FusedDequantLinear(torch.autograd.Function):
         M = q.shape[0]
         y = torch.empty((M, N), dtype=torch.bfloat16, device=q.device)
         if M and N:
-            _launch(weight.detach().contiguous(), q, scales, zp, None if bias is None else bias.detach().contiguous(), y, N, M, K, group_size, False)
+            _launch(weight.contiguous(), q, scales, zp, None if bias is None else bias.contiguous(), y, N, M, K, group_size, False)
         ctx.save_for_backward(q, scales, zp)
         ctx.sizes, ctx.group_size = (M, N, K), group_size
         return y
@@ -137,11 +133,8 @@ class _FusedDequantLinear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         q, scales, zp = ctx.saved_tensors
-        with torch.cuda.device(dy.device):
-            dy2, ld = _dy_operand(dy)
-            ws = _Workspace(*ctx.sizes, dy.device)
-            stream = ctypes.c_void_p(torch.cuda.current_stream(dy.device).cuda_stream)
-            dw, db = _grad_weight(dy2, ld, _aligned(q), scales, zp, ctx.sizes, ctx.group_size, ctx.needs_input_grad[0], ctx.needs_input_grad[1], ws, stream)
+        need_dw, need_db = ctx.needs_input_grad[:2]
+        _, dw, db = _backward(dy, ctx.sizes, None, q, scales, zp, ctx.group_size, False, need_dw, need_db)
         return dw, db, None, None, None, None
 
 

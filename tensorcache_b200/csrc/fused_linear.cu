@@ -52,7 +52,7 @@
 //               table of 32 groups per row that the warp refills itself one table ahead
 //               (global -> registers -> table), so a turn-over needs only a warp sync.
 //   warps 10-17 epilogue, one per TMEM lane quadrant and accumulator:
-//               tcgen05.ld -> (+bias) -> bf16 -> global (32-byte stores)
+//               tcgen05.ld -> (+bias) -> bf16 -> global (32- or 16-byte stores, or rows of 16 values)
 // No TMA multicast anywhere.
 //
 // The dequantised value is bf16((q - zp) * scale), the number the decode kernel produces:
@@ -93,7 +93,7 @@ constexpr uint32_t kStageBytesC = kTileRows * kBlockK;                       // 
 constexpr int kTableGroups = 32;                                             // groups per row in the scale table
 constexpr uint32_t kTableRowBytes = kTableGroups * 4 + 16;                   // 144: the pad spreads 8 rows over all banks
 constexpr uint32_t kTableBytes = kTileRows * kTableRowBytes;                 // 18 KB
-constexpr uint32_t kSmemTiles = kStages * (kStageBytesQ + kStageBytesD + kStageBytesC) + kTableBytes;
+constexpr uint32_t kSmemTiles = kStages * (kStageBytesQ + kStageBytesD + kStageBytesC) + kTableBytes + kNumEpilogueWarps * kStoreStageBytes;
 constexpr uint32_t kSmemBytes = kSmemTiles + 1024 /* alignment slack */ + 256 /* barriers */;
 // ----------------------------------------------------------------------- PTX
 
@@ -229,6 +229,7 @@ fused_dequant_gemm_kernel(const __grid_constant__ CUtensorMap dense_map, const _
     uint8_t* smem_d = smem + kStages * kStageBytesQ;          // kStages x 16 KB, dense operand (TMA)
     uint8_t* smem_c = smem_d + kStages * kStageBytesD;        // kStages x 8 KB, raw codes (TMA)
     uint8_t* smem_t = smem_c + kStages * kStageBytesC;        // 18 KB, scale / zero point tables of the 8 producer warps
+    uint8_t* smem_e = smem_t + kTableBytes;                   // 9 KB, store buffers of the 8 epilogue warps
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemTiles);
     // barrier ids: [0,S) full, [S,2S) empty, [2S,3S) full_c, 3S+{0,1} tmem_full, 3S+{2,3} tmem_empty.
     // full and tmem_empty are used in the leader CTA only (the other CTA arrives on them remotely).
@@ -417,10 +418,9 @@ fused_dequant_gemm_kernel(const __grid_constant__ CUtensorMap dense_map, const _
         // Accumulator h (TMEM columns [256 h, 256 h + 256)) holds, per CTA, 128 rows of the A operand against 256 rows of the
         // B operand.  Dense rows of a tile are split as CTA r: [256 r, 256 r + 256), of which MMA group h took [128 h, +128).
         const int ew = warp & 3;                 // TMEM lane quadrant this warp may read
-        const int r_in_tile = ew * 32 + lane;
         const int64_t rows_a = p.quant_is_a ? p.R_q : p.R_d, rows_b = p.quant_is_a ? p.R_d : p.R_q;
-        const bool out_vec = (rows_b % 16 == 0) && ((reinterpret_cast<uintptr_t>(p.out) & 31) == 0) &&
-                             ((reinterpret_cast<uintptr_t>(p.bias) & 3) == 0);
+        const StoreMode mode = store_mode(p.out, rows_b, p.bias);
+        uint32_t* stage = reinterpret_cast<uint32_t*>(smem_e + (warp - kFirstEpilogueWarp) * kStoreStageBytes);
         uint32_t local_tile = 0;
         bool ok = true;
         for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step, ++local_tile) {
@@ -431,15 +431,15 @@ fused_dequant_gemm_kernel(const __grid_constant__ CUtensorMap dense_map, const _
             tc_fence_after();
             {
                 const int h = (warp - kFirstEpilogueWarp) >> 2;   // one warp per lane quadrant and accumulator
-                // output row of this lane and first output column of accumulator column 0 / 128
-                int64_t row, col_lo, col_hi;
+                // output row of lane 0 and first output column of accumulator column 0 / 128
+                int64_t row0, col_lo, col_hi;
                 const int dense_per_cta = t.half ? kTileRows : kDenseRows;
                 if (p.quant_is_a) {
-                    row = int64_t(t.tq) * kPairRows + int64_t(rank) * kTileRows + r_in_tile;
+                    row0 = int64_t(t.tq) * kPairRows + int64_t(rank) * kTileRows + ew * 32;
                     col_lo = int64_t(t.d_unit) * kPairRows + 128 * h;      // B rows held by CTA 0
                     col_hi = col_lo + dense_per_cta;                        // B rows held by CTA 1
                 } else {
-                    row = int64_t(t.d_unit) * kPairRows + int64_t(rank) * dense_per_cta + 128 * h + r_in_tile;
+                    row0 = int64_t(t.d_unit) * kPairRows + int64_t(rank) * dense_per_cta + 128 * h + ew * 32;
                     col_lo = int64_t(t.tq) * kPairRows;
                     col_hi = col_lo + kTileRows;
                 }
@@ -451,34 +451,7 @@ fused_dequant_gemm_kernel(const __grid_constant__ CUtensorMap dense_map, const _
                     uint32_t v[32];
                     tmem_ld32(taddr0 + uint32_t(c * 32), v);
                     tmem_ld_wait();
-                    if (row < rows_a) {
-                        uint16_t* dst = p.out + row * rows_b + col0;
-                        if (out_vec && col0 + 32 <= rows_b) {
-#pragma unroll
-                            for (int hh = 0; hh < 2; ++hh) {
-                                uint32_t w[8];
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    float a = __uint_as_float(v[16 * hh + 2 * i]), b = __uint_as_float(v[16 * hh + 2 * i + 1]);
-                                    if (p.bias) {
-                                        const uint32_t bb = __ldg(reinterpret_cast<const uint32_t*>(p.bias + col0) + 8 * hh + i);
-                                        a += __uint_as_float(bb << 16);
-                                        b += __uint_as_float(bb & 0xFFFF0000u);
-                                    }
-                                    w[i] = pack_bf16(a, b);
-                                }
-                                st_global_v8(dst + 16 * hh, w);
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (col0 + i < rows_b) {
-                                    float a = __uint_as_float(v[i]);
-                                    if (p.bias) a += __uint_as_float(uint32_t(p.bias[col0 + i]) << 16);
-                                    dst[i] = f32_to_bf16_bits(a);
-                                }
-                        }
-                    }
+                    store_32x32(p.out, rows_b, row0, rows_a, col0, rows_b, p.bias, v, mode, stage);
                 }
             }
             tc_fence_before();

@@ -8,9 +8,8 @@
 // kept input exists as int8 / uint8 codes and group scales only; deq(q) is the bf16 number the decode kernels
 // produce, made in shared memory by producer warps, and never goes to global memory.
 //
-// One kernel serves all three: D[a, b] = sum_c A[a, c] B[b, c] on tiles of 256 x 256 per pair of CTAs
-// (tcgen05.mma.cta_group::2; each CTA stages 128 rows of A and 128 of B), 64 of the contraction per stage.  What
-// differs is which way the operands lie in memory:
+// One kernel serves all three: D[a, b] = sum_c A[a, c] B[b, c] on tiles of a pair of CTAs (tcgen05.mma.cta_group::2),
+// 64 of the contraction per stage.  What differs is which way the operands lie in memory:
 //     forward       A = x  (contraction contiguous)        B = w   (contraction contiguous)
 //     input grad    A = dy (contraction contiguous)        B = w   (rows contiguous)
 //     weight grad   A = dy (rows contiguous)               B = q   (rows contiguous, dequantised)
@@ -18,10 +17,17 @@
 // rows are contiguous as two boxes of 64 contraction steps x 64 rows, in the same swizzle: the tensor core reads either
 // (the "major" bits of the instruction descriptor), so nothing is transposed by anyone.
 //
-// Warps per CTA: 0 TMA, 1 MMA issue (leader CTA) and TMEM, 2-5 epilogue, 6-13 dequantising producers (weight
-// gradient only).  The two 256-column accumulators alternate between tiles, so a tile's epilogue runs under the next
-// one's products.  Where the output has too few tiles to fill the GPU the contraction is split: each part leaves fp32
-// sums in a workspace and a second kernel adds them in a fixed order (results do not depend on timing).
+// Forward and input gradient: tiles of 256 x 256 (each CTA stages 128 rows of A and 128 of B); the two 256-column
+// accumulators alternate between tiles, so a tile's epilogue runs under the next one's products.
+// Weight gradient: tiles of 512 x 256, both accumulators on one tile.  Decoding 128 rows costs the producers and the
+// shared-memory pipe about as long as one 256 x 256 step of MMAs takes (measured with 256 x 256 tiles: 854 us for 16384
+// x 4096 x 4096, 330 us for the products without decoding); used against 512 rows of A it hides behind two of them.
+// A tile whose second half would lie outside runs one half only.
+// Where the output has too few tiles to fill the GPU the contraction is split: each part leaves fp32 sums in a workspace
+// and a second kernel adds them in a fixed order (results do not depend on timing).
+//
+// Warps per CTA: 0 TMA, 1 MMA issue (leader CTA) and TMEM, then four epilogue warps per accumulator of a tile (one per
+// lane quadrant), then eight dequantising producers (weight gradient only).
 //
 // Waits are bounded as in the fused dequantising product; the status word is read by tcb_fused_dequant_linear_check().
 #include <type_traits>
@@ -36,8 +42,7 @@ constexpr int kBlockK = 64;                          // contraction per stage
 constexpr uint32_t kOperandBytes = 128 * 64 * 2;     // 16 KB: one operand, one CTA, one stage
 constexpr uint32_t kCodeBytes = 128 * 64;            // 8 KB of raw codes
 constexpr uint32_t kBoxBytes = 64 * 64 * 2;          // 8 KB: 64 contraction steps x 64 rows
-constexpr int kEpilogueWarps = 4, kProducerWarps = 8;
-constexpr int kFirstEpilogueWarp = 2, kFirstProducerWarp = kFirstEpilogueWarp + kEpilogueWarps;
+constexpr int kProducerWarps = 8, kFirstEpilogueWarp = 2;
 constexpr uint32_t kMaxSmem = 232448;
 
 enum Source { kContraction, kRows, kCodes };         // how an operand lies in memory (kCodes: rows contiguous, 8-bit codes)
@@ -45,9 +50,17 @@ enum Source { kContraction, kRows, kCodes };         // how an operand lies in m
 template <Source B>
 struct Config {
     static constexpr bool kDeq = B == kCodes;
+    static constexpr int kGroups = kDeq ? 2 : 1;             // accumulators per tile = 128-row units of A per CTA
+    static constexpr int kBuffers = 2 / kGroups;             // tiles in flight in tensor memory
+    static constexpr int kTileA = kGroups * kPairRows;       // output rows per tile
+    static constexpr int kEpilogueWarps = 4 * kGroups;
+    static constexpr int kFirstProducerWarp = kFirstEpilogueWarp + kEpilogueWarps;
     static constexpr int kThreads = 32 * (kFirstProducerWarp + (kDeq ? kProducerWarps : 0));
-    static constexpr int kStages = kDeq ? 5 : 6;
-    static constexpr uint32_t kTiles = kStages * (2 * kOperandBytes + (kDeq ? kCodeBytes : 0));
+    static constexpr int kStages = kDeq ? 4 : 6;
+    static constexpr uint32_t kBytesA = kGroups * kOperandBytes;
+    // store buffers of the epilogue; the weight gradient's columns are a multiple of 16 and its output aligned: none
+    static constexpr uint32_t kStore = kDeq ? 0 : kEpilogueWarps * kStoreStageBytes;
+    static constexpr uint32_t kTiles = kStages * (kBytesA + kOperandBytes + (kDeq ? kCodeBytes : 0)) + kStore;
     static constexpr uint32_t kSmem = kTiles + 1024 /* alignment */ + 256 /* barriers */;
     static_assert(kSmem <= kMaxSmem, "shared memory");
 };
@@ -67,10 +80,12 @@ struct Params {
 
 struct Item {
     int ta, tb, split, kb0, kb1;
+    int groups;   // 256-row halves of the tile that hold rows of the output
 };
 
 // Work items: the tiles of split 0, then those of split 1, ...  Tiles run in bands of 8 tile rows, down the band first,
 // so that the tiles in flight share their operands in L2.
+template <int GROUPS>
 __device__ __forceinline__ Item decode_item(const Params& p, int item) {
     Item r;
     r.split = item / p.tiles;
@@ -82,6 +97,7 @@ __device__ __forceinline__ Item decode_item(const Params& p, int item) {
     r.tb = u / height;
     r.kb0 = r.split * p.kb_per_split;
     r.kb1 = r.kb0 + p.kb_per_split < p.num_kb ? r.kb0 + p.kb_per_split : p.num_kb;
+    r.groups = GROUPS == 2 && int64_t(r.ta) * (2 * kPairRows) + kPairRows < p.rows_a ? 2 : 1;
     return r;
 }
 
@@ -136,8 +152,9 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* smem_a = smem;
-    uint8_t* smem_b = smem + S * kOperandBytes;
-    uint8_t* smem_c = smem + 2 * S * kOperandBytes;
+    uint8_t* smem_b = smem_a + S * C::kBytesA;
+    uint8_t* smem_c = smem_b + S * kOperandBytes;
+    uint8_t* smem_e = smem + C::kTiles - C::kStore;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kTiles);
     // barriers: full (leader), empty, full_c (raw codes), accumulator full [2], accumulator empty [2] (leader)
     constexpr int FULL = 0, EMPTY = S, FULL_C = 2 * S, TFULL = 3 * S, TEMPTY = 3 * S + 2;
@@ -161,7 +178,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(TFULL + i), 1);
-            mbar_init(bar(TEMPTY + i), 2 * kEpilogueWarps);
+            mbar_init(bar(TEMPTY + i), 2 * C::kEpilogueWarps);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -183,20 +200,22 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             uint32_t ph = 0;
             bool ok = true;
             for (int item = first; ok && item < p.items; item += step) {
-                const Item t = decode_item(p, item);
-                const int row_a = t.ta * kPairRows + int(rank) * kTileRows, row_b = t.tb * kPairRows + int(rank) * kTileRows;
+                const Item t = decode_item<C::kGroups>(p, item);
+                const int units = t.groups;   // 128-row units of A per CTA
+                const int row_a = t.ta * C::kTileA + int(rank) * units * kTileRows, row_b = t.tb * kPairRows + int(rank) * kTileRows;
                 for (int kb = t.kb0; kb < t.kb1; ++kb) {
                     ok = mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag, abort_peer, (1 << 8) | (EMPTY + s));
                     if (!ok) break;
-                    const uint32_t full = leader_bar(FULL + s);
-                    load_operand<A>(smem_u32(smem_a + s * kOperandBytes), &map_a, row_a, kb * kBlockK, full);
+                    const uint32_t full = leader_bar(FULL + s), dst_a = smem_u32(smem_a) + uint32_t(s) * C::kBytesA;
+                    for (int u = 0; u < units; ++u)
+                        load_operand<A>(dst_a + uint32_t(u) * kOperandBytes, &map_a, row_a + u * kTileRows, kb * kBlockK, full);
                     if constexpr (C::kDeq) {
                         mbar_arrive_expect_tx(bar(FULL_C + s), kCodeBytes);
                         tma_load_2d(smem_u32(smem_c + s * kCodeBytes), &map_b, row_b, kb * kBlockK, bar(FULL_C + s));
                     } else {
                         load_operand<B>(smem_u32(smem_b + s * kOperandBytes), &map_b, row_b, kb * kBlockK, full);
                     }
-                    if (leader) mbar_arrive_expect_tx(bar(FULL + s), (C::kDeq ? 2 : 4) * kOperandBytes);
+                    if (leader) mbar_arrive_expect_tx(bar(FULL + s), 2 * (uint32_t(units) + (C::kDeq ? 0 : 1)) * kOperandBytes);
                     else mbar_arrive_cluster(full);
                     if (++s == S) { s = 0; ph ^= 1; }
                 }
@@ -214,49 +233,60 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             bool ok = true;
             const uint32_t a0 = operand_lo<A != kContraction>(smem_u32(smem_a)), b0 = operand_lo<B != kContraction>(smem_u32(smem_b));
             for (int item = first; ok && item < p.items; item += step, ++local) {
-                const Item t = decode_item(p, item);
-                const int buf = local & 1;
-                ok = mbar_wait(bar(TEMPTY + buf), ((local >> 1) & 1) ^ 1, abort_flag, abort_peer, (2 << 8) | (TEMPTY + buf));
+                const Item t = decode_item<C::kGroups>(p, item);
+                const int buf = local % C::kBuffers;
+                ok = mbar_wait(bar(TEMPTY + buf), ((local / C::kBuffers) & 1) ^ 1, abort_flag, abort_peer, (2 << 8) | (TEMPTY + buf));
                 if (!ok) break;
                 tc_fence_after();
-                for (int kb = t.kb0; kb < t.kb1; ++kb) {
-                    ok = mbar_wait(bar(FULL + s), ph, abort_flag, abort_peer, (2 << 8) | (FULL + s));
-                    if (!ok) break;
-                    tc_fence_after();
-                    umma_x4<kStepA, kStepB>(tmem_base + uint32_t(buf * kPairRows), a0 + uint32_t(s) * (kOperandBytes >> 4),
-                                            b0 + uint32_t(s) * (kOperandBytes >> 4), kIdesc, kb > t.kb0 ? 1u : 0u);
-                    umma_commit_both(bar(EMPTY + s));
-                    if (++s == S) { s = 0; ph ^= 1; }
-                }
+                // once per number of groups, so that the issue sequence of a stage has no branch in it
+                auto sum_up = [&](auto groups_tag) {
+                    for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                        ok = mbar_wait(bar(FULL + s), ph, abort_flag, abort_peer, (2 << 8) | (FULL + s));
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int h = 0; h < decltype(groups_tag)::value; ++h)
+                            umma_x4<kStepA, kStepB>(tmem_base + uint32_t((buf + h) * kPairRows),
+                                                    a0 + (uint32_t(s) * C::kBytesA + uint32_t(h) * kOperandBytes) / 16,
+                                                    b0 + uint32_t(s) * (kOperandBytes / 16), kIdesc, kb > t.kb0 ? 1u : 0u);
+                        umma_commit_both(bar(EMPTY + s));
+                        if (++s == S) { s = 0; ph ^= 1; }
+                    }
+                };
+                if (C::kGroups == 2 && t.groups == 2) sum_up(std::integral_constant<int, C::kGroups>());
+                else sum_up(std::integral_constant<int, 1>());
                 if (ok) umma_commit_both(bar(TFULL + buf));
             }
         }
-    } else if (warp < kFirstProducerWarp) {
+    } else if (warp < C::kFirstProducerWarp) {
         // ---------------------------------------------------------------- epilogue
-        const int quad = warp & 3;   // the TMEM lanes this warp may read
-        const bool vec = (p.rows_b % 16 == 0) && ((reinterpret_cast<uintptr_t>(p.out) & 31) == 0) &&
-                         ((reinterpret_cast<uintptr_t>(p.bias) & 3) == 0);
+        const int quad = warp & 3;                            // the TMEM lanes this warp may read
+        const int group = (warp - kFirstEpilogueWarp) >> 2;   // the accumulator of the tile
+        const StoreMode mode = store_mode(p.out, p.rows_b, p.bias);
+        uint32_t* stage = reinterpret_cast<uint32_t*>(smem_e + (C::kStore ? (warp - kFirstEpilogueWarp) * kStoreStageBytes : 0));
         int local = 0;
         bool ok = true;
         for (int item = first; ok && item < p.items; item += step, ++local) {
-            const Item t = decode_item(p, item);
-            const int buf = local & 1;
-            ok = __all_sync(0xffffffffu, mbar_wait(bar(TFULL + buf), (local >> 1) & 1, abort_flag, abort_peer, (4 << 8) | (TFULL + buf)));
+            const Item t = decode_item<C::kGroups>(p, item);
+            const int buf = local % C::kBuffers;
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait(bar(TFULL + buf), (local / C::kBuffers) & 1, abort_flag, abort_peer, (4 << 8) | (TFULL + buf)));
             if (!ok) break;
             tc_fence_after();
-            const int64_t row = int64_t(t.ta) * kPairRows + int64_t(rank) * kTileRows + quad * 32 + lane;
-            const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(buf * kPairRows);
+            const int64_t row0 = int64_t(t.ta) * C::kTileA + (int64_t(rank) * t.groups + group) * kTileRows + quad * 32;
+            const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + uint32_t((buf + group) * kPairRows);
 #pragma unroll 1
             for (int c = 0; c < kPairRows / 32; ++c) {
                 const int64_t col0 = int64_t(t.tb) * kPairRows + c * 32;
-                if (col0 >= p.rows_b) break;   // warp-uniform
+                if (col0 >= p.rows_b || group >= t.groups) break;   // warp-uniform
                 uint32_t v[32];
                 tmem_ld32(taddr + uint32_t(c * 32), v);
                 tmem_ld_wait();
-                if (row >= p.rows_a) continue;
-                if (p.partial) {
+                if (p.partial == nullptr) {
+                    store_32x32(p.out, p.rows_b, row0, p.rows_a, col0, p.rows_b, p.bias, v, mode, stage);
+                } else if (row0 + lane < p.rows_a) {
                     // ld_partial is a multiple of 8 and padded columns may be written
-                    float* dst = p.partial + (int64_t(t.split) * p.rows_a + row) * p.ld_partial + col0;
+                    float* dst = p.partial + (int64_t(t.split) * p.rows_a + row0 + lane) * p.ld_partial + col0;
 #pragma unroll
                     for (int h = 0; h < 4; ++h)
                         if (col0 + 8 * h < p.rows_b) {
@@ -264,34 +294,6 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 #pragma unroll
                             for (int i = 0; i < 8; ++i) w[i] = v[8 * h + i];
                             st_global_v8(dst + 8 * h, w);
-                        }
-                    continue;
-                }
-                uint16_t* dst = p.out + row * p.rows_b + col0;
-                if (vec) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (col0 + 16 * h >= p.rows_b) continue;
-                        uint32_t w[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float x = __uint_as_float(v[16 * h + 2 * i]), y = __uint_as_float(v[16 * h + 2 * i + 1]);
-                            if (p.bias) {
-                                const uint32_t bb = __ldg(reinterpret_cast<const uint32_t*>(p.bias + col0) + 8 * h + i);
-                                x += __uint_as_float(bb << 16);
-                                y += __uint_as_float(bb & 0xffff0000u);
-                            }
-                            w[i] = pack_bf16(x, y);
-                        }
-                        st_global_v8(dst + 16 * h, w);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (col0 + i < p.rows_b) {
-                            float x = __uint_as_float(v[i]);
-                            if (p.bias) x += __uint_as_float(uint32_t(p.bias[col0 + i]) << 16);
-                            dst[i] = f32_to_bf16_bits(x);
                         }
                 }
             }
@@ -304,35 +306,40 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         // Warp pw takes contraction rows [8 pw, 8 pw + 8) of the stage, a lane 2 x 16 codes of one row: columns
         // 16 kq + 64 h of the CTA's 128 (h = 0, 1).  Rows of odd number read their upper half first, so that neither the
         // reads of codes nor the writes of operand pieces meet in a bank.
-        const int pw = warp - kFirstProducerWarp, r = pw * 8 + (lane >> 2), kq = lane & 3, h0 = r & 1;
+        const int pw = warp - C::kFirstProducerWarp, r = pw * 8 + (lane >> 2), kq = lane & 3, h0 = r & 1;
         const uint32_t piece0 = uint32_t(((2 * kq) ^ (r & 7)) * 16), piece1 = piece0 ^ 16u;
-        const int64_t gpr = p.rows_b >> LOG2_G;
-        // scale and zero point of the lane's two pieces, fetched two stages ahead
-        int pf_item = first, pf_kb = 0;
-        Item pf = decode_item(p, pf_item < p.items ? pf_item : 0);
-        pf_kb = pf.kb0;
+        const int64_t gpr = p.rows_b >> LOG2_G, stage_groups = gpr * kBlockK;
+        // scale and zero point of the lane's two pieces, fetched two stages ahead; g: group of column 0 of the lane's row
+        int pf_item = first, pf_kb = 0, pf_end = 0;
+        int64_t g = 0;
+        int off[2] = {0, 0};          // the pieces' groups in the row; -1: outside
+        auto start = [&]() {
+            const Item t = decode_item<C::kGroups>(p, pf_item);
+            pf_kb = t.kb0;
+            pf_end = t.kb1;
+            g = (int64_t(pf_kb) * kBlockK + r) * gpr;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int64_t k = int64_t(t.tb) * kPairRows + int64_t(rank) * kTileRows + 16 * kq + 64 * (h0 ^ i);
+                off[i] = k < p.rows_b ? int(k >> LOG2_G) : -1;
+            }
+        };
+        start();
         auto fetch = [&](uint32_t (&sz)[2]) {
             sz[0] = sz[1] = 0;
             if (pf_item >= p.items) return;
-            const int64_t m = int64_t(pf_kb) * kBlockK + r;
-            const int64_t col = int64_t(pf.tb) * kPairRows + int64_t(rank) * kTileRows + 16 * kq;
-            if (m < p.contraction) {
+            if (pf_kb * kBlockK + r < p.contraction) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int64_t k = col + 64 * (h0 ^ i);
-                    if (k < p.rows_b) {
-                        const int64_t g = m * gpr + (k >> LOG2_G);
-                        sz[i] = uint32_t(__ldg(p.scales + g)) << 16;
-                        if (HAS_ZP) sz[i] |= __ldg(p.zp + g);
+                for (int i = 0; i < 2; ++i)
+                    if (off[i] >= 0) {
+                        sz[i] = uint32_t(__ldg(p.scales + g + off[i])) << 16;
+                        if (HAS_ZP) sz[i] |= __ldg(p.zp + g + off[i]);
                     }
-                }
             }
-            if (++pf_kb == pf.kb1) {
+            g += stage_groups;
+            if (++pf_kb == pf_end) {
                 pf_item += step;
-                if (pf_item < p.items) {
-                    pf = decode_item(p, pf_item);
-                    pf_kb = pf.kb0;
-                }
+                if (pf_item < p.items) start();
             }
         };
         uint32_t ahead0[2], ahead1[2];
@@ -342,7 +349,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         uint32_t ph = 0;
         bool ok = true;
         for (int item = first; ok && item < p.items; item += step) {
-            const Item t = decode_item(p, item);
+            const Item t = decode_item<C::kGroups>(p, item);
             for (int kb = t.kb0; kb < t.kb1; ++kb) {
                 const uint32_t sz0 = ahead0[0], sz1 = ahead0[1];
                 ahead0[0] = ahead1[0];
@@ -396,7 +403,8 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const float* __restrict_
     }
 }
 
-// Column sums of dy: block (x, y) adds rows y, y + gridDim.y, ... (8 at a time) of 256 columns and leaves fp32 sums.
+// Column sums of dy, bound by reading it once: block (x, y) adds every gridDim.y-th run of 32 rows of 256 columns (a warp
+// per row, four rows ahead) and leaves fp32 sums.
 __global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __restrict__ dy, int64_t rows, int64_t cols, int64_t ld,
                                                           float* __restrict__ partial) {
     __shared__ float acc[8][256];
@@ -404,13 +412,19 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __rest
     const int64_t col = int64_t(blockIdx.x) * 256 + c;
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (col < cols)   // ld is a multiple of 8: a whole 16-byte piece is there
-        for (int64_t row = int64_t(blockIdx.y) * 8 + r; row < rows; row += int64_t(gridDim.y) * 8) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(dy + row * ld + col));
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        for (int64_t row = int64_t(blockIdx.y) * 32 + r; row < rows; row += int64_t(gridDim.y) * 32) {
+            uint4 v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[2 * i] += __uint_as_float(w[i] << 16);
-                s[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+            for (int j = 0; j < 4; ++j)
+                v[j] = row + 8 * j < rows ? __ldg(reinterpret_cast<const uint4*>(dy + (row + 8 * j) * ld + col)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[2 * i] += __uint_as_float(w[i] << 16);
+                    s[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+                }
             }
         }
 #pragma unroll
@@ -423,12 +437,23 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __rest
     if (out_col < cols) partial[int64_t(blockIdx.y) * cols + out_col] = sum;
 }
 
+// A block adds the parts of 32 columns: eight warps take every eighth part, in a fixed order.
 __global__ void __launch_bounds__(256) add_column_sums_kernel(const float* __restrict__ partial, int parts, int64_t cols, uint16_t* __restrict__ out) {
-    const int64_t col = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (col >= cols) return;
+    __shared__ float acc[8][32];
+    const int r = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t col = int64_t(blockIdx.x) * 32 + lane;
     float sum = 0.0f;
-    for (int i = 0; i < parts; ++i) sum += partial[int64_t(i) * cols + col];
-    out[col] = f32_to_bf16_bits(sum);
+    if (col < cols) {
+#pragma unroll 4
+        for (int i = r; i < parts; i += 8) sum += partial[int64_t(i) * cols + col];
+    }
+    acc[r][lane] = sum;
+    __syncthreads();
+    if (r == 0 && col < cols) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) sum += acc[i][lane];
+        out[col] = f32_to_bf16_bits(sum);
+    }
 }
 
 // ------------------------------------------------------------------------ host
@@ -441,9 +466,9 @@ struct Plan {
 };
 
 // Splits the contraction while tiles leave pairs of CTAs idle, but not into parts of fewer than 8 stages.
-Plan make_plan(int64_t rows_a, int64_t rows_b, int64_t contraction) {
+Plan make_plan(int64_t rows_a, int64_t rows_b, int64_t contraction, int tile_a) {
     Plan p;
-    p.tiles_a = (rows_a + kPairRows - 1) / kPairRows;
+    p.tiles_a = (rows_a + tile_a - 1) / tile_a;
     p.tiles_b = (rows_b + kPairRows - 1) / kPairRows;
     p.num_kb = (contraction + kBlockK - 1) / kBlockK;
     const int64_t pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1;
@@ -456,9 +481,13 @@ Plan make_plan(int64_t rows_a, int64_t rows_b, int64_t contraction) {
     return p;
 }
 
+int64_t weight_partial_bytes(int64_t M, int64_t N, int64_t K) {
+    return (make_plan(N, K, M, Config<kCodes>::kTileA).partial_bytes(N) + 31) / 32 * 32;
+}
+
 int column_parts(int64_t rows, int64_t cols) {
     const int64_t across = (cols + 255) / 256, most = (rows + 63) / 64;
-    int64_t parts = (2 * int64_t(tcb::sm_count()) + across - 1) / across;
+    int64_t parts = (8 * int64_t(tcb::sm_count()) + across - 1) / across;
     if (parts > most) parts = most;
     return int(parts < 1 ? 1 : parts);
 }
@@ -493,7 +522,7 @@ int operand_map(const char* who, CUtensorMap* map, const Operand& o) {
 template <Source A, Source B, int LOG2_G, bool HAS_ZP>
 int launch(const char* who, const Operand& a, const Operand& b, const uint16_t* scales, const uint8_t* zp, const uint16_t* bias, uint16_t* out,
            void* workspace, int64_t workspace_bytes, cudaStream_t st) {
-    const Plan plan = make_plan(a.rows, b.rows, a.contraction);
+    const Plan plan = make_plan(a.rows, b.rows, a.contraction, Config<B>::kTileA);
     if (plan.tiles_a * plan.tiles_b * plan.splits > (int64_t(1) << 30)) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: too many output tiles", who);
     if (plan.partial_bytes(a.rows) > workspace_bytes)
         return tcb::fail(TCB_ERR_BAD_ARG, "%s: the workspace holds %lld bytes, %lld are needed", who, (long long)workspace_bytes,
@@ -555,10 +584,11 @@ int check_operands(const char* who, const void* a, const void* b, const void* ou
     return TCB_OK;
 }
 
-int check_ld(const char* who, int64_t ld, int64_t N) {
-    if (ld < N || ld % 8 != 0)
-        return tcb::fail(TCB_ERR_BAD_ARG, "%s: rows of dy are %lld elements apart: a multiple of 8, at least N = %lld, is needed", who,
-                         (long long)ld, (long long)N);
+int check_group(const char* who, int64_t K, int group_size) {
+    if (!tcb::core_group_size_ok(group_size) && group_size != 128)
+        return tcb::fail(TCB_ERR_GROUP_SIZE, "%s: group_size %d not in {16, 32, 64, 128}", who, group_size);
+    if (K % group_size != 0)
+        return tcb::fail(TCB_ERR_BAD_ARG, "%s: K = %lld must be a multiple of the group size %d", who, (long long)K, group_size);
     return TCB_OK;
 }
 
@@ -579,67 +609,69 @@ int take_linear_status(int* status) {
 
 extern "C" int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const int64_t sizes[3] = {make_plan(M, N, K).partial_bytes(M), make_plan(M, K, N).partial_bytes(M),
-                              (make_plan(N, K, M).partial_bytes(N) + 31) / 32 * 32 + column_parts(M, N) * N * 4};
+    const int64_t sizes[3] = {make_plan(M, N, K, kPairRows).partial_bytes(M), make_plan(M, K, N, kPairRows).partial_bytes(M),
+                              weight_partial_bytes(M, N, K) + column_parts(M, N) * N * 4};
     int64_t most = sizes[0];
     for (int i = 1; i < 3; ++i) most = sizes[i] > most ? sizes[i] : most;
     return most;
 }
 
-extern "C" int tcb_linear_forward(const uint16_t* x, const uint16_t* w, const uint16_t* bias_or_null, uint16_t* y, int64_t M, int64_t N, int64_t K,
-                                  void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int tcb_linear_forward(const uint16_t* x, const uint16_t* w, const uint16_t* bias_or_null, uint16_t* y, uint8_t* q_or_null,
+                                  uint16_t* scales_or_null, int64_t M, int64_t N, int64_t K, int group_size, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
     const char* who = "tcb_linear_forward";
     int rc = check_sizes(who, M, N, K);
+    if (rc == TCB_OK && q_or_null) rc = check_group(who, K, group_size);
     if (rc != TCB_OK || M == 0 || N == 0) return rc;
     rc = check_operands(who, x, w, y, bias_or_null, workspace);
     if (rc != TCB_OK) return rc;
+    if (q_or_null) {
+        if (!scales_or_null) return tcb::fail(TCB_ERR_BAD_ARG, "%s: codes without scales", who);
+        rc = tcb_compress_sym(x, TCB_DT_BF16, M * K, group_size, nullptr, 0, reinterpret_cast<int8_t*>(q_or_null), scales_or_null, stream);
+        if (rc != TCB_OK) return rc;
+    }
     return launch<kContraction, kContraction, 0, false>(who, Operand{x, M, K, K}, Operand{w, N, K, K}, nullptr, nullptr, bias_or_null, y, workspace,
                                                         workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int tcb_linear_grad_input(const uint16_t* dy, int64_t ld_dy, const uint16_t* w, uint16_t* dx, int64_t M, int64_t N, int64_t K,
-                                     void* workspace, int64_t workspace_bytes, void* stream) {
-    const char* who = "tcb_linear_grad_input";
+extern "C" int tcb_linear_backward(const uint16_t* dy, int64_t ld_dy, const uint16_t* w_or_null, const uint8_t* q_or_null,
+                                   const uint16_t* scales_or_null, const uint8_t* zp_or_null, uint16_t* dx_or_null, uint16_t* dw_or_null,
+                                   uint16_t* db_or_null, int64_t M, int64_t N, int64_t K, int group_size, void* workspace,
+                                   int64_t workspace_bytes, void* stream) {
+    const char* who = "tcb_linear_backward";
     int rc = check_sizes(who, M, N, K);
-    if (rc == TCB_OK) rc = check_ld(who, ld_dy, N);
+    if (rc == TCB_OK && (ld_dy < N || ld_dy % 8 != 0))
+        rc = tcb::fail(TCB_ERR_BAD_ARG, "%s: rows of dy are %lld elements apart: a multiple of 8, at least N = %lld, is needed", who,
+                       (long long)ld_dy, (long long)N);
+    if (rc == TCB_OK && dw_or_null) rc = check_group(who, K, group_size);
     if (rc != TCB_OK || M == 0 || N == 0) return rc;
-    rc = check_operands(who, dy, w, dx, nullptr, workspace);
+    if (dx_or_null) rc = check_operands(who, dy, w_or_null, dx_or_null, nullptr, workspace);
+    if (rc == TCB_OK && dw_or_null) {
+        if (!scales_or_null) return tcb::fail(TCB_ERR_BAD_ARG, "%s: null pointer", who);
+        rc = check_operands(who, dy, q_or_null, dw_or_null, scales_or_null, workspace);
+    }
+    if (rc == TCB_OK && db_or_null) rc = check_operands(who, dy, dy, db_or_null, nullptr, workspace);
     if (rc != TCB_OK) return rc;
-    return launch<kContraction, kRows, 0, false>(who, Operand{dy, M, N, ld_dy}, Operand{w, K, N, K}, nullptr, nullptr, nullptr, dx, workspace,
-                                                 workspace_bytes, static_cast<cudaStream_t>(stream));
-}
-
-extern "C" int tcb_linear_grad_weight(const uint16_t* dy, int64_t ld_dy, const uint8_t* q, const uint16_t* scales, const uint8_t* zp_or_null,
-                                      uint16_t* dw_or_null, uint16_t* db_or_null, int64_t M, int64_t N, int64_t K, int group_size, void* workspace,
-                                      int64_t workspace_bytes, void* stream) {
-    const char* who = "tcb_linear_grad_weight";
-    int rc = check_sizes(who, M, N, K);
-    if (rc == TCB_OK) rc = check_ld(who, ld_dy, N);
-    if (rc != TCB_OK) return rc;
-    if (dw_or_null && !tcb::core_group_size_ok(group_size) && group_size != 128)
-        return tcb::fail(TCB_ERR_GROUP_SIZE, "%s: group_size %d not in {16, 32, 64, 128}", who, group_size);
-    if (M == 0 || N == 0) return TCB_OK;
-    if (dw_or_null && K % group_size != 0)
-        return tcb::fail(TCB_ERR_BAD_ARG, "%s: K = %lld must be a multiple of the group size %d", who, (long long)K, group_size);
+    const int64_t dw_bytes = weight_partial_bytes(M, N, K);
+    const int parts = column_parts(M, N);
+    if (db_or_null && (!workspace || workspace_bytes < dw_bytes + parts * N * 4))
+        return tcb::fail(TCB_ERR_BAD_ARG, "%s: the workspace holds %lld bytes, %lld are needed", who, (long long)workspace_bytes,
+                         (long long)(dw_bytes + parts * N * 4));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (!dy || (reinterpret_cast<uintptr_t>(dy) & 15)) return tcb::fail(TCB_ERR_BAD_ARG, "%s: dy is null or not 16-byte aligned", who);
-    if (dw_or_null) {
-        if (!scales) return tcb::fail(TCB_ERR_BAD_ARG, "%s: null pointer", who);
-        rc = check_operands(who, dy, q, dw_or_null, scales, workspace);
+    if (dx_or_null) {
+        rc = launch<kContraction, kRows, 0, false>(who, Operand{dy, M, N, ld_dy}, Operand{w_or_null, K, N, K}, nullptr, nullptr, nullptr, dx_or_null,
+                                                   workspace, workspace_bytes, st);
         if (rc != TCB_OK) return rc;
     }
-    const int64_t dw_bytes = (make_plan(N, K, M).partial_bytes(N) + 31) / 32 * 32;
     if (db_or_null) {
-        const int parts = column_parts(M, N);
-        if (!workspace || workspace_bytes < dw_bytes + parts * N * 4 || (reinterpret_cast<uintptr_t>(workspace) & 31))
-            return tcb::fail(TCB_ERR_BAD_ARG, "%s: the workspace is too small or not 32-byte aligned", who);
         float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + dw_bytes);
         column_sums_kernel<<<dim3(unsigned((N + 255) / 256), unsigned(parts)), 256, 0, st>>>(dy, M, N, ld_dy, partial);
-        add_column_sums_kernel<<<unsigned((N + 255) / 256), 256, 0, st>>>(partial, parts, N, db_or_null);
+        add_column_sums_kernel<<<unsigned((N + 31) / 32), 256, 0, st>>>(partial, parts, N, db_or_null);
         TCB_CUDA_TRY(cudaGetLastError());
     }
     if (!dw_or_null) return TCB_OK;
-    const Operand a{dy, N, M, ld_dy}, b{q, K, M, K};
+    const Operand a{dy, N, M, ld_dy}, b{q_or_null, K, M, K};
+    const uint16_t* scales = scales_or_null;
     uint16_t* dw = dw_or_null;
     const uint8_t* zp = zp_or_null;
     switch (group_size) {

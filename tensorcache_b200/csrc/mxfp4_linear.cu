@@ -30,7 +30,8 @@ constexpr uint32_t kScaleBytesB = 2048;            // 256 rows x 8 blocks
 constexpr uint32_t kStageBytes = 2 * kOperandBytes + kScaleBytesA + kScaleBytesB;
 constexpr int kEpilogueWarps = 8, kFirstEpilogueWarp = 2;
 constexpr int kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);
-constexpr uint32_t kSmem = kStages * kStageBytes + 1024 /* alignment */ + 256 /* barriers */;
+constexpr uint32_t kSmemTiles = kStages * kStageBytes + kEpilogueWarps * kStoreStageBytes;
+constexpr uint32_t kSmem = kSmemTiles + 1024 /* alignment */ + 256 /* barriers */;
 constexpr uint32_t kAcc1 = 208, kScaleCols = 464;  // tensor-memory columns
 
 struct Params {
@@ -84,8 +85,8 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     constexpr int S = kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    // a stage: codes of x, codes of w, scales of x, scales of w (1024-byte aligned each)
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S * kStageBytes);
+    // stages (codes of x, codes of w, scales of x, scales of w, 1024-byte aligned each), store buffers, barriers
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemTiles);
     // barriers: full (leader), empty, accumulator full [2], shared columns free (leader)
     constexpr int FULL = 0, EMPTY = S, TFULL = 2 * S, TFREE = 2 * S + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 3);
@@ -187,7 +188,8 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     } else {
         // ---------------------------------------------------------------- epilogue
         const int quad = warp & 3, half = (warp - kFirstEpilogueWarp) >> 2;
-        const bool vec = (p.N % 16 == 0) && ((reinterpret_cast<uintptr_t>(p.out) & 31) == 0) && ((reinterpret_cast<uintptr_t>(p.bias) & 3) == 0);
+        const StoreMode mode = store_mode(p.out, p.N, p.bias);
+        uint32_t* stage = reinterpret_cast<uint32_t*>(smem + S * kStageBytes + (warp - kFirstEpilogueWarp) * kStoreStageBytes);
         int local = 0;
         bool ok = true;
         for (int tile = first; ok && tile < p.tiles; tile += step, ++local) {
@@ -196,7 +198,7 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             ok = __all_sync(0xffffffffu, mbar_wait(bar(TFULL + buf), (local >> 1) & 1, abort_flag, abort_peer, (4 << 8) | (TFULL + buf)));
             if (!ok) break;
             tc_fence_after();
-            const int64_t row = int64_t(t.m) * kPairRows + int64_t(rank) * kTileRows + quad * 32 + lane;
+            const int64_t row0 = int64_t(t.m) * kPairRows + int64_t(rank) * kTileRows + quad * 32;
             const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + (buf ? kAcc1 : 0u);
 #pragma unroll 1
             for (int i = 0; i < 4; ++i) {
@@ -211,34 +213,7 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(leader_bar(TFREE));
                 }
-                if (row >= p.M || col0 >= p.N) continue;
-                uint16_t* dst = p.out + row * p.N + col0;
-                if (vec) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (col0 + 16 * h >= p.N) continue;
-                        uint32_t w[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            float x = __uint_as_float(v[16 * h + 2 * j]), y = __uint_as_float(v[16 * h + 2 * j + 1]);
-                            if (p.bias) {
-                                const uint32_t bb = __ldg(reinterpret_cast<const uint32_t*>(p.bias + col0) + 8 * h + j);
-                                x += __uint_as_float(bb << 16);
-                                y += __uint_as_float(bb & 0xffff0000u);
-                            }
-                            w[j] = pack_bf16(x, y);
-                        }
-                        st_global_v8(dst + 16 * h, w);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (col0 + j < p.N) {
-                            float x = __uint_as_float(v[j]);
-                            if (p.bias) x += __uint_as_float(uint32_t(p.bias[col0 + j]) << 16);
-                            dst[j] = f32_to_bf16_bits(x);
-                        }
-                }
+                if (col0 < p.N) store_32x32(p.out, p.N, row0, p.M, col0, p.N, p.bias, v, mode, stage);
             }
         }
     }

@@ -181,6 +181,70 @@ __device__ __forceinline__ uint16_t f32_to_bf16_bits(float v) {
     return *reinterpret_cast<uint16_t*>(&b);
 }
 
+// ---------------------------------------------------------------------- epilogue stores
+//
+// A warp holds 32 columns of 32 consecutive output rows, one row per lane.  Rows whose start is a multiple of 32 (16) bytes
+// take 32-byte (16-byte) stores straight from the registers; any other row length goes through a small buffer of
+// the warp's own, 8 columns at a time, so that 8 neighbouring lanes write one row (a lane of its own per row would touch
+// 32 sectors with every 2-byte store).
+enum StoreMode { kStaged, kVec16, kVec32 };
+constexpr uint32_t kStoreStageBytes = 32 * 9 * 4;   // per warp: rows of 9 words, so that neither side meets in a bank
+
+__device__ __forceinline__ StoreMode store_mode(const void* out, int64_t ld, const void* bias) {
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out);
+    if (reinterpret_cast<uintptr_t>(bias) & 3) return kStaged;
+    return (ld % 16 == 0 && (o & 31) == 0) ? kVec32 : (ld % 8 == 0 && (o & 15) == 0) ? kVec16 : kStaged;
+}
+
+// Lane l stores bf16(v + bias) to out[row0 + l, col0 .. col0 + 31] as far as that lies inside [rows, cols].  Called by the
+// whole warp; `stage` is the warp's buffer (kStaged only).
+__device__ __forceinline__ void store_32x32(uint16_t* out, int64_t ld, int64_t row0, int64_t rows, int64_t col0, int64_t cols,
+                                            const uint16_t* bias, const uint32_t (&v)[32], StoreMode mode, uint32_t* stage) {
+    const int lane = threadIdx.x & 31;
+    if (mode != kStaged) {
+        if (row0 + lane >= rows) return;
+        uint16_t* dst = out + (row0 + lane) * ld + col0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float a = __uint_as_float(v[16 * h + 2 * i]), b = __uint_as_float(v[16 * h + 2 * i + 1]);
+                if (bias && col0 + 16 * h + 2 * i < cols) {
+                    const uint32_t bb = __ldg(reinterpret_cast<const uint32_t*>(bias + col0) + 8 * h + i);
+                    a += __uint_as_float(bb << 16);
+                    b += __uint_as_float(bb & 0xFFFF0000u);
+                }
+                w[i] = pack_bf16(a, b);
+            }
+            if (mode == kVec32) {   // cols is a multiple of 16
+                if (col0 + 16 * h < cols) st_global_v8(dst + 16 * h, w);
+            } else {                // a multiple of 8
+                if (col0 + 16 * h < cols) *reinterpret_cast<uint4*>(dst + 16 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+                if (col0 + 16 * h + 8 < cols) *reinterpret_cast<uint4*>(dst + 16 * h + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+        }
+        return;
+    }
+    // the bias joins before the one rounding, so the buffer holds fp32
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) stage[lane * 9 + i] = v[8 * g + i];
+        __syncwarp();
+        const int64_t col = col0 + 8 * g + (lane & 7);
+        if (col >= cols) continue;
+        const float b = bias ? __uint_as_float(uint32_t(bias[col]) << 16) : 0.0f;
+        int64_t row = row0 + (lane >> 3);
+        uint16_t* dst = out + row * ld + col;
+        const uint32_t* src = stage + (lane >> 3) * 9 + (lane & 7);
+#pragma unroll
+        for (int i = 0; i < 8; ++i, row += 4, dst += 4 * ld)
+            if (row < rows) *dst = f32_to_bf16_bits(__uint_as_float(src[36 * i]) + b);
+    }
+}
+
 // ---------------------------------------------------------------------- host
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,

@@ -7,14 +7,13 @@ they are written and decoded as they are read, at any row index, with the codec 
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from .codec import _DTYPES, _check_group_size, _ptr
+from .codec import _DTYPES, _check_group_size
 from .fused_linear import _aligned
 
 Indices = Union[torch.Tensor, Sequence[int]]
@@ -62,10 +61,11 @@ class DeviceFeatureCache:
 
     def _indices(self, indices: Indices) -> torch.Tensor:
         idx = torch.as_tensor(indices)
-        if idx.numel() == 0:
-            idx = idx.long()
-        if idx.dim() != 1 or idx.dtype not in (torch.int64, torch.int32):
-            raise ValueError(f"indices must be one-dimensional int64 or int32, got {tuple(idx.shape)} of {idx.dtype}")
+        if idx.dtype is not torch.int64 or idx.dim() != 1:
+            if idx.numel() == 0:
+                idx = idx.long()
+            if idx.dim() != 1 or idx.dtype not in (torch.int64, torch.int32):
+                raise ValueError(f"indices must be one-dimensional int64 or int32, got {tuple(idx.shape)} of {idx.dtype}")
         if idx.is_cuda:
             if idx.device != self.device:
                 raise ValueError(f"indices are on {idx.device}, the cache is on {self.device}")
@@ -80,7 +80,7 @@ class DeviceFeatureCache:
         given on the host that raises ``IndexError``.  Of an index that occurs more than once the last occurrence stays.  Values that are
         not finite are stored as 0.  bf16, fp16 and fp32 are read as they are, other types are converted to fp32.
         """
-        with torch.cuda.device(self.device):
+        with _lib.on_device(self.device):
             idx = self._indices(indices)
             n = idx.numel()
             if tuple(x.shape) not in ((n, *self.row_shape), (n, self.width)):
@@ -89,15 +89,15 @@ class DeviceFeatureCache:
                 raise ValueError(f"x is on {x.device}, the cache is on {self.device}")
             if x.dtype not in _DTYPES:
                 x = x.float()
-            xd = _aligned(x.detach().to(self.device).reshape(n, self.width).contiguous())
-            stream = ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
-            _lib.check(_lib.lib().tcb_cache_write(_ptr(xd), _DTYPES[xd.dtype], _ptr(idx), n, _ptr(self.codes), _ptr(self.scales),
-                                                  self.num_rows, self.width, self.group_size, _ptr(self._claims), stream))
+            xd = _aligned(x.to(self.device).contiguous())
+            _lib.check(_lib.lib().tcb_cache_write(xd.data_ptr(), _DTYPES[xd.dtype], idx.data_ptr(), n, self.codes.data_ptr(),
+                                                  self.scales.data_ptr(), self.num_rows, self.width, self.group_size,
+                                                  self._claims.data_ptr(), _lib.stream_of(self.device)))
 
     def read(self, indices: Indices, out_buffer: Optional[torch.Tensor] = None) -> torch.Tensor:
         """bf16 ``[n, *row_shape]``: row ``indices[t]`` decoded; a row that ``write`` would leave out is zeros.
         If ``out_buffer`` is given it is written in place and returned."""
-        with torch.cuda.device(self.device):
+        with _lib.on_device(self.device):
             idx = self._indices(indices)
             n = idx.numel()
             if out_buffer is None:
@@ -108,9 +108,8 @@ class DeviceFeatureCache:
                 return out_buffer
             direct = out_buffer.device == self.device and out_buffer.is_contiguous() and out_buffer.data_ptr() % 16 == 0
             od = out_buffer if direct else torch.empty(n * self.width, dtype=torch.bfloat16, device=self.device)
-            stream = ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
-            _lib.check(_lib.lib().tcb_cache_read(_ptr(self.codes), _ptr(self.scales), self.num_rows, self.width, self.group_size,
-                                                 _ptr(idx), n, _ptr(od), stream))
+            _lib.check(_lib.lib().tcb_cache_read(self.codes.data_ptr(), self.scales.data_ptr(), self.num_rows, self.width, self.group_size,
+                                                 idx.data_ptr(), n, od.data_ptr(), _lib.stream_of(self.device)))
             if not direct:
                 out_buffer.copy_(od.view(out_buffer.shape))
         return out_buffer

@@ -27,10 +27,6 @@ from . import _lib
 SUPPORTED_GROUP_SIZES = (16, 32, 64, 128)  # group sizes the tensor-core kernel is instantiated for
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return ctypes.c_void_p(t.data_ptr() if t is not None else 0)
-
-
 def _aligned(t: Optional[torch.Tensor], nbytes: int = 16) -> Optional[torch.Tensor]:
     """The TMA descriptors need 16-byte aligned operands.  A contiguous view into a larger tensor (``w[1:]``,
     ``q[3:]``) can start anywhere, so such an operand is copied once; aligned tensors pass through untouched."""
@@ -41,11 +37,10 @@ def _aligned(t: Optional[torch.Tensor], nbytes: int = 16) -> Optional[torch.Tens
 
 def _launch(dense, q, scales, zp, bias, out, R_d, R_q, K, group_size, quant_is_rhs):
     dense, q = _aligned(dense), _aligned(q)
-    dev = dense.device
-    with torch.cuda.device(dev):
-        stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-        _lib.check(_lib.lib().tcb_fused_dequant_linear(_ptr(dense), _ptr(q), _ptr(scales), _ptr(zp), _ptr(bias), _ptr(out),
-                                                       R_d, R_q, K, group_size, 1 if quant_is_rhs else 0, stream))
+    dev, adr = dense.device, _lib.address
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().tcb_fused_dequant_linear(adr(dense), adr(q), adr(scales), adr(zp), adr(bias), adr(out),
+                                                       R_d, R_q, K, group_size, 1 if quant_is_rhs else 0, _lib.stream_of(dev)))
 
 
 def _check_common(codes, scales, zp, K, rows, group_size):

@@ -8,14 +8,13 @@ errors follow ``codec.py``.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from .codec import _DTYPES, _compute_device, _ptr
+from .codec import _DTYPES, _compute_device
 from .fused_linear import _aligned
 
 BLOCK = 32          # values that share a scale
@@ -58,17 +57,6 @@ def mxfp4_scales_from_rows(row_scales: torch.Tensor) -> torch.Tensor:
     return t.view(tr, 4, 32, tk, _TILE_BLOCKS).permute(0, 3, 2, 1, 4).reshape(-1)
 
 
-def _quantize_on_device(x2: torch.Tensor, rows: int, cols: int):
-    """Contiguous CUDA ``[rows, cols]`` -> codes ``[rows, cols / 2]`` and scales, on the current device."""
-    codes = torch.empty((rows, cols // 2), dtype=torch.uint8, device=x2.device)
-    scales = torch.empty(mxfp4_scale_bytes(rows, cols), dtype=torch.uint8, device=x2.device)
-    if codes.numel():
-        x2 = _aligned(x2)
-        stream = ctypes.c_void_p(torch.cuda.current_stream(x2.device).cuda_stream)
-        _lib.check(_lib.lib().tcb_quantize_mxfp4(_ptr(x2), _DTYPES[x2.dtype], rows, cols, _ptr(codes), _ptr(scales), stream))
-    return codes, scales
-
-
 def quantize_mxfp4(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, Tuple[int, ...]]:
     """Encode -> ``(codes uint8 [..., K / 2], scales uint8 [...], orig_shape)`` on ``x.device``.
 
@@ -82,9 +70,13 @@ def quantize_mxfp4(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, Tuple[i
     if x.dtype not in _DTYPES:
         x = x.float()
     dev = _compute_device(x)
-    with torch.cuda.device(dev):
-        codes, scales = _quantize_on_device(x.detach().reshape(rows, cols).contiguous().to(dev), rows, cols)
-    codes = codes.view(*x.shape[:-1], cols // 2)
+    with _lib.on_device(dev):
+        codes = torch.empty((*x.shape[:-1], cols // 2), dtype=torch.uint8, device=dev)
+        scales = torch.empty(mxfp4_scale_bytes(rows, cols), dtype=torch.uint8, device=dev)
+        if codes.numel():
+            xd = _aligned((x if x.is_cuda else x.to(dev)).contiguous())
+            _lib.check(_lib.lib().tcb_quantize_mxfp4(xd.data_ptr(), _DTYPES[x.dtype], rows, cols, codes.data_ptr(), scales.data_ptr(),
+                                                     _lib.stream_of(dev)))
     if not x.is_cuda:
         codes, scales = codes.cpu(), scales.cpu()
     return codes, scales, x.shape
@@ -114,12 +106,11 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, orig_shape: Tupl
         raise ValueError("out_buffer must be a bf16 tensor of the decoded size")
     if out_buffer.numel() == 0:
         return out_buffer
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         cd, sd = _aligned(codes.contiguous().to(dev)), _aligned(scales.contiguous().to(dev))
         direct = out_buffer.device == dev and out_buffer.is_contiguous() and out_buffer.data_ptr() % 16 == 0
         od = out_buffer if direct else torch.empty(rows * cols, dtype=torch.bfloat16, device=dev)
-        stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-        _lib.check(_lib.lib().tcb_dequantize_mxfp4(_ptr(cd), _ptr(sd), rows, cols, _ptr(od), stream))
+        _lib.check(_lib.lib().tcb_dequantize_mxfp4(cd.data_ptr(), sd.data_ptr(), rows, cols, od.data_ptr(), _lib.stream_of(dev)))
         if not direct:
             out_buffer.copy_(od.view(out_buffer.shape))
     return out_buffer
@@ -149,16 +140,15 @@ def mxfp4_matmul(x: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor, bias
         raise ValueError("mxfp4_matmul has no gradient: call it under torch.no_grad() or detach x")
     if not x.is_cuda:
         raise RuntimeError("mxfp4_matmul runs on CUDA tensors only (no CPU fallback)")
-    x2 = x.detach().reshape(-1, K)
-    M = x2.shape[0]
-    out = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    x2 = x.reshape(-1, K)
+    M, dev = x2.shape[0], x.device
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
     if M and N:
-        with torch.cuda.device(x.device):
+        with _lib.on_device(dev):
             x2, cd, sd = _aligned(x2.contiguous()), _aligned(wq.contiguous()), _aligned(w_scales.contiguous())
-            b = None if bias is None else bias.detach().contiguous()
-            L = _lib.lib()
-            nbytes = L.tcb_mxfp4_linear_workspace(M, K)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-            stream = ctypes.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)
-            _lib.check(L.tcb_mxfp4_linear(_ptr(x2), _DTYPES[x2.dtype], _ptr(cd), _ptr(sd), _ptr(b), _ptr(out), M, N, K, _ptr(ws), nbytes, stream))
+            b = None if bias is None else bias.contiguous()
+            nbytes = -(-M * (K // 2) // 512) * 512 + mxfp4_scale_bytes(M, K)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            _lib.check(_lib.lib().tcb_mxfp4_linear(x2.data_ptr(), _DTYPES[x2.dtype], cd.data_ptr(), sd.data_ptr(), _lib.address(b), out.data_ptr(),
+                                                   M, N, K, ws.data_ptr(), nbytes, _lib.stream_of(dev)))
     return out.view(*x.shape[:-1], N)

@@ -128,21 +128,24 @@ def test_linear_entry_points_refuse_bad_arguments(built_lib):
 
     L, p = built_lib, 1 << 20
     fwd = lambda *a: L.tcb_linear_forward(*a, None)  # noqa: E731
-    assert fwd(None, None, None, None, 0, 8, 32, None, 0) == _lib.TCB_OK
-    assert fwd(p, p, None, p, 4, 8, 12, p, 0) == _lib.ERR_BAD_ARG            # K % 8
-    assert fwd(p, p, None, p, 4, -8, 16, p, 0) == _lib.ERR_BAD_ARG
-    assert fwd(None, p, None, p, 4, 8, 16, p, 0) == _lib.ERR_BAD_ARG
-    assert fwd(p + 2, p, None, p, 4, 8, 16, p, 0) == _lib.ERR_ALIGNMENT
-    assert fwd(p, p, p + 1, p, 4, 8, 16, p, 0) == _lib.ERR_ALIGNMENT
-    assert fwd(p, p, None, p, 1 << 31, 8, 16, p, 0) == _lib.ERR_TOO_LARGE
-    gi = lambda *a: L.tcb_linear_grad_input(*a, None)  # noqa: E731
-    assert gi(p, 8, p, p, 4, 16, 32, p, 0) == _lib.ERR_BAD_ARG               # ld < N
-    assert gi(p, 20, p, p, 4, 16, 32, p, 0) == _lib.ERR_BAD_ARG              # ld % 8
-    gw = lambda *a: L.tcb_linear_grad_weight(*a, None)  # noqa: E731
-    assert gw(p, 8, p, p, None, p, None, 4, 8, 32, 24, p, 0) == _lib.ERR_GROUP_SIZE
-    assert gw(p, 8, p, p, None, p, None, 4, 8, 48, 32, p, 0) == _lib.ERR_BAD_ARG
-    assert gw(p, 8, p, None, None, p, None, 4, 8, 32, 32, p, 0) == _lib.ERR_BAD_ARG
-    assert gw(p, 8, p, p, None, None, p, 4, 8, 32, 32, p, 4) == _lib.ERR_BAD_ARG   # workspace too small
+    assert fwd(None, None, None, None, None, None, 0, 8, 32, 32, None, 0) == _lib.TCB_OK
+    assert fwd(p, p, None, p, None, None, 4, 8, 12, 32, p, 0) == _lib.ERR_BAD_ARG            # K % 8
+    assert fwd(p, p, None, p, None, None, 4, -8, 16, 32, p, 0) == _lib.ERR_BAD_ARG
+    assert fwd(None, p, None, p, None, None, 4, 8, 16, 32, p, 0) == _lib.ERR_BAD_ARG
+    assert fwd(p + 2, p, None, p, None, None, 4, 8, 16, 32, p, 0) == _lib.ERR_ALIGNMENT
+    assert fwd(p, p, p + 1, p, None, None, 4, 8, 16, 32, p, 0) == _lib.ERR_ALIGNMENT
+    assert fwd(p, p, None, p, None, None, 1 << 31, 8, 16, 32, p, 0) == _lib.ERR_TOO_LARGE
+    assert fwd(p, p, None, p, p, p, 4, 8, 48, 24, p, 0) == _lib.ERR_GROUP_SIZE
+    assert fwd(p, p, None, p, p, p, 4, 8, 48, 32, p, 0) == _lib.ERR_BAD_ARG                  # K % G
+    assert fwd(p, p, None, p, p, None, 4, 8, 64, 32, p, 0) == _lib.ERR_BAD_ARG               # codes without scales
+    bwd = lambda *a: L.tcb_linear_backward(*a, None)  # noqa: E731
+    assert bwd(p, 8, p, p, p, None, p, p, p, 4, 16, 32, 32, p, 0) == _lib.ERR_BAD_ARG        # ld < N
+    assert bwd(p, 20, p, p, p, None, p, p, p, 4, 16, 32, 32, p, 0) == _lib.ERR_BAD_ARG       # ld % 8
+    assert bwd(p, 8, p, p, p, None, None, p, None, 4, 8, 32, 24, p, 0) == _lib.ERR_GROUP_SIZE
+    assert bwd(p, 8, p, p, p, None, None, p, None, 4, 8, 48, 32, p, 0) == _lib.ERR_BAD_ARG
+    assert bwd(p, 8, p, p, None, None, None, p, None, 4, 8, 32, 32, p, 0) == _lib.ERR_BAD_ARG    # scales missing
+    assert bwd(p, 8, None, p, p, None, p, None, None, 4, 8, 32, 32, p, 0) == _lib.ERR_BAD_ARG    # weight missing
+    assert bwd(p, 8, None, None, None, None, None, None, p, 4, 8, 32, 32, p, 4) == _lib.ERR_BAD_ARG  # workspace too small
     assert L.tcb_linear_workspace(0, 8, 32) == 0 and L.tcb_linear_workspace(4, 8, 32) > 0
 
 
