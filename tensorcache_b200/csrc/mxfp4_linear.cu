@@ -46,14 +46,31 @@ __device__ __forceinline__ constexpr uint32_t inst_desc(uint32_t sf) {
     return (sf << 4) | (1u << 7) | (1u << 10) | (uint32_t(kPairRows >> 3) << 17) | (1u << 23) | (uint32_t(kPairRows >> 7) << 27) | (sf << 29);
 }
 
-__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                                          uint32_t accumulate) {
+// One lane of the warp.  The issuing warp stays converged and only the tensor-core instructions are predicated on this:
+// addresses and descriptors then live in uniform registers, where these instructions want them.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+// The four MMAs of a stage (64 of K = 32 bytes of codes each); the scales of MMAs 2 and 3 sit four (x) and eight (w)
+// columns after those of 0 and 1, within a column the odd ones use the upper half.
+__device__ __forceinline__ void umma_mxf4_x4(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t sfa, uint32_t sfb, uint32_t accumulate_first) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-        "setp.ne.b32 p, %7, 0;\n\t"
+        "{\n\t.reg .pred p, t;\n\t.reg .b64 a, b;\n\t.reg .b32 al, bl, sa, sb;\n\t"
+        "setp.ne.b32 p, %8, 0;\n\t"
+        "setp.eq.b32 t, %8, %8;\n\t"
         "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [%5], [%6], p;\n\t}" ::"r"(d_tmem),
-        "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [%6], [%7], p;\n\t"
+        "add.u32 al, %1, 2;\n\tadd.u32 bl, %2, 2;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %5, [%6], [%7], t;\n\t"
+        "add.u32 al, %1, 4;\n\tadd.u32 bl, %2, 4;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
+        "add.u32 sa, %6, 4;\n\tadd.u32 sb, %7, 8;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [sa], [sb], t;\n\t"
+        "add.u32 al, %1, 6;\n\tadd.u32 bl, %2, 6;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %5, [sa], [sb], t;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(inst_desc(0)), "r"(inst_desc(2)), "r"(sfa), "r"(sfb), "r"(accumulate_first)
         : "memory");
 }
 
@@ -92,7 +109,7 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 3);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
     const uint32_t bar0 = smem_u32(bars), smem0 = smem_u32(smem);
@@ -150,39 +167,41 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issue
-        if (lane == 0 && leader) {
+        if (leader) {
             int s = 0, local = 0;
             uint32_t ph = 0, set = 0;
             bool ok = true;
+            const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            const bool elected = elect_one();
             for (int tile = first; ok && tile < p.tiles; tile += step, ++local) {
                 // the columns the two accumulators share have been read (and with them everything of the tile before that)
-                ok = mbar_wait(bar(TFREE), (local & 1) ^ 1, abort_flag, abort_peer, (2 << 8) | TFREE);
+                ok = __all_sync(0xffffffffu, mbar_wait(bar(TFREE), (local & 1) ^ 1, abort_flag, abort_peer, (2 << 8) | TFREE));
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t d = tmem_base + ((local & 1) ? kAcc1 : 0u);
+                const uint32_t d = tmem + ((local & 1) ? kAcc1 : 0u);
                 for (int kb = 0; kb < p.num_kb; ++kb) {
-                    ok = mbar_wait(bar(FULL + s), ph, abort_flag, abort_peer, (2 << 8) | (FULL + s));
+                    ok = __all_sync(0xffffffffu, mbar_wait(bar(FULL + s), ph, abort_flag, abort_peer, (2 << 8) | (FULL + s)));
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t src = smem0 + uint32_t(s) * kStageBytes;
                     const uint32_t sa = src + 2 * kOperandBytes, sb = sa + kScaleBytesA;
-                    const uint32_t ta = tmem_base + kScaleCols + 24u * set, tb = ta + 8u;
+                    const uint32_t ta = tmem + kScaleCols + 24u * set, tb = ta + 8u;
+                    if (elected) {
 #pragma unroll
-                    for (uint32_t c = 0; c < 2; ++c) {   // 128 of K: four scales a row
-                        copy_scales(ta + 4 * c, sa + 512 * c);
-                        copy_scales(tb + 8 * c, sb + 512 * c);               // rows 0..127 of the tile of w
-                        copy_scales(tb + 8 * c + 4, sb + 1024 + 512 * c);    // rows 128..255
+                        for (uint32_t c = 0; c < 2; ++c) {   // 128 of K: four scales a row
+                            copy_scales(ta + 4 * c, sa + 512 * c);
+                            copy_scales(tb + 8 * c, sb + 512 * c);               // rows 0..127 of the tile of w
+                            copy_scales(tb + 8 * c + 4, sb + 1024 + 512 * c);    // rows 128..255
+                        }
+                        umma_mxf4_x4(d, smem_desc_lo(src), smem_desc_lo(src + kOperandBytes), ta, tb, kb > 0 ? 1u : 0u);
+                        umma_commit_both(bar(EMPTY + s));
                     }
-                    const uint32_t a_lo = smem_desc_lo(src), b_lo = smem_desc_lo(src + kOperandBytes);
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k)     // 64 of K = 32 bytes of codes
-                        umma_mxf4(d, a_lo + 2 * k, b_lo + 2 * k, inst_desc((k & 1) * 2), ta + 4 * (k >> 1), tb + 8 * (k >> 1),
-                                  kb > 0 || k > 0 ? 1u : 0u);
-                    umma_commit_both(bar(EMPTY + s));
+                    __syncwarp();
                     set ^= 1;
                     if (++s == S) { s = 0; ph ^= 1; }
                 }
-                if (ok) umma_commit_both(bar(TFULL + (local & 1)));
+                if (ok && elected) umma_commit_both(bar(TFULL + (local & 1)));
+                __syncwarp();
             }
         }
     } else {
