@@ -39,7 +39,7 @@
 //   warp 0      TMA producer (one thread): raw code tile [128 x 64] uint8 into the CTA's
 //               own barrier, dense tile [256 x 64] bf16 (128-byte swizzle) into the
 //               leader CTA's barrier (cp.async.bulk.tensor with cta_group::2, no multicast)
-//   warp 1      leader CTA only, one thread: per stage ONE barrier wait (dense rows of both
+//   warp 1      leader CTA only, one elected lane: per stage ONE barrier wait (dense rows of both
 //               CTAs landed + all 16 producer warps of the pair done), 8 x tcgen05.mma and
 //               ONE tcgen05.commit that arrives on the stage barrier of both CTAs; after the
 //               last K step one more on both accumulator barriers.  This thread's serial
@@ -236,7 +236,7 @@ fused_dequant_gemm_kernel(const __grid_constant__ CUtensorMap dense_map, const _
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * kStages + 4);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = uniform_warp();
     const int lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();   // 0: leader (issues the MMAs)
     const bool leader = rank == 0;
@@ -302,14 +302,16 @@ fused_dequant_gemm_kernel(const __grid_constant__ CUtensorMap dense_map, const _
         }
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer (leader CTA only)
-        if (lane == 0 && leader) {
+        if (leader) {
             int s = 0;
             uint32_t ph = 0, local_tile = 0;
             bool ok = true;
+            const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            const bool elected = elect_one();
             for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step, ++local_tile) {
                 // both accumulators (TMEM columns [0,256) and [256,512)) belong to this tile: wait until the epilogue has
                 // moved the previous tile out
-                ok = mbar_wait(bar(TEMPTY), (local_tile & 1) ^ 1, abort_flag, abort_peer, (2 << 8) | TEMPTY);
+                ok = __all_sync(0xffffffffu, mbar_wait(bar(TEMPTY), (local_tile & 1) ^ 1, abort_flag, abort_peer, (2 << 8) | TEMPTY));
                 if (!ok) break;
                 tc_fence_after();
                 // the K loop, once per tile kind, so that the issue sequence of a stage has no branch in it
@@ -318,19 +320,22 @@ fused_dequant_gemm_kernel(const __grid_constant__ CUtensorMap dense_map, const _
                     constexpr int kGroups = decltype(groups_tag)::value;   // MMA groups per stage: 2 (wide tile) or 1
                     constexpr bool kQuantIsA = decltype(quant_is_a_tag)::value;
                     for (int kb = 0; kb < num_kb; ++kb) {
-                        ok = mbar_wait(bar(FULL + s), ph, abort_flag, abort_peer, (2 << 8) | (FULL + s));
+                        ok = __all_sync(0xffffffffu, mbar_wait(bar(FULL + s), ph, abort_flag, abort_peer, (2 << 8) | (FULL + s)));
                         if (!ok) break;
                         tc_fence_after();
                         const uint32_t q_lo = q_lo0 + uint32_t(s) * (kStageBytesQ >> 4);
                         const uint32_t d_lo = d_lo0 + uint32_t(s) * (kStageBytesD >> 4);
+                        if (elected) {
 #pragma unroll
-                        for (int h = 0; h < kGroups; ++h) {   // dense rows [128 h, 128 h + 128) of each CTA -> accumulator h
-                            const uint32_t dh = d_lo + uint32_t(h) * ((128u * kBlockK * 2u) >> 4);
-                            umma_bf16_pair_x4(tmem_base + uint32_t(h * kPairRows), kQuantIsA ? q_lo : dh, kQuantIsA ? dh : q_lo, kDescHi,
-                                              kInstrDesc, kb > 0 ? 1u : 0u);
+                            for (int h = 0; h < kGroups; ++h) {   // dense rows [128 h, 128 h + 128) of each CTA -> accumulator h
+                                const uint32_t dh = d_lo + uint32_t(h) * ((128u * kBlockK * 2u) >> 4);
+                                umma_bf16_pair_x4(tmem + uint32_t(h * kPairRows), kQuantIsA ? q_lo : dh, kQuantIsA ? dh : q_lo, kDescHi,
+                                                  kInstrDesc, kb > 0 ? 1u : 0u);
+                            }
+                            // the stage may be refilled, in both CTAs, once these MMAs have read it
+                            umma_commit_both(bar(EMPTY + s));
                         }
-                        // the stage may be refilled, in both CTAs, once these MMAs have read it
-                        umma_commit_both(bar(EMPTY + s));
+                        __syncwarp();
                         if (++s == kStages) { s = 0; ph ^= 1; }
                     }
                 };
@@ -342,7 +347,8 @@ fused_dequant_gemm_kernel(const __grid_constant__ CUtensorMap dense_map, const _
                     if (half) k_loop(std::integral_constant<int, 1>(), std::false_type());
                     else k_loop(std::integral_constant<int, 2>(), std::false_type());
                 }
-                if (ok) umma_commit_both(bar(TFULL));  // accumulators complete: each CTA's epilogue reads its own 128 lanes
+                if (ok && elected) umma_commit_both(bar(TFULL));  // accumulators complete: each CTA's epilogue reads its own 128 lanes
+                __syncwarp();
             }
         }
     } else if (warp < kFirstEpilogueWarp) {

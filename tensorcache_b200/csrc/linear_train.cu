@@ -161,7 +161,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * S + 4);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
     const uint32_t bar0 = smem_u32(bars);
@@ -227,35 +227,42 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issue
-        if (lane == 0 && leader) {
+        if (leader) {
             int s = 0, local = 0;
             uint32_t ph = 0;
             bool ok = true;
+            const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            const bool elected = elect_one();
             const uint32_t a0 = operand_lo<A != kContraction>(smem_u32(smem_a)), b0 = operand_lo<B != kContraction>(smem_u32(smem_b));
             for (int item = first; ok && item < p.items; item += step, ++local) {
                 const Item t = decode_item<C::kGroups>(p, item);
                 const int buf = local % C::kBuffers;
-                ok = mbar_wait(bar(TEMPTY + buf), ((local / C::kBuffers) & 1) ^ 1, abort_flag, abort_peer, (2 << 8) | (TEMPTY + buf));
+                ok = __all_sync(0xffffffffu, mbar_wait(bar(TEMPTY + buf), ((local / C::kBuffers) & 1) ^ 1, abort_flag, abort_peer,
+                                                       (2 << 8) | (TEMPTY + buf)));
                 if (!ok) break;
                 tc_fence_after();
                 // once per number of groups, so that the issue sequence of a stage has no branch in it
                 auto sum_up = [&](auto groups_tag) {
                     for (int kb = t.kb0; kb < t.kb1; ++kb) {
-                        ok = mbar_wait(bar(FULL + s), ph, abort_flag, abort_peer, (2 << 8) | (FULL + s));
+                        ok = __all_sync(0xffffffffu, mbar_wait(bar(FULL + s), ph, abort_flag, abort_peer, (2 << 8) | (FULL + s)));
                         if (!ok) break;
                         tc_fence_after();
+                        if (elected) {
 #pragma unroll
-                        for (int h = 0; h < decltype(groups_tag)::value; ++h)
-                            umma_x4<kStepA, kStepB>(tmem_base + uint32_t((buf + h) * kPairRows),
-                                                    a0 + (uint32_t(s) * C::kBytesA + uint32_t(h) * kOperandBytes) / 16,
-                                                    b0 + uint32_t(s) * (kOperandBytes / 16), kIdesc, kb > t.kb0 ? 1u : 0u);
-                        umma_commit_both(bar(EMPTY + s));
+                            for (int h = 0; h < decltype(groups_tag)::value; ++h)
+                                umma_x4<kStepA, kStepB>(tmem + uint32_t((buf + h) * kPairRows),
+                                                        a0 + (uint32_t(s) * C::kBytesA + uint32_t(h) * kOperandBytes) / 16,
+                                                        b0 + uint32_t(s) * (kOperandBytes / 16), kIdesc, kb > t.kb0 ? 1u : 0u);
+                            umma_commit_both(bar(EMPTY + s));
+                        }
+                        __syncwarp();
                         if (++s == S) { s = 0; ph ^= 1; }
                     }
                 };
                 if (C::kGroups == 2 && t.groups == 2) sum_up(std::integral_constant<int, C::kGroups>());
                 else sum_up(std::integral_constant<int, 1>());
-                if (ok) umma_commit_both(bar(TFULL + buf));
+                if (ok && elected) umma_commit_both(bar(TFULL + buf));
+                __syncwarp();
             }
         }
     } else if (warp < C::kFirstProducerWarp) {

@@ -46,14 +46,6 @@ __device__ __forceinline__ constexpr uint32_t inst_desc(uint32_t sf) {
     return (sf << 4) | (1u << 7) | (1u << 10) | (uint32_t(kPairRows >> 3) << 17) | (1u << 23) | (uint32_t(kPairRows >> 7) << 27) | (sf << 29);
 }
 
-// One lane of the warp.  The issuing warp stays converged and only the tensor-core instructions are predicated on this:
-// addresses and descriptors then live in uniform registers, where these instructions want them.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t p;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
-    return p != 0;
-}
-
 // The four MMAs of a stage (64 of K = 32 bytes of codes each); the scales of MMAs 2 and 3 sit four (x) and eight (w)
 // columns after those of 0 and 1, within a column the odd ones use the upper half.
 __device__ __forceinline__ void umma_mxf4_x4(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t sfa, uint32_t sfb, uint32_t accumulate_first) {
@@ -109,7 +101,7 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 3);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
     const uint32_t bar0 = smem_u32(bars), smem0 = smem_u32(smem);

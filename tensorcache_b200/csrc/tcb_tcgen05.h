@@ -116,6 +116,16 @@ __device__ __forceinline__ void umma_commit_both(uint32_t bar) {
                  : "memory");
 }
 
+// One lane of the warp.  The issuing warp stays converged and only the tensor-core instructions are predicated on this:
+// addresses and descriptors then live in uniform registers, where these instructions want them.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// Index of this warp in the block, as a value the compiler knows to be the same in all lanes.
+__device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0); }
+
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
