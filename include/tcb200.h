@@ -179,7 +179,7 @@ TCB_API int tcb_decompress_sym(const int8_t* q, const uint16_t* scales, uint16_t
  *                                    + r % 32 * 16 + r % 128 / 32 * 4 + b % 4;
  *           padding is written as 0
  *   out     [rows, cols] bf16 bits = code * scale, exact; a scale byte of 255 decodes to NaN
- * cols must be a multiple of 32; all arrays 16-byte aligned.
+ * cols must be a multiple of 32; x and out 32-byte, codes and scales 16-byte aligned.
  */
 TCB_API int tcb_quantize_mxfp4(const void* x, int dtype, int64_t rows, int64_t cols, uint8_t* codes, uint8_t* scales,
                                void* stream);
@@ -192,7 +192,7 @@ TCB_API int tcb_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, in
  * with X = the MXFP4 values of x (quantised by the call, as tcb_quantize_mxfp4 does) and W the
  * values of wq [N, K / 2], w_scales (tile order; no padding byte may be 255: it would be a NaN).
  * No counterpart in the reference.
- *   x [M, K] of `dtype`, 16-byte aligned like wq and w_scales; bias bf16 [N] or NULL;
+ *   x [M, K] of `dtype`, 32-byte aligned; wq, w_scales 16-byte aligned; bias bf16 [N] or NULL;
  *   out [M, N] bf16; workspace: tcb_mxfp4_linear_workspace(M, K) bytes, 16-byte aligned, used by
  *   the call's own work on `stream` only.  K a positive multiple of 32; M, N arbitrary.
  */
@@ -212,7 +212,7 @@ TCB_API int tcb_mxfp4_linear(const void* x, int dtype, const uint8_t* wq, const 
  *           outside [0, num_rows) leaves the cache alone (write) or yields zeros (read).
  *           An index that occurs more than once in one write: the last occurrence stays.
  *   claims  [num_rows + 1] device array of the cache, zeroed once when the cache is made
- * width must be a multiple of G (8, 16, 24, 32, 48, 64 or 128); x, out and codes 16-byte
+ * width must be a multiple of G (8, 16, 24, 32, 48, 64 or 128); x, out and codes 32-byte
  * aligned; n < 2^31.  Writes to one cache must be ordered by the caller (one stream).
  */
 TCB_API int tcb_cache_write(const void* x, int dtype, const int64_t* indices, int64_t n, int8_t* codes, uint16_t* scales,
@@ -254,13 +254,13 @@ TCB_API int tcb_fused_dequant_linear(const uint16_t* dense, const uint8_t* q, co
  * deq(q) is the bf16 number tcb_decompress_amo / tcb_decompress_sym gives for the codes
  * (zp != NULL: uint8 codes, else signed).  All other arrays are bf16.
  *   ld_dy      elements between rows of dy: a multiple of 8, at least N
- *   workspace  tcb_linear_workspace(M, N, K) bytes on the current device, 32-byte aligned,
- *              enough for either call; used by the call's own work on `stream` only
+ *   workspace  tcb_linear_workspace(M, N, K, backward ? 1 : 0) bytes on the current device
+ *              (NULL where that is 0), 32-byte aligned, used by the call's own work only
  * Requirements: K a positive multiple of 8, and of G in {16, 32, 64, 128} where codes are written
  * or read; x, w, dy and q 16-byte aligned; M, N arbitrary.  With M == 0 or N == 0 nothing is
  * computed.  A contraction that is split over the GPU is added up in a fixed order.
  */
-TCB_API int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K);
+TCB_API int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K, int backward);
 TCB_API int tcb_linear_forward(const uint16_t* x, const uint16_t* w, const uint16_t* bias_or_null, uint16_t* y,
                                uint8_t* q_or_null, uint16_t* scales_or_null, int64_t M, int64_t N, int64_t K,
                                int group_size, void* workspace, int64_t workspace_bytes, void* stream);

@@ -68,7 +68,7 @@ SIGNATURES = {
     "tcb_cache_write": (_i32, [_vp, _i32, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp, _vp]),
     "tcb_cache_read": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp]),
     "tcb_fused_dequant_linear": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
-    "tcb_linear_workspace": (_i64, [_i64, _i64, _i64]),
+    "tcb_linear_workspace": (_i64, [_i64, _i64, _i64, _i32]),
     "tcb_linear_forward": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
     "tcb_linear_backward": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
     "tcb_fused_dequant_linear_check": (_i32, [_vp]),

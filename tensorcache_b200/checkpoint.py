@@ -45,19 +45,20 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
 
 
 @lru_cache(maxsize=1024)
-def _workspace_bytes(M: int, N: int, K: int, device_index: int) -> int:
-    """Scratch bytes of a step of these sizes (they depend on the device's number of SMs)."""
-    return _lib.lib().tcb_linear_workspace(M, N, K)
+def _workspace_bytes(M: int, N: int, K: int, backward: int, device_index: int) -> int:
+    """Scratch bytes of a pass of these sizes (they depend on the device's number of SMs)."""
+    return _lib.lib().tcb_linear_workspace(M, N, K, backward)
 
 
-def _workspace(M: int, N: int, K: int, device: torch.device):
+def _workspace(M: int, N: int, K: int, backward: int, device: torch.device):
     """(buffer or None, bytes): the split sums of one call, from the caching allocator of the current stream."""
-    nbytes = _workspace_bytes(M, N, K, device.index)
+    nbytes = _workspace_bytes(M, N, K, backward, device.index)
     return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None), nbytes
 
 
 def _backward(dy: torch.Tensor, sizes, weight, q, scales, zp, group_size: int, need_dx: bool, need_dw: bool, need_db: bool):
-    """``(dx, dw, db)`` of a layer, None where not needed; ``dx`` is ``[M, K]``."""
+    """``(dx, dw, db)`` of a layer, None where not needed; ``dx`` is ``[M, K]``.  ``scales`` None: they follow the codes
+    in ``q``, which is one buffer then."""
     M, N, K = sizes
     dev = dy.device
     bf16 = torch.bfloat16
@@ -75,11 +76,15 @@ def _backward(dy: torch.Tensor, sizes, weight, q, scales, zp, group_size: int, n
         dw = make((N, K), dtype=bf16, device=dev) if need_dw else None
         db = make(N, dtype=bf16, device=dev) if need_db else None
         if M and N and (need_dx or need_dw or need_db):
-            ws, nbytes = _workspace(M, N, K, dev)
+            ws, nbytes = _workspace(M, N, K, 1, dev)
             w = _operand(weight) if need_dx else None
-            q = _aligned(q) if need_dw else None
             adr = _lib.address
-            _lib.check(_lib.lib().tcb_linear_backward(adr(dy), ld, adr(w), adr(q), adr(scales), adr(zp), adr(dx), adr(dw), adr(db),
+            codes = sc = None
+            if need_dw:
+                q = _aligned(q)
+                codes = q.data_ptr()
+                sc = codes + M * K if scales is None else scales.data_ptr()
+            _lib.check(_lib.lib().tcb_linear_backward(dy.data_ptr(), ld, adr(w), codes, sc, adr(zp), adr(dx), adr(dw), adr(db),
                                                       M, N, K, group_size, adr(ws), nbytes, _lib.stream_of(dev)))
     return dx, dw, db
 
@@ -93,27 +98,26 @@ class _CheckpointLinear(torch.autograd.Function):
         M = x2.shape[0]
         y = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
         need_dx, need_dw = ctx.needs_input_grad[:2]
-        q = scales = None
-        if need_dw:
-            q = torch.empty(M * K, dtype=torch.int8, device=dev)
-            scales = torch.empty(M * K // group_size, dtype=torch.bfloat16, device=dev)
+        # codes [M, K], then scales [M, K / G]: one buffer (M K is a multiple of 16, so the scales are aligned)
+        kept = torch.empty(M * K + 2 * (M * K // group_size), dtype=torch.uint8, device=dev) if need_dw else None
         if M and N:
             with _lib.on_device(dev):
                 w, b = _operand(weight), None if bias is None else bias.contiguous()
-                ws, nbytes = _workspace(M, N, K, dev)
+                ws, nbytes = _workspace(M, N, K, 0, dev)
                 adr = _lib.address
-                _lib.check(_lib.lib().tcb_linear_forward(adr(x2), adr(w), adr(b), adr(y), adr(q), adr(scales), M, N, K, group_size,
-                                                         adr(ws), nbytes, _lib.stream_of(dev)))
-        ctx.save_for_backward(q, scales, weight if need_dx else None)
+                q = adr(kept)
+                _lib.check(_lib.lib().tcb_linear_forward(x2.data_ptr(), w.data_ptr(), adr(b), y.data_ptr(), q, q + M * K if need_dw else None,
+                                                         M, N, K, group_size, adr(ws), nbytes, _lib.stream_of(dev)))
+        ctx.save_for_backward(kept, weight if need_dx else None)
         ctx.x_shape, ctx.sizes, ctx.group_size = x.shape, (M, N, K), group_size
-        return y.view(*x.shape[:-1], N)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        q, scales, weight = ctx.saved_tensors
+        kept, weight = ctx.saved_tensors
         need_dx, need_dw, need_db, _ = ctx.needs_input_grad
-        dx, dw, db = _backward(dy, ctx.sizes, weight, q, scales, None, ctx.group_size, need_dx, need_dw, need_db)
+        dx, dw, db = _backward(dy, ctx.sizes, weight, kept, None, None, ctx.group_size, need_dx, need_dw, need_db)
         return dx.view(ctx.x_shape) if need_dx else None, dw, db, None
 
 

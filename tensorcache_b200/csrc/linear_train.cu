@@ -410,20 +410,20 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const float* __restrict_
     }
 }
 
-// Column sums of dy, bound by reading it once: block (x, y) adds every gridDim.y-th run of 32 rows of 256 columns (a warp
-// per row, four rows ahead) and leaves fp32 sums.
+// Column sums of dy, bound by reading it once: block (x, y) takes 64 columns (8 lanes of 16 bytes a row) of every
+// gridDim.y-th run of 128 rows, four rows a thread ahead.  One part: the sums are the result; else they are left as fp32.
 __global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __restrict__ dy, int64_t rows, int64_t cols, int64_t ld,
-                                                          float* __restrict__ partial) {
-    __shared__ float acc[8][256];
-    const int r = threadIdx.x >> 5, c = (threadIdx.x & 31) * 8;
-    const int64_t col = int64_t(blockIdx.x) * 256 + c;
+                                                          float* __restrict__ partial, uint16_t* __restrict__ out) {
+    __shared__ float acc[32][65];
+    const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8;
+    const int64_t col = int64_t(blockIdx.x) * 64 + c;
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (col < cols)   // ld is a multiple of 8: a whole 16-byte piece is there
-        for (int64_t row = int64_t(blockIdx.y) * 32 + r; row < rows; row += int64_t(gridDim.y) * 32) {
+        for (int64_t row = int64_t(blockIdx.y) * 128 + r; row < rows; row += int64_t(gridDim.y) * 128) {
             uint4 v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                v[j] = row + 8 * j < rows ? __ldg(reinterpret_cast<const uint4*>(dy + (row + 8 * j) * ld + col)) : make_uint4(0, 0, 0, 0);
+                v[j] = row + 32 * j < rows ? __ldg(reinterpret_cast<const uint4*>(dy + (row + 32 * j) * ld + col)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
@@ -437,11 +437,13 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __rest
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[r][c + i] = s[i];
     __syncthreads();
+    const int64_t out_col = int64_t(blockIdx.x) * 64 + threadIdx.x;
+    if (threadIdx.x >= 64 || out_col >= cols) return;
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += acc[i][threadIdx.x];
-    const int64_t out_col = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (out_col < cols) partial[int64_t(blockIdx.y) * cols + out_col] = sum;
+    for (int i = 0; i < 32; ++i) sum += acc[i][threadIdx.x];
+    if (gridDim.y == 1) out[out_col] = f32_to_bf16_bits(sum);
+    else partial[int64_t(blockIdx.y) * cols + out_col] = sum;
 }
 
 // A block adds the parts of 32 columns: eight warps take every eighth part, in a fixed order.
@@ -492,11 +494,17 @@ int64_t weight_partial_bytes(int64_t M, int64_t N, int64_t K) {
     return (make_plan(N, K, M, Config<kCodes>::kTileA).partial_bytes(N) + 31) / 32 * 32;
 }
 
+// Parts of the column sums: enough blocks for several per SM, 2048 rows or fewer in one launch of one part.
 int column_parts(int64_t rows, int64_t cols) {
-    const int64_t across = (cols + 255) / 256, most = (rows + 63) / 64;
-    int64_t parts = (8 * int64_t(tcb::sm_count()) + across - 1) / across;
+    if (rows <= 2048) return 1;
+    const int64_t across = (cols + 63) / 64, most = (rows + 511) / 512;
+    int64_t parts = (6 * int64_t(tcb::sm_count()) + across - 1) / across;
     if (parts > most) parts = most;
     return int(parts < 1 ? 1 : parts);
+}
+int64_t column_bytes(int64_t rows, int64_t cols) {
+    const int64_t parts = column_parts(rows, cols);
+    return parts > 1 ? parts * cols * 4 : 0;
 }
 
 // A tensor map over a row-major [outer, inner] array with rows of `ld` elements.
@@ -587,7 +595,8 @@ int check_operands(const char* who, const void* a, const void* b, const void* ou
         return tcb::fail(TCB_ERR_ALIGNMENT, "%s: operands must be 16-byte aligned", who);
     if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) & 1)
         return tcb::fail(TCB_ERR_ALIGNMENT, "%s: bias and output must be 2-byte aligned", who);
-    if (reinterpret_cast<uintptr_t>(workspace) & 31) return tcb::fail(TCB_ERR_ALIGNMENT, "%s: the workspace must be 32-byte aligned", who);
+    if (reinterpret_cast<uintptr_t>(workspace) & 31)
+        return tcb::fail(TCB_ERR_ALIGNMENT, "%s: the workspace must be 32-byte aligned", who);
     return TCB_OK;
 }
 
@@ -614,13 +623,11 @@ int take_linear_status(int* status) {
 }
 }  // namespace tcb
 
-extern "C" int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K) {
+extern "C" int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K, int backward) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const int64_t sizes[3] = {make_plan(M, N, K, kPairRows).partial_bytes(M), make_plan(M, K, N, kPairRows).partial_bytes(M),
-                              weight_partial_bytes(M, N, K) + column_parts(M, N) * N * 4};
-    int64_t most = sizes[0];
-    for (int i = 1; i < 3; ++i) most = sizes[i] > most ? sizes[i] : most;
-    return most;
+    if (!backward) return make_plan(M, N, K, kPairRows).partial_bytes(M);
+    const int64_t dx = make_plan(M, K, N, kPairRows).partial_bytes(M), dw = weight_partial_bytes(M, N, K) + column_bytes(M, N);
+    return dx > dw ? dx : dw;
 }
 
 extern "C" int tcb_linear_forward(const uint16_t* x, const uint16_t* w, const uint16_t* bias_or_null, uint16_t* y, uint8_t* q_or_null,
@@ -661,9 +668,9 @@ extern "C" int tcb_linear_backward(const uint16_t* dy, int64_t ld_dy, const uint
     if (rc != TCB_OK) return rc;
     const int64_t dw_bytes = weight_partial_bytes(M, N, K);
     const int parts = column_parts(M, N);
-    if (db_or_null && (!workspace || workspace_bytes < dw_bytes + parts * N * 4))
+    if (db_or_null && workspace_bytes < dw_bytes + column_bytes(M, N))
         return tcb::fail(TCB_ERR_BAD_ARG, "%s: the workspace holds %lld bytes, %lld are needed", who, (long long)workspace_bytes,
-                         (long long)(dw_bytes + parts * N * 4));
+                         (long long)(dw_bytes + column_bytes(M, N)));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dx_or_null) {
         rc = launch<kContraction, kRows, 0, false>(who, Operand{dy, M, N, ld_dy}, Operand{w_or_null, K, N, K}, nullptr, nullptr, nullptr, dx_or_null,
@@ -672,8 +679,8 @@ extern "C" int tcb_linear_backward(const uint16_t* dy, int64_t ld_dy, const uint
     }
     if (db_or_null) {
         float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + dw_bytes);
-        column_sums_kernel<<<dim3(unsigned((N + 255) / 256), unsigned(parts)), 256, 0, st>>>(dy, M, N, ld_dy, partial);
-        add_column_sums_kernel<<<unsigned((N + 31) / 32), 256, 0, st>>>(partial, parts, N, db_or_null);
+        column_sums_kernel<<<dim3(unsigned((N + 63) / 64), unsigned(parts)), 256, 0, st>>>(dy, M, N, ld_dy, partial, db_or_null);
+        if (parts > 1) add_column_sums_kernel<<<unsigned((N + 31) / 32), 256, 0, st>>>(partial, parts, N, db_or_null);
         TCB_CUDA_TRY(cudaGetLastError());
     }
     if (!dw_or_null) return TCB_OK;

@@ -14,8 +14,8 @@
 //
 // Both kernels are bound by HBM: bf16 in, 2 + 0.5 + 1/32 bytes a value.  One thread block owns one scale tile (128
 // rows x 128 columns): thread (row = t / 4, block = t % 4) takes rows row, row + 32, row + 64 and row + 96, so a warp
-// reads 8 rows x 256 contiguous bytes and has 16 loads of 16 bytes a thread in flight, and the 512 scale bytes of the
-// tile leave as contiguous 16-byte pieces after a 4 x 4 byte transpose over four lanes.
+// reads 8 rows x 256 contiguous bytes with 8 loads of 32 bytes a thread in flight, and the 512 scale bytes of the tile
+// leave as contiguous 16-byte pieces after a 4 x 4 byte transpose over four lanes.
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -28,24 +28,33 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kTileRows = 128, kTileCols = 128;
 
-// One block of 32 values as 16-byte words.
+// Streamed once: 32-byte accesses that leave L2 first.
+__device__ __forceinline__ void ldg_stream_v8(const void* p, uint32_t* w) {
+    asm volatile("ld.global.nc.L1::no_allocate.L2::evict_first.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void stg_stream_v8(void* p, const uint32_t* w) {
+    asm volatile("st.global.L2::evict_first.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+// One block of 32 values.
 template <typename T>
 struct Block32 {
-    static constexpr int kWords = 32 * sizeof(T) / 16;
-    uint4 w[kWords];
+    static constexpr int kWords = 32 * sizeof(T) / 4;
+    uint32_t w[kWords];
 
     __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+        for (int i = 0; i < kWords; i += 8) ldg_stream_v8(reinterpret_cast<const uint32_t*>(p) + i, w + i);
     }
     __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
     }
-    __device__ __forceinline__ uint32_t word(int i) const {
-        const uint4& v = w[i >> 2];
-        return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
-    }
+    __device__ __forceinline__ uint32_t word(int i) const { return w[i]; }
     __device__ __forceinline__ float get(int i) const;
 };
 template <>
@@ -170,7 +179,7 @@ quantize_mxfp4_kernel(const T* __restrict__ x, int64_t rows, int64_t blocks_per_
 
 // Eight codes -> eight bf16 values times 2^(byte - 127).  The magnitudes come from two byte tables (byte permutes
 // that index with the three magnitude bits), the packed product is exact.
-__device__ __forceinline__ void decode8(uint32_t c, __nv_bfloat162 scale, uint32_t (&o)[4]) {
+__device__ __forceinline__ void decode8(uint32_t c, __nv_bfloat162 scale, uint32_t* o) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const uint32_t q = h ? c >> 16 : c;
@@ -213,12 +222,13 @@ dequantize_mxfp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __rest
         const uint32_t s2 = sbits | (sbits << 16);
         const __nv_bfloat162 scale = *reinterpret_cast<const __nv_bfloat162*>(&s2);
         const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
-        uint4* dst = reinterpret_cast<uint4*>(out + (row * blocks_per_row + blk) * 32);
+        uint16_t* dst = out + (row * blocks_per_row + blk) * 32;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            uint32_t o[4];
-            decode8(w[k], scale, o);
-            __stcs(dst + k, make_uint4(o[0], o[1], o[2], o[3]));
+        for (int k = 0; k < 2; ++k) {
+            uint32_t o[8];
+            decode8(w[2 * k], scale, o);
+            decode8(w[2 * k + 1], scale, o + 4);
+            stg_stream_v8(dst + 16 * k, o);
         }
     }
 }
@@ -230,8 +240,8 @@ int check_codec(const char* who, int64_t rows, int64_t cols, const void* a, cons
     if (cols % 32 != 0) return tcb::fail(TCB_ERR_BAD_ARG, "%s: the last dimension (%lld) must be a multiple of 32", who, (long long)cols);
     if (rows == 0 || cols == 0) return TCB_OK;
     if (!a || !codes || !scales) return tcb::fail(TCB_ERR_BAD_ARG, "%s: null pointer", who);
-    if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15)
-        return tcb::fail(TCB_ERR_ALIGNMENT, "%s: all arrays must be 16-byte aligned", who);
+    if ((reinterpret_cast<uintptr_t>(a) & 31) || ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15))
+        return tcb::fail(TCB_ERR_ALIGNMENT, "%s: the values must be 32-byte and codes and scales 16-byte aligned", who);
     const int64_t limit = (int64_t(1) << 31) - 1, tr = (rows + kTileRows - 1) / kTileRows, tk = (cols + kTileCols - 1) / kTileCols;
     if (tr > limit || tk > limit || tr * tk > limit) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: more than 2^31 - 1 tiles of 128 x 128", who);
     *tiles = tr * tk;

@@ -297,8 +297,8 @@ extern "C" int tcb_mxfp4_linear(const void* x, int dtype, const uint8_t* wq, con
     const int64_t tiles_m = (M + kPairRows - 1) / kPairRows, tiles_n = (N + kPairRows - 1) / kPairRows;
     if (tiles_m * tiles_n > (int64_t(1) << 30)) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: too many output tiles", who);
     if (!x || !wq || !w_scales || !out) return tcb::fail(TCB_ERR_BAD_ARG, "%s: null pointer", who);
-    if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(wq) | reinterpret_cast<uintptr_t>(w_scales)) & 15)
-        return tcb::fail(TCB_ERR_ALIGNMENT, "%s: x, the codes and the scales must be 16-byte aligned", who);
+    if ((reinterpret_cast<uintptr_t>(x) & 31) || ((reinterpret_cast<uintptr_t>(wq) | reinterpret_cast<uintptr_t>(w_scales)) & 15))
+        return tcb::fail(TCB_ERR_ALIGNMENT, "%s: x must be 32-byte and codes and scales 16-byte aligned", who);
     if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias_or_null)) & 1)
         return tcb::fail(TCB_ERR_ALIGNMENT, "%s: bias and out must be 2-byte aligned", who);
     if (!workspace || workspace_bytes < tcb_mxfp4_linear_workspace(M, K) || (reinterpret_cast<uintptr_t>(workspace) & 15))

@@ -10,8 +10,9 @@
 // slot with an atomic maximum over (call number << 32 | row).  The call number lives in device memory and is advanced
 // by the write kernel, so that claims need no clearing and a captured graph can be replayed.
 //
-// Both kernels are bound by HBM.  A thread takes V values of one group (G = 8: 8; 16, 32, 64, 128: 16; 24, 48: 24),
-// 1, 2, 4 or 8 neighbouring lanes make up a group and combine max|x| by shuffles.
+// Both kernels are bound by HBM.  A thread takes V values of one group (write: G = 8: 8; 16, 32, 64, 128: 16; 24, 48: 24;
+// read: 32 for G = 32, 64, 128), so that most accesses are 32 bytes; 1 to 8 neighbouring lanes make up a group and combine
+// max|x| by shuffles.  Two units a thread are in flight: each starts with a chain of dependent loads (index, claim, data).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -24,40 +25,83 @@ constexpr int64_t kScanRows = 1024;
 
 template <int G>
 struct Split {
-    static constexpr int V = G == 8 ? 8 : G % 24 == 0 ? 24 : 16;   // values per thread
+    static constexpr int V = G == 8 ? 8 : G % 24 == 0 ? 24 : 16;   // values per thread, write
     static constexpr int LPG = G / V;                              // lanes per group
+    static constexpr int R = G % 32 == 0 ? 32 : V;                 // values per thread, read
 };
 
+// Streamed once: 32-byte accesses that leave L2 first.
+__device__ __forceinline__ void ldg_stream_v8(const void* p, uint32_t* w) {
+    asm volatile("ld.global.nc.L1::no_allocate.L2::evict_first.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void stg_stream_v8(void* p, const uint32_t* w) {
+    asm volatile("st.global.L2::evict_first.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+// BYTES contiguous bytes: 32 at a time where a unit's size keeps them aligned, else 16, else 8.
+template <int BYTES>
+__device__ __forceinline__ void load_bytes(const void* p, uint32_t* w) {
+    if constexpr (BYTES % 32 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 32; ++i) ldg_stream_v8(static_cast<const uint8_t*>(p) + 32 * i, w + 8 * i);
+    } else if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) {
+            const uint4 v = __ldcs(static_cast<const uint4*>(p) + i);
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    } else {
+        static_assert(BYTES % 8 == 0, "units are multiples of 8 bytes");
+#pragma unroll
+        for (int i = 0; i < BYTES / 8; ++i) {
+            const uint2 v = __ldcs(static_cast<const uint2*>(p) + i);
+            w[2 * i] = v.x, w[2 * i + 1] = v.y;
+        }
+    }
+}
+template <int BYTES>
+__device__ __forceinline__ void store_bytes(void* p, const uint32_t* w) {
+    if constexpr (BYTES % 32 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 32; ++i) stg_stream_v8(static_cast<uint8_t*>(p) + 32 * i, w + 8 * i);
+    } else if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) __stcs(static_cast<uint4*>(p) + i, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < BYTES / 8; ++i) __stcs(static_cast<uint2*>(p) + i, make_uint2(w[2 * i], w[2 * i + 1]));
+    }
+}
+
+// Value i of a unit held as packed words.
 template <typename T>
-__device__ __forceinline__ float widen(T v);
+__device__ __forceinline__ float value_of(const uint32_t* w, int i);
 template <>
-__device__ __forceinline__ float widen<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float value_of<__nv_bfloat16>(const uint32_t* w, int i) {
+    return __uint_as_float((i & 1) ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
+}
 template <>
-__device__ __forceinline__ float widen<__half>(__half v) { return __half2float(v); }
+__device__ __forceinline__ float value_of<__half>(const uint32_t* w, int i) {
+    return __half2float(__ushort_as_half(uint16_t((i & 1) ? (w[i >> 1] >> 16) : (w[i >> 1] & 0xffffu))));
+}
 template <>
-__device__ __forceinline__ float widen<float>(float v) { return v; }
+__device__ __forceinline__ float value_of<float>(const uint32_t* w, int i) { return __uint_as_float(w[i]); }
 
 __device__ __forceinline__ bool finite_f32(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 
-// V values of one group (8-value pieces are 16 or 32 bytes and 16-byte aligned) -> codes at q and, from the group's
-// first lane, the scale.  Every lane of the warp calls this; `live` lanes store.
+// The V values of a unit -> codes at q and, from the group's first lane, the scale.  Every lane of the warp calls this;
+// `live` lanes store.
 template <int G, typename T>
-__device__ __forceinline__ void encode_unit(const T* __restrict__ x, bool live, int8_t* __restrict__ q, uint16_t* __restrict__ scale) {
+__device__ __forceinline__ void encode_unit(const uint32_t* raw, bool live, int8_t* __restrict__ q, uint16_t* __restrict__ scale) {
     constexpr int V = Split<G>::V, LPG = Split<G>::LPG;
     float v[V];
-#pragma unroll
-    for (int i = 0; i < V; i += 16 / int(sizeof(T))) {
-        union {
-            uint4 w;
-            T t[16 / sizeof(T)];
-        } u;
-        u.w = live ? __ldcs(reinterpret_cast<const uint4*>(x + i)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < 16 / int(sizeof(T)); ++j) v[i + j] = widen<T>(u.t[j]);
-    }
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
+        v[i] = value_of<T>(raw, i);
         v[i] = finite_f32(v[i]) ? v[i] : 0.0f;
         amax = fmaxf(amax, fabsf(v[i]));
     }
@@ -80,12 +124,7 @@ __device__ __forceinline__ void encode_unit(const T* __restrict__ x, bool live, 
         w[i] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     }
     if (!live) return;
-    if constexpr (V == 16) {
-        __stcs(reinterpret_cast<uint4*>(q), make_uint4(w[0], w[1], w[2], w[3]));
-    } else {
-#pragma unroll
-        for (int i = 0; i < V / 8; ++i) __stcs(reinterpret_cast<uint2*>(q) + i, make_uint2(w[2 * i], w[2 * i + 1]));
-    }
+    store_bytes<V>(q, w);
     if ((threadIdx.x & (LPG - 1)) == 0) *scale = sbits;
 }
 
@@ -113,75 +152,104 @@ write_rows_scan_kernel(const T* __restrict__ x, const int64_t* __restrict__ indi
     for (int64_t u0 = int64_t(blockIdx.y) * kThreads; u0 < units; u0 += int64_t(gridDim.y) * kThreads) {
         const int64_t u = u0 + threadIdx.x;
         const bool live = u < units;
-        encode_unit<G, T>(x + int64_t(t) * width + u * V, live, codes + row * width + u * V, scales + row * (width / G) + u * V / G);
+        uint32_t raw[V * sizeof(T) / 4] = {};
+        if (live) load_bytes<V * int(sizeof(T))>(x + int64_t(t) * width + u * V, raw);
+        encode_unit<G, T>(raw, live, codes + row * width + u * V, scales + row * (width / G) + u * V / G);
     }
 }
 
-// Many rows: units of all rows in one grid-stride loop; a row whose claim did not stay is left out.
-template <int G, typename T>
+// Row and unit of a position in the list of all rows' units; Index is 32 bits wide where that suffices (the division).
+template <typename Index>
+struct Place {
+    Index t, k;
+    __device__ __forceinline__ Place(int64_t u, Index upr) : t(Index(u) / upr), k(Index(u) - t * upr) {}
+};
+
+// Many rows: units of all rows in one grid-stride loop, two at a time; a row whose claim did not stay is left out.
+template <int G, typename T, typename Index>
 __global__ void __launch_bounds__(kThreads)
 write_rows_kernel(const T* __restrict__ x, const int64_t* __restrict__ indices, int64_t n, int8_t* __restrict__ codes,
                   uint16_t* __restrict__ scales, int64_t num_rows, int64_t width, unsigned long long* __restrict__ claims) {
-    constexpr int V = Split<G>::V;
-    const int64_t upr = width / V, units = n * upr;
-    for (int64_t u0 = int64_t(blockIdx.x) * kThreads; u0 < units; u0 += int64_t(gridDim.x) * kThreads) {
-        const int64_t u = u0 + threadIdx.x;
-        int64_t t = 0, k = 0, row = -1;
-        if (u < units) {
-            t = u / upr;
-            k = u - t * upr;
-            row = __ldg(indices + t);
-            if (row >= num_rows || (row >= 0 && uint32_t(claims[row]) != uint32_t(t))) row = -1;
+    constexpr int V = Split<G>::V, kUnits = 2;
+    const Index upr = Index(width / V);
+    const int64_t units = n * int64_t(upr), gpr = width / G;
+    for (int64_t u0 = int64_t(blockIdx.x) * (kThreads * kUnits); u0 < units; u0 += int64_t(gridDim.x) * (kThreads * kUnits)) {
+        int64_t row[kUnits], k[kUnits];
+        uint32_t raw[kUnits][V * sizeof(T) / 4];
+#pragma unroll
+        for (int j = 0; j < kUnits; ++j) {
+            const int64_t u = u0 + j * kThreads + threadIdx.x;
+            row[j] = -1;
+            k[j] = 0;
+#pragma unroll
+            for (int i = 0; i < V * int(sizeof(T)) / 4; ++i) raw[j][i] = 0;
+            if (u < units) {
+                const Place<Index> at(u, upr);
+                row[j] = __ldg(indices + at.t);
+                k[j] = int64_t(at.k);
+                // loaded before the row is known to stay: the claim is one more dependent load
+                load_bytes<V * int(sizeof(T))>(x + u * V, raw[j]);
+                if (row[j] >= num_rows || (row[j] >= 0 && uint32_t(claims[row[j]]) != uint32_t(at.t))) row[j] = -1;
+            }
         }
-        const bool live = row >= 0;
-        encode_unit<G, T>(x + t * width + k * V, live, codes + row * width + k * V, scales + row * (width / G) + k * V / G);
+#pragma unroll
+        for (int j = 0; j < kUnits; ++j)
+            encode_unit<G, T>(raw[j], row[j] >= 0, codes + row[j] * width + k[j] * V, scales + row[j] * gpr + k[j] * V / G);
     }
     // nothing in this launch reads the call number: the claims of the next call get another one
     if (blockIdx.x == 0 && threadIdx.x == 0) claims[num_rows] += 1;
 }
 
-template <int G>
+template <int G, typename Index>
 __global__ void __launch_bounds__(kThreads)
 read_rows_kernel(const int8_t* __restrict__ codes, const uint16_t* __restrict__ scales, int64_t num_rows, int64_t width,
                  const int64_t* __restrict__ indices, int64_t n, uint16_t* __restrict__ out) {
-    constexpr int V = Split<G>::V;
-    const int64_t upr = width / V, units = n * upr;
-    for (int64_t u = int64_t(blockIdx.x) * kThreads + threadIdx.x; u < units; u += int64_t(gridDim.x) * kThreads) {
-        const int64_t t = u / upr, k = u - t * upr, row = __ldg(indices + t);
-        uint32_t c[V / 4];
-        float s = 0.0f;
+    constexpr int R = Split<G>::R, kUnits = 2;
+    const Index upr = Index(width / R);
+    const int64_t units = n * int64_t(upr), gpr = width / G;
+    for (int64_t u0 = int64_t(blockIdx.x) * (kThreads * kUnits) + threadIdx.x; u0 < units; u0 += int64_t(gridDim.x) * (kThreads * kUnits)) {
+        uint32_t c[kUnits][R / 4];
+        float s[kUnits];
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i) c[i] = 0;
-        if (row >= 0 && row < num_rows) {
-            const int8_t* q = codes + row * width + k * V;
-            s = __uint_as_float(uint32_t(__ldg(scales + row * (width / G) + k * V / G)) << 16);
-            if constexpr (V == 16) {
-                const uint4 w = __ldcs(reinterpret_cast<const uint4*>(q));
-                c[0] = w.x, c[1] = w.y, c[2] = w.z, c[3] = w.w;
-            } else {
+        for (int j = 0; j < kUnits; ++j) {
+            const int64_t u = u0 + j * kThreads;
+            s[j] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < V / 8; ++i) {
-                    const uint2 w = __ldcs(reinterpret_cast<const uint2*>(q) + i);
-                    c[2 * i] = w.x, c[2 * i + 1] = w.y;
+            for (int i = 0; i < R / 4; ++i) c[j][i] = 0;
+            if (u < units) {
+                const Place<Index> at(u, upr);
+                const int64_t row = __ldg(indices + at.t), k = int64_t(at.k);
+                if (row >= 0 && row < num_rows) {
+                    s[j] = __uint_as_float(uint32_t(__ldg(scales + row * gpr + k * R / G)) << 16);
+                    load_bytes<R>(codes + row * width + k * R, c[j]);
                 }
             }
         }
-        // code byte + 128 in the mantissa of 2^23, minus (2^23 + 128): the code, exactly; one rounding of the product
-        uint32_t o[V / 2];
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i) {
-            const uint32_t w = c[i] ^ 0x80808080u;
-            float f[4];
+        for (int j = 0; j < kUnits; ++j) {
+            const int64_t u = u0 + j * kThreads;
+            if (u >= units) break;
+            // code byte + 128 in the mantissa of 2^23, minus (2^23 + 128): the code, exactly; one rounding of the product
+            uint32_t o[R / 2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                f[j] = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | j)), 8388736.0f), s);
-            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[2 * i]) : "f"(f[1]), "f"(f[0]));
-            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[2 * i + 1]) : "f"(f[3]), "f"(f[2]));
+            for (int i = 0; i < R / 4; ++i) {
+                const uint32_t w = c[j][i] ^ 0x80808080u;
+                float f[4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                    f[h] = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | h)), 8388736.0f), s[j]);
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[2 * i]) : "f"(f[1]), "f"(f[0]));
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[2 * i + 1]) : "f"(f[3]), "f"(f[2]));
+            }
+            store_bytes<2 * R>(out + u * R, o);
         }
-        uint4* dst = reinterpret_cast<uint4*>(out + t * width + k * V);
-#pragma unroll
-        for (int i = 0; i < V / 8; ++i) __stcs(dst + i, make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
     }
+}
+
+// Blocks of a grid-stride loop over `units` units, two per thread: one wave at most.
+int64_t wave(int64_t units) {
+    const int64_t blocks = (units + 2 * kThreads - 1) / (2 * kThreads), most = int64_t(tcb::sm_count()) * 8;
+    return blocks < most ? blocks : most;
 }
 
 template <int G, typename T>
@@ -196,9 +264,12 @@ cudaError_t launch_write(const void* x, const int64_t* indices, int64_t n, int8_
     }
     unsigned long long* c = reinterpret_cast<unsigned long long*>(claims);
     claim_rows_kernel<<<unsigned((n + kThreads - 1) / kThreads), kThreads, 0, st>>>(indices, n, num_rows, c);
-    const int64_t blocks = (n * upr + kThreads - 1) / kThreads, most = int64_t(tcb::sm_count()) * 8;
-    write_rows_kernel<G, T><<<unsigned(blocks < most ? blocks : most), kThreads, 0, st>>>(static_cast<const T*>(x), indices, n, codes, scales,
-                                                                                         num_rows, width, c);
+    const unsigned grid = unsigned(wave(n * upr));
+    const T* xt = static_cast<const T*>(x);
+    if (n * upr < (int64_t(1) << 32))
+        write_rows_kernel<G, T, uint32_t><<<grid, kThreads, 0, st>>>(xt, indices, n, codes, scales, num_rows, width, c);
+    else
+        write_rows_kernel<G, T, int64_t><<<grid, kThreads, 0, st>>>(xt, indices, n, codes, scales, num_rows, width, c);
     return cudaGetLastError();
 }
 
@@ -215,8 +286,12 @@ cudaError_t launch_write_typed(const void* x, int dtype, const int64_t* indices,
 template <int G>
 cudaError_t launch_read(const int8_t* codes, const uint16_t* scales, int64_t num_rows, int64_t width, const int64_t* indices, int64_t n,
                         uint16_t* out, cudaStream_t st) {
-    const int64_t blocks = (n * (width / Split<G>::V) + kThreads - 1) / kThreads, most = int64_t(tcb::sm_count()) * 8;
-    read_rows_kernel<G><<<unsigned(blocks < most ? blocks : most), kThreads, 0, st>>>(codes, scales, num_rows, width, indices, n, out);
+    const int64_t units = n * (width / Split<G>::R);
+    const unsigned grid = unsigned(wave(units));
+    if (units < (int64_t(1) << 32))
+        read_rows_kernel<G, uint32_t><<<grid, kThreads, 0, st>>>(codes, scales, num_rows, width, indices, n, out);
+    else
+        read_rows_kernel<G, int64_t><<<grid, kThreads, 0, st>>>(codes, scales, num_rows, width, indices, n, out);
     return cudaGetLastError();
 }
 
@@ -230,8 +305,8 @@ int check_cache(const char* who, const void* data, const void* codes, const void
     if (n > (int64_t(1) << 31) - 1) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: more than 2^31 - 1 rows in one call", who);
     if (n == 0 || width == 0) return TCB_OK;
     if (!data || !indices || (num_rows > 0 && (!codes || !scales))) return tcb::fail(TCB_ERR_BAD_ARG, "%s: null pointer", who);
-    if ((reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(codes)) & 15)
-        return tcb::fail(TCB_ERR_ALIGNMENT, "%s: data and codes must be 16-byte aligned", who);
+    if ((reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(codes)) & 31)
+        return tcb::fail(TCB_ERR_ALIGNMENT, "%s: data and codes must be 32-byte aligned", who);
     if ((reinterpret_cast<uintptr_t>(indices) & 7) || (reinterpret_cast<uintptr_t>(scales) & 1))
         return tcb::fail(TCB_ERR_ALIGNMENT, "%s: indices must be 8-byte and scales 2-byte aligned", who);
     return TCB_OK;

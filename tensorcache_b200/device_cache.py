@@ -89,7 +89,7 @@ class DeviceFeatureCache:
                 raise ValueError(f"x is on {x.device}, the cache is on {self.device}")
             if x.dtype not in _DTYPES:
                 x = x.float()
-            xd = _aligned(x.to(self.device).contiguous())
+            xd = _aligned(x.to(self.device).contiguous(), 32)
             _lib.check(_lib.lib().tcb_cache_write(xd.data_ptr(), _DTYPES[xd.dtype], idx.data_ptr(), n, self.codes.data_ptr(),
                                                   self.scales.data_ptr(), self.num_rows, self.width, self.group_size,
                                                   self._claims.data_ptr(), _lib.stream_of(self.device)))
@@ -106,7 +106,7 @@ class DeviceFeatureCache:
                 raise ValueError(f"out_buffer must be a bf16 tensor of {n} rows of {self.width} values")
             if out_buffer.numel() == 0:
                 return out_buffer
-            direct = out_buffer.device == self.device and out_buffer.is_contiguous() and out_buffer.data_ptr() % 16 == 0
+            direct = out_buffer.device == self.device and out_buffer.is_contiguous() and out_buffer.data_ptr() % 32 == 0
             od = out_buffer if direct else torch.empty(n * self.width, dtype=torch.bfloat16, device=self.device)
             _lib.check(_lib.lib().tcb_cache_read(self.codes.data_ptr(), self.scales.data_ptr(), self.num_rows, self.width, self.group_size,
                                                  idx.data_ptr(), n, od.data_ptr(), _lib.stream_of(self.device)))

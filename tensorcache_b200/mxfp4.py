@@ -74,7 +74,7 @@ def quantize_mxfp4(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, Tuple[i
         codes = torch.empty((*x.shape[:-1], cols // 2), dtype=torch.uint8, device=dev)
         scales = torch.empty(mxfp4_scale_bytes(rows, cols), dtype=torch.uint8, device=dev)
         if codes.numel():
-            xd = _aligned((x if x.is_cuda else x.to(dev)).contiguous())
+            xd = _aligned((x if x.is_cuda else x.to(dev)).contiguous(), 32)
             _lib.check(_lib.lib().tcb_quantize_mxfp4(xd.data_ptr(), _DTYPES[x.dtype], rows, cols, codes.data_ptr(), scales.data_ptr(),
                                                      _lib.stream_of(dev)))
     if not x.is_cuda:
@@ -108,7 +108,7 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, orig_shape: Tupl
         return out_buffer
     with _lib.on_device(dev):
         cd, sd = _aligned(codes.contiguous().to(dev)), _aligned(scales.contiguous().to(dev))
-        direct = out_buffer.device == dev and out_buffer.is_contiguous() and out_buffer.data_ptr() % 16 == 0
+        direct = out_buffer.device == dev and out_buffer.is_contiguous() and out_buffer.data_ptr() % 32 == 0
         od = out_buffer if direct else torch.empty(rows * cols, dtype=torch.bfloat16, device=dev)
         _lib.check(_lib.lib().tcb_dequantize_mxfp4(cd.data_ptr(), sd.data_ptr(), rows, cols, od.data_ptr(), _lib.stream_of(dev)))
         if not direct:
@@ -145,7 +145,7 @@ def mxfp4_matmul(x: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor, bias
     out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
     if M and N:
         with _lib.on_device(dev):
-            x2, cd, sd = _aligned(x2.contiguous()), _aligned(wq.contiguous()), _aligned(w_scales.contiguous())
+            x2, cd, sd = _aligned(x2.contiguous(), 32), _aligned(wq.contiguous()), _aligned(w_scales.contiguous())
             b = None if bias is None else bias.contiguous()
             nbytes = -(-M * (K // 2) // 512) * 512 + mxfp4_scale_bytes(M, K)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)

@@ -27,7 +27,7 @@ def test_library_refuses_bad_arguments_before_any_device_work(built_lib):
     assert L.tcb_cache_write(p, 0, p, 4, p, p, 10, 72, 32, p, None) == _lib.ERR_BAD_ARG
     assert L.tcb_cache_write(p, 0, p, 4, p, p, 10, 64, 32, None, None) == _lib.ERR_BAD_ARG
     assert L.tcb_cache_write(p, 0, None, 4, p, p, 10, 64, 32, p, None) == _lib.ERR_BAD_ARG
-    assert L.tcb_cache_write(p + 4, 0, p, 4, p, p, 10, 64, 32, p, None) == _lib.ERR_ALIGNMENT
+    assert L.tcb_cache_write(p + 16, 0, p, 4, p, p, 10, 64, 32, p, None) == _lib.ERR_ALIGNMENT
     assert L.tcb_cache_write(p, 0, p + 4, 4, p, p, 10, 64, 32, p, None) == _lib.ERR_ALIGNMENT
     assert L.tcb_cache_write(p, 0, p, 1 << 31, p, p, 10, 64, 32, p, None) == _lib.ERR_TOO_LARGE
     assert L.tcb_cache_read(p, p, 10, 64, 32, p, -1, p, None) == _lib.ERR_BAD_ARG
@@ -145,8 +145,9 @@ def test_linear_entry_points_refuse_bad_arguments(built_lib):
     assert bwd(p, 8, p, p, p, None, None, p, None, 4, 8, 48, 32, p, 0) == _lib.ERR_BAD_ARG
     assert bwd(p, 8, p, p, None, None, None, p, None, 4, 8, 32, 32, p, 0) == _lib.ERR_BAD_ARG    # scales missing
     assert bwd(p, 8, None, p, p, None, p, None, None, 4, 8, 32, 32, p, 0) == _lib.ERR_BAD_ARG    # weight missing
-    assert bwd(p, 8, None, None, None, None, None, None, p, 4, 8, 32, 32, p, 4) == _lib.ERR_BAD_ARG  # workspace too small
-    assert L.tcb_linear_workspace(0, 8, 32) == 0 and L.tcb_linear_workspace(4, 8, 32) > 0
+    assert bwd(p, 8, None, None, None, None, None, None, p, 5000, 8, 32, 32, p, 4) == _lib.ERR_BAD_ARG  # workspace too small
+    assert L.tcb_linear_workspace(0, 8, 32, 1) == 0 and L.tcb_linear_workspace(4, 8, 32, 1) == 0
+    assert L.tcb_linear_workspace(100000, 8, 32, 1) > 0 and L.tcb_linear_workspace(4, 8, 4096, 0) > 0
 
 
 def test_linear_layer_refusals():
