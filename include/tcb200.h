@@ -193,10 +193,10 @@ TCB_API int tcb_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, in
  * values of wq [N, K / 2], w_scales (tile order; no padding byte may be 255: it would be a NaN).
  * No counterpart in the reference.
  *   x [M, K] of `dtype`, 32-byte aligned; wq, w_scales 16-byte aligned; bias bf16 [N] or NULL;
- *   out [M, N] bf16; workspace: tcb_mxfp4_linear_workspace(M, K) bytes, 16-byte aligned, used by
- *   the call's own work on `stream` only.  K a positive multiple of 32; M, N arbitrary.
+ *   out [M, N] bf16; workspace: tcb_mxfp4_linear_workspace(M, N, K) bytes (NULL where that
+ *   is 0), 16-byte aligned, used by the call's own work on `stream` only.  K a positive multiple of 32; M, N arbitrary.
  */
-TCB_API int64_t tcb_mxfp4_linear_workspace(int64_t M, int64_t K);
+TCB_API int64_t tcb_mxfp4_linear_workspace(int64_t M, int64_t N, int64_t K);
 TCB_API int tcb_mxfp4_linear(const void* x, int dtype, const uint8_t* wq, const uint8_t* w_scales,
                              const uint16_t* bias_or_null, uint16_t* out, int64_t M, int64_t N, int64_t K,
                              void* workspace, int64_t workspace_bytes, void* stream);

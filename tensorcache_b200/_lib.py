@@ -63,7 +63,7 @@ SIGNATURES = {
     "tcb_decompress_sym": (_i32, [_vp, _vp, _vp, _i64, _i32, _vp]),
     "tcb_quantize_mxfp4": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp]),
     "tcb_dequantize_mxfp4": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp]),
-    "tcb_mxfp4_linear_workspace": (_i64, [_i64, _i64]),
+    "tcb_mxfp4_linear_workspace": (_i64, [_i64, _i64, _i64]),
     "tcb_mxfp4_linear": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
     "tcb_cache_write": (_i32, [_vp, _i32, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp, _vp]),
     "tcb_cache_read": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp]),

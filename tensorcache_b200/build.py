@@ -33,6 +33,7 @@ SOURCES = [
     ("noalloc.cu", []),
     ("linear_train.cu", []),
     ("mxfp4.cu", []),
+    ("mxfp4_few.cu", []),
     ("mxfp4_linear.cu", []),
     ("row_cache.cu", []),
 ]

@@ -73,6 +73,7 @@
 namespace tcb {
 int take_linear_status(int* status);
 int take_mxfp4_status(int* status);
+int take_mxfp4_few_status(int* status);
 }
 
 namespace {
@@ -611,19 +612,15 @@ extern "C" int tcb_selftest_bounded_wait(int budget_ms, void* stream) {
 
 extern "C" int tcb_fused_dequant_linear_check(void* stream) {
     TCB_CUDA_TRY(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
-    int status = 0, linear = 0, mxfp4 = 0;
-    int rc = tcb::take_linear_status(&linear);
-    if (rc == TCB_OK) rc = tcb::take_mxfp4_status(&mxfp4);
+    const char* names[4] = {"tcb_fused_dequant_linear", "tcb_linear_*", "tcb_mxfp4_linear", "tcb_mxfp4_linear (few rows)"};
+    int status[4];
+    int rc = take_status(g_status, &status[0]);
+    if (rc == TCB_OK) rc = tcb::take_linear_status(&status[1]);
+    if (rc == TCB_OK) rc = tcb::take_mxfp4_status(&status[2]);
+    if (rc == TCB_OK) rc = tcb::take_mxfp4_few_status(&status[3]);
     if (rc != TCB_OK) return rc;
-    TCB_CUDA_TRY(cudaMemcpyFromSymbol(&status, g_status, sizeof(int)));
-    if (status != 0) {
-        const int zero = 0;
-        TCB_CUDA_TRY(cudaMemcpyToSymbol(g_status, &zero, sizeof(int)));
-        return tcb::fail(TCB_ERR_TIMEOUT, "tcb_fused_dequant_linear: a bounded wait ran out (role %d, barrier %d)", status >> 8, status & 0xff);
-    }
-    if (linear != 0)
-        return tcb::fail(TCB_ERR_TIMEOUT, "tcb_linear_*: a bounded wait ran out (role %d, barrier %d)", linear >> 8, linear & 0xff);
-    if (mxfp4 != 0)
-        return tcb::fail(TCB_ERR_TIMEOUT, "tcb_mxfp4_linear: a bounded wait ran out (role %d, barrier %d)", mxfp4 >> 8, mxfp4 & 0xff);
+    for (int i = 0; i < 4; ++i)
+        if (status[i] != 0)
+            return tcb::fail(TCB_ERR_TIMEOUT, "%s: a bounded wait ran out (role %d, barrier %d)", names[i], status[i] >> 8, status[i] & 0xff);
     return TCB_OK;
 }

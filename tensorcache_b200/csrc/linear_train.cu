@@ -611,16 +611,7 @@ int check_group(const char* who, int64_t K, int group_size) {
 }  // namespace
 
 namespace tcb {
-// Reads and clears this file's status word (the stream has been synchronised).
-int take_linear_status(int* status) {
-    *status = 0;
-    TCB_CUDA_TRY(cudaMemcpyFromSymbol(status, g_status, sizeof(int)));
-    if (*status) {
-        const int zero = 0;
-        TCB_CUDA_TRY(cudaMemcpyToSymbol(g_status, &zero, sizeof(int)));
-    }
-    return TCB_OK;
-}
+int take_linear_status(int* status) { return take_status(g_status, status); }
 }  // namespace tcb
 
 extern "C" int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K, int backward) {

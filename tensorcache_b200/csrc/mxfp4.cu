@@ -16,128 +16,12 @@
 // rows x 128 columns): thread (row = t / 4, block = t % 4) takes rows row, row + 32, row + 64 and row + 96, so a warp
 // reads 8 rows x 256 contiguous bytes with 8 loads of 32 bytes a thread in flight, and the 512 scale bytes of the tile
 // leave as contiguous 16-byte pieces after a 4 x 4 byte transpose over four lanes.
-#include <type_traits>
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include "tcb_common.h"
+#include "tcb_mxfp4.h"
 
 namespace {
 
 constexpr int kThreads = 128;
 constexpr int kTileRows = 128, kTileCols = 128;
-
-// Streamed once: 32-byte accesses that leave L2 first.
-__device__ __forceinline__ void ldg_stream_v8(const void* p, uint32_t* w) {
-    asm volatile("ld.global.nc.L1::no_allocate.L2::evict_first.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                 : "l"(p));
-}
-__device__ __forceinline__ void stg_stream_v8(void* p, const uint32_t* w) {
-    asm volatile("st.global.L2::evict_first.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-}
-
-// One block of 32 values.
-template <typename T>
-struct Block32 {
-    static constexpr int kWords = 32 * sizeof(T) / 4;
-    uint32_t w[kWords];
-
-    __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-        for (int i = 0; i < kWords; i += 8) ldg_stream_v8(reinterpret_cast<const uint32_t*>(p) + i, w + i);
-    }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = 0;
-    }
-    __device__ __forceinline__ uint32_t word(int i) const { return w[i]; }
-    __device__ __forceinline__ float get(int i) const;
-};
-template <>
-__device__ __forceinline__ float Block32<__nv_bfloat16>::get(int i) const {
-    const uint32_t v = word(i >> 1);
-    return __uint_as_float((i & 1) ? (v & 0xffff0000u) : (v << 16));
-}
-template <>
-__device__ __forceinline__ float Block32<__half>::get(int i) const {
-    const uint32_t v = word(i >> 1);
-    return __half2float(__ushort_as_half((i & 1) ? (v >> 16) : (v & 0xffffu)));
-}
-template <>
-__device__ __forceinline__ float Block32<float>::get(int i) const { return __uint_as_float(word(i)); }
-
-// Exponent field (fp32) of the largest magnitude, 255 if a value is not finite.  16-bit types compare two magnitudes
-// at once as integers (the order of the bit patterns is the order of the values).
-template <typename T>
-__device__ __forceinline__ uint32_t max_exponent(const Block32<T>& b) {
-    uint32_t m = 0;
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) m = __vmaxu2(m, b.word(i) & 0x7fff7fffu);
-        m = max(m & 0xffffu, m >> 16);
-        if constexpr (std::is_same<T, __half>::value) {
-            if (m >= 0x7c00u) return 255u;
-            return __float_as_uint(__half2float(__ushort_as_half(uint16_t(m)))) >> 23;
-        } else {
-            return m >> 7;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) m = max(m, b.word(i) & 0x7fffffffu);
-        return m >> 23;
-    }
-}
-
-__device__ __forceinline__ uint32_t float8_to_e2m1x8(const float (&v)[8]) {
-    uint32_t r;
-    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
-        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
-        : "=r"(r)
-        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
-    return r;
-}
-
-// Scale byte and 32 codes of one block.
-template <typename T>
-__device__ __forceinline__ uint32_t encode_block(const Block32<T>& b, uint4& codes) {
-    uint32_t e = max_exponent(b);
-    const bool clean = e != 255u;
-    if (!clean) {   // rare: leave out what is not finite
-        e = 0;
-#pragma unroll 1
-        for (int i = 0; i < 32; ++i) {
-            float f = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) f = j == i ? b.get(j) : f;
-            const uint32_t x = (__float_as_uint(f) >> 23) & 255u;
-            if (x != 255u) e = max(e, x);
-        }
-    }
-    const uint32_t byte = e > 2u ? e - 2u : 0u;
-    const float inv = __uint_as_float((254u - byte) << 23);   // 2^(127 - byte), exact product
-    uint32_t o[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = b.get(8 * k + i);
-            v[i] = __fmul_rn(x, inv);
-            if (!clean && (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) v[i] = 0.0f;
-        }
-        o[k] = float8_to_e2m1x8(v);
-    }
-    codes = make_uint4(o[0], o[1], o[2], o[3]);
-    return byte;
-}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)

@@ -19,6 +19,12 @@
 // Waits are bounded as in the fused dequantising product; the status word is read by tcb_fused_dequant_linear_check().
 #include "tcb_tcgen05.h"
 
+namespace tcb {
+bool mxfp4_few_rows(int64_t M, int64_t N, int64_t K);
+int launch_mxfp4_few_rows(const char* who, const void* x, int dtype, const CUtensorMap& map_w, const CUtensorMap& map_ws, const uint16_t* bias,
+                          uint16_t* out, int64_t M, int64_t N, int64_t K, cudaStream_t st);
+}  // namespace tcb
+
 namespace {
 
 constexpr int kTileRows = 128, kPairRows = 256;
@@ -269,20 +275,12 @@ int encode_maps(const char* who, CUtensorMap* codes_map, CUtensorMap* scales_map
 }  // namespace
 
 namespace tcb {
-// Reads and clears this file's status word (the stream has been synchronised).
-int take_mxfp4_status(int* status) {
-    *status = 0;
-    TCB_CUDA_TRY(cudaMemcpyFromSymbol(status, g_status, sizeof(int)));
-    if (*status) {
-        const int zero = 0;
-        TCB_CUDA_TRY(cudaMemcpyToSymbol(g_status, &zero, sizeof(int)));
-    }
-    return TCB_OK;
-}
+int take_mxfp4_status(int* status) { return take_status(g_status, status); }
 }  // namespace tcb
 
-extern "C" int64_t tcb_mxfp4_linear_workspace(int64_t M, int64_t K) {
-    return M <= 0 || K <= 0 ? 0 : code_bytes(M, K) + scale_bytes(M, K);
+extern "C" int64_t tcb_mxfp4_linear_workspace(int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || tcb::mxfp4_few_rows(M, N, K)) return 0;
+    return code_bytes(M, K) + scale_bytes(M, K);
 }
 
 extern "C" int tcb_mxfp4_linear(const void* x, int dtype, const uint8_t* wq, const uint8_t* w_scales, const uint16_t* bias_or_null, uint16_t* out,
@@ -301,14 +299,18 @@ extern "C" int tcb_mxfp4_linear(const void* x, int dtype, const uint8_t* wq, con
         return tcb::fail(TCB_ERR_ALIGNMENT, "%s: x must be 32-byte and codes and scales 16-byte aligned", who);
     if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias_or_null)) & 1)
         return tcb::fail(TCB_ERR_ALIGNMENT, "%s: bias and out must be 2-byte aligned", who);
-    if (!workspace || workspace_bytes < tcb_mxfp4_linear_workspace(M, K) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    const int64_t need = tcb_mxfp4_linear_workspace(M, N, K);
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
         return tcb::fail(TCB_ERR_BAD_ARG, "%s: the workspace is too small or not 16-byte aligned", who);
+    CUtensorMap map_x, map_w, map_xs, map_ws;
+    if (need == 0) {   // few rows: w in boxes of 128 rows, x quantised by the product itself
+        const int few = encode_maps(who, &map_w, &map_ws, wq, w_scales, N, K, 1);
+        return few != TCB_OK ? few : tcb::launch_mxfp4_few_rows(who, x, dtype, map_w, map_ws, bias_or_null, out, M, N, K, static_cast<cudaStream_t>(stream));
+    }
     uint8_t* xq = static_cast<uint8_t*>(workspace);
     uint8_t* xs = xq + code_bytes(M, K);
     int rc = tcb_quantize_mxfp4(x, dtype, M, K, xq, xs, stream);
-    if (rc != TCB_OK) return rc;
-    CUtensorMap map_x, map_w, map_xs, map_ws;
-    rc = encode_maps(who, &map_x, &map_xs, xq, xs, M, K, 1);
+    if (rc == TCB_OK) rc = encode_maps(who, &map_x, &map_xs, xq, xs, M, K, 1);
     if (rc == TCB_OK) rc = encode_maps(who, &map_w, &map_ws, wq, w_scales, N, K, 2);
     if (rc != TCB_OK) return rc;
     static std::atomic<bool> attr_set[64] = {};

@@ -257,6 +257,17 @@ __device__ __forceinline__ void store_32x32(uint16_t* out, int64_t ld, int64_t r
 
 // ---------------------------------------------------------------------- host
 
+// Reads and clears a file's status word (the stream has been synchronised).
+inline int take_status(const int& symbol, int* status) {
+    *status = 0;
+    TCB_CUDA_TRY(cudaMemcpyFromSymbol(status, symbol, sizeof(int)));
+    if (*status) {
+        const int zero = 0;
+        TCB_CUDA_TRY(cudaMemcpyToSymbol(symbol, &zero, sizeof(int)));
+    }
+    return TCB_OK;
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

@@ -9,6 +9,7 @@ errors follow ``codec.py``.
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -116,6 +117,12 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, orig_shape: Tupl
     return out_buffer
 
 
+@lru_cache(maxsize=1024)
+def _workspace_bytes(M: int, N: int, K: int, device_index: int) -> int:
+    """Scratch bytes of a product of these sizes (which kernel runs depends on the device's number of SMs)."""
+    return _lib.lib().tcb_mxfp4_linear_workspace(M, N, K)
+
+
 def mxfp4_matmul(x: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``mxfp4(x) @ dequant(W).T (+ bias)`` on the 4-bit tensor cores, with W stored as MXFP4 (``wq`` uint8 ``[N, K / 2]``,
     ``w_scales`` in tile order, both as ``quantize_mxfp4`` returns them for ``[N, K]``).
@@ -147,8 +154,8 @@ def mxfp4_matmul(x: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor, bias
         with _lib.on_device(dev):
             x2, cd, sd = _aligned(x2.contiguous(), 32), _aligned(wq.contiguous()), _aligned(w_scales.contiguous())
             b = None if bias is None else bias.contiguous()
-            nbytes = -(-M * (K // 2) // 512) * 512 + mxfp4_scale_bytes(M, K)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            nbytes = _workspace_bytes(M, N, K, dev.index)     # x in MXFP4; 0 for few rows
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
             _lib.check(_lib.lib().tcb_mxfp4_linear(x2.data_ptr(), _DTYPES[x2.dtype], cd.data_ptr(), sd.data_ptr(), _lib.address(b), out.data_ptr(),
-                                                   M, N, K, ws.data_ptr(), nbytes, _lib.stream_of(dev)))
+                                                   M, N, K, _lib.address(ws), nbytes, _lib.stream_of(dev)))
     return out.view(*x.shape[:-1], N)

@@ -170,6 +170,28 @@ def test_product(M, N, K, dtype):
     product_close(tc.mxfp4_matmul(x, wq, ws, bias=b), X, W, b)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 14336, 4096), (5, 4096, 14336), (16, 128, 2080), (31, 4100, 1184), (32, 700, 4096), (1, 300, 70016), (20, 130, 33024),
+                                   (32, 100, 262144), (33, 100, 4096), (1, 40000, 96)])
+def test_product_of_few_rows(M, N, K):
+    """One part and several, parts of unequal length, sums too long for the kernel of few rows, and the sizes beside its limit."""
+    x, w, b = product_inputs(M, N, K, seed=M + K)
+    wq, ws, _ = tc.quantize_mxfp4(w)
+    y = tc.mxfp4_matmul(x, wq, ws, bias=b)
+    check_device_status()
+    product_close(y, plain.mx_values(*plain.mx_encode(x)), plain.mx_values(*plain.mx_encode(w)), b)
+
+
+def test_scales_that_pad_a_row_do_not_reach_the_sums():
+    """K = 32 in a tile of 128: the other three scales of a row are padding."""
+    for M in (3, 40):
+        x, w, _ = product_inputs(M, 50, 32, seed=M)
+        wq, ws, _ = tc.quantize_mxfp4(w)
+        rows = torch.full((128, 4), 254, dtype=torch.uint8, device=DEV)      # the largest finite scale wherever nothing is stored
+        rows[:50, :1] = tc.mxfp4_scales_to_rows(ws, 50, 32)
+        loud = tc.mxfp4_scales_from_rows(rows)
+        assert torch.equal(tc.mxfp4_matmul(x, wq, loud), tc.mxfp4_matmul(x, wq, ws))
+
+
 def test_product_of_the_identity_returns_the_weight():
     """One non-zero code per row of x, with its own scale: every weight and every scale comes back where it belongs."""
     K, N = 1024, 700

@@ -40,8 +40,8 @@ def test_mxfp4_product_refusals(built_lib):
     from tensorcache_b200 import _lib
 
     L, p = built_lib, 1 << 20
-    need = L.tcb_mxfp4_linear_workspace(4, 64)
-    assert need == 512 + 512 and L.tcb_mxfp4_linear_workspace(0, 64) == 0
+    need = L.tcb_mxfp4_linear_workspace(40, 8, 64)
+    assert need == 40 * 32 + 256 + 512 and L.tcb_mxfp4_linear_workspace(0, 8, 64) == 0 and L.tcb_mxfp4_linear_workspace(4, 8, 64) == 0
     f = lambda *a: L.tcb_mxfp4_linear(*a, None)  # noqa: E731
     assert f(None, 0, None, None, None, None, 0, 8, 64, None, 0) == _lib.TCB_OK
     assert f(p, 3, p, p, None, p, 4, 8, 64, p, need) == _lib.ERR_BAD_ARG            # dtype
@@ -50,7 +50,7 @@ def test_mxfp4_product_refusals(built_lib):
     assert f(p, 0, None, p, None, p, 4, 8, 64, p, need) == _lib.ERR_BAD_ARG
     assert f(p + 8, 0, p, p, None, p, 4, 8, 64, p, need) == _lib.ERR_ALIGNMENT
     assert f(p, 0, p, p, None, p + 1, 4, 8, 64, p, need) == _lib.ERR_ALIGNMENT
-    assert f(p, 0, p, p, None, p, 4, 8, 64, p, need - 1) == _lib.ERR_BAD_ARG        # workspace
+    assert f(p, 0, p, p, None, p, 40, 8, 64, p, need - 1) == _lib.ERR_BAD_ARG       # workspace
     assert f(p, 0, p, p, None, p, 1 << 31, 8, 64, p, need) == _lib.ERR_TOO_LARGE
     x, wq, ws = torch.zeros(4, 64), torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8)
     for bad, match in (((x[:, :32], wq, ws), "inner dimensions"), ((x, wq.view(-1), ws), "wq"), ((x, wq, ws[:-1]), "scales"),
