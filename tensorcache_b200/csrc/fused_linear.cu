@@ -132,7 +132,7 @@ struct Params {
     uint16_t* out;            // [rows of the A operand, rows of the B operand]
     int64_t R_q, R_d, K;
     int64_t gpr;              // groups per row = K / G
-    int table_vec_ok;         // scales / zero points of a table can be fetched with 16-byte loads
+    int table_vec_ok;         // scales / zero points of a table can be fetched eight groups at a time
     int quant_is_a;           // the dequantised operand is the M side (output rows); otherwise the dense one is
     // Tile list of a launch.  Dense rows are counted in units of 256.  Tiles [0, n_wide) are wide (256 x 512: dense units
     // 2j, 2j + 1); the next 2 n_conv tiles are the halves (256 x 256) of the wide tiles that would have made up a last,
@@ -159,11 +159,21 @@ __device__ __forceinline__ void table_fetch(const Params& p, int64_t grow, int64
     c.s0 = c.s1 = c.z = make_uint4(0, 0, 0, 0);
     if (!row_ok || g_first >= p.gpr) return;
     const int64_t base = grow * p.gpr + g_first;
-    if (p.table_vec_ok && g_first + 16 <= p.gpr) {
+    if (p.table_vec_ok) {   // eight groups at a time: rows of 24 groups (K = 768 at G = 32) start on 16-byte boundaries too
         const uint4* sp = reinterpret_cast<const uint4*>(p.scales + base);
+        const uint2* zp = reinterpret_cast<const uint2*>(p.zp + base);
         c.s0 = __ldg(sp);
-        c.s1 = __ldg(sp + 1);
-        if (p.zp) c.z = __ldg(reinterpret_cast<const uint4*>(p.zp + base));
+        if (p.zp) {
+            const uint2 z = __ldg(zp);
+            c.z.x = z.x, c.z.y = z.y;
+        }
+        if (g_first + 16 <= p.gpr) {
+            c.s1 = __ldg(sp + 1);
+            if (p.zp) {
+                const uint2 z = __ldg(zp + 1);
+                c.z.z = z.x, c.z.w = z.y;
+            }
+        }
         return;
     }
     uint32_t sw[8] = {0, 0, 0, 0, 0, 0, 0, 0}, zw[4] = {0, 0, 0, 0};
@@ -577,8 +587,8 @@ extern "C" int tcb_fused_dequant_linear(const uint16_t* dense, const uint8_t* q,
     p.R_d = R_d;
     p.K = K;
     p.gpr = K / group_size;
-    p.table_vec_ok = p.gpr % 16 == 0 && (reinterpret_cast<uintptr_t>(scales) & 15) == 0 &&
-                     (zp_or_null == nullptr || (reinterpret_cast<uintptr_t>(zp_or_null) & 15) == 0);
+    p.table_vec_ok = p.gpr % 8 == 0 && (reinterpret_cast<uintptr_t>(scales) & 15) == 0 &&
+                     (zp_or_null == nullptr || (reinterpret_cast<uintptr_t>(zp_or_null) & 7) == 0);
     p.quant_is_a = quant_is_rhs ? 0 : 1;
     // The tile list: wide (256 x 512) tiles as far as they fill whole rounds of the CTA pairs; if what is left of them
     // would occupy at most half of the pairs for a last round, those become twice as many 256 x 256 tiles, which run
