@@ -316,52 +316,52 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         const int pw = warp - C::kFirstProducerWarp, r = pw * 8 + (lane >> 2), kq = lane & 3, h0 = r & 1;
         const uint32_t piece0 = uint32_t(((2 * kq) ^ (r & 7)) * 16), piece1 = piece0 ^ 16u;
         const int64_t gpr = p.rows_b >> LOG2_G, stage_groups = gpr * kBlockK;
-        // scale and zero point of the lane's two pieces, fetched two stages ahead; g: group of column 0 of the lane's row
+        // Scale and zero point of the lane's two pieces are fetched a whole ring ahead, into registers named by the stage: the
+        // loop is unrolled over the ring, because moving (or even shifting) a value that is still on its way would wait for it
+        // -- that cost a tenth of the kernel's time.
         int pf_item = first, pf_kb = 0, pf_end = 0;
-        int64_t g = 0;
-        int off[2] = {0, 0};          // the pieces' groups in the row; -1: outside
+        int64_t g[2] = {0, 0};        // group of the piece in the row being fetched; negative: outside
         auto start = [&]() {
             const Item t = decode_item<C::kGroups>(p, pf_item);
             pf_kb = t.kb0;
             pf_end = t.kb1;
-            g = (int64_t(pf_kb) * kBlockK + r) * gpr;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int64_t k = int64_t(t.tb) * kPairRows + int64_t(rank) * kTileRows + 16 * kq + 64 * (h0 ^ i);
-                off[i] = k < p.rows_b ? int(k >> LOG2_G) : -1;
+                g[i] = k < p.rows_b ? (int64_t(pf_kb) * kBlockK + r) * gpr + (k >> LOG2_G) : INT64_MIN;
             }
         };
         start();
-        auto fetch = [&](uint32_t (&sz)[2]) {
-            sz[0] = sz[1] = 0;
-            if (pf_item >= p.items) return;
-            if (pf_kb * kBlockK + r < p.contraction) {
+        uint32_t scale[S][2], zero[S][2];
+        auto fetch = [&](int slot) {
+            const bool inside = pf_item < p.items && pf_kb * kBlockK + r < int(p.contraction);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (off[i] >= 0) {
-                        sz[i] = uint32_t(__ldg(p.scales + g + off[i])) << 16;
-                        if (HAS_ZP) sz[i] |= __ldg(p.zp + g + off[i]);
-                    }
+            for (int i = 0; i < 2; ++i) {
+                const bool ok = inside && g[i] >= 0;
+                scale[slot][i] = ok ? __ldg(p.scales + g[i]) : uint16_t(0);
+                zero[slot][i] = HAS_ZP && ok ? __ldg(p.zp + g[i]) : uint8_t(0);
+                g[i] += stage_groups;
             }
-            g += stage_groups;
             if (++pf_kb == pf_end) {
                 pf_item += step;
                 if (pf_item < p.items) start();
             }
         };
-        uint32_t ahead0[2], ahead1[2];
-        fetch(ahead0);
-        fetch(ahead1);
-        int s = 0;
+        int total = 0;                // stages of all of this pair's items
+        for (int item = first; item < p.items; item += step) {
+            const Item t = decode_item<C::kGroups>(p, item);
+            total += t.kb1 - t.kb0;
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) fetch(s);
         uint32_t ph = 0;
         bool ok = true;
-        for (int item = first; ok && item < p.items; item += step) {
-            const Item t = decode_item<C::kGroups>(p, item);
-            for (int kb = t.kb0; kb < t.kb1; ++kb) {
-                const uint32_t sz0 = ahead0[0], sz1 = ahead0[1];
-                ahead0[0] = ahead1[0];
-                ahead0[1] = ahead1[1];
-                fetch(ahead1);
+        for (int i0 = 0; ok && i0 < total; i0 += S, ph ^= 1) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                if (i0 + s >= total) break;
+                const uint32_t sz0 = (scale[s][0] << 16) | zero[s][0], sz1 = (scale[s][1] << 16) | zero[s][1];
+                fetch(s);
                 // warp-uniform verdict: the warp-level sync below needs every lane
                 ok = __all_sync(0xffffffffu, mbar_wait(bar(FULL_C + s), ph, abort_flag, abort_peer, (3 << 8) | (FULL_C + s)));
                 if (!ok) break;
@@ -374,7 +374,6 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 fence_proxy_async();   // the stores above become visible to the tensor cores
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(leader_bar(FULL + s));
-                if (++s == S) { s = 0; ph ^= 1; }
             }
         }
     }
