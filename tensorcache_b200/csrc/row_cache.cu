@@ -13,6 +13,8 @@
 // Both kernels are bound by HBM.  A thread takes V values of one group (write: G = 8: 8; 16, 32, 64, 128: 16; 24, 48: 24;
 // read: 32 for G = 32, 64, 128), so that most accesses are 32 bytes; 1 to 8 neighbouring lanes make up a group and combine
 // max|x| by shuffles.  Two units a thread are in flight: each starts with a chain of dependent loads (index, claim, data).
+#include <type_traits>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -92,18 +94,47 @@ __device__ __forceinline__ float value_of<float>(const uint32_t* w, int i) { ret
 
 __device__ __forceinline__ bool finite_f32(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 
+// max|x| over a unit, NaN or infinity if a value is not finite: the order of the bit patterns without sign is the order of
+// the magnitudes, and everything that is not finite lies above.  16-bit types compare two at once.
+template <typename T, int WORDS>
+__device__ __forceinline__ float max_magnitude(const uint32_t (&w)[WORDS]) {
+    uint32_t m = 0;
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) m = max(m, w[i] & 0x7fffffffu);
+        return __uint_as_float(m);
+    } else {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+        const uint32_t one[1] = {max(m & 0xffffu, m >> 16)};
+        return value_of<T>(one, 0);
+    }
+}
+// Values that are not finite become 0.
+template <typename T, int WORDS>
+__device__ __forceinline__ void clear_nonfinite(uint32_t (&w)[WORDS]) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+        if constexpr (std::is_same<T, float>::value) {
+            if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] = 0;
+        } else {
+            constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+            if ((w[i] & kExp) == kExp) w[i] &= 0xffff0000u;
+            if ((w[i] & (kExp << 16)) == (kExp << 16)) w[i] &= 0x0000ffffu;
+        }
+    }
+}
+
 // The V values of a unit -> codes at q and, from the group's first lane, the scale.  Every lane of the warp calls this;
 // `live` lanes store.
 template <int G, typename T>
-__device__ __forceinline__ void encode_unit(const uint32_t* raw, bool live, int8_t* __restrict__ q, uint16_t* __restrict__ scale) {
+__device__ __forceinline__ void encode_unit(uint32_t (&raw)[Split<G>::V * sizeof(T) / 4], bool live, int8_t* __restrict__ q,
+                                            uint16_t* __restrict__ scale) {
     constexpr int V = Split<G>::V, LPG = Split<G>::LPG;
-    float v[V];
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        v[i] = value_of<T>(raw, i);
-        v[i] = finite_f32(v[i]) ? v[i] : 0.0f;
-        amax = fmaxf(amax, fabsf(v[i]));
+    float amax = max_magnitude<T>(raw);
+    if (__builtin_expect(!finite_f32(amax), 0)) {
+        clear_nonfinite<T>(raw);
+        amax = max_magnitude<T>(raw);
     }
 #pragma unroll
     for (int off = 1; off < LPG; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
@@ -118,7 +149,7 @@ __device__ __forceinline__ void encode_unit(const uint32_t* raw, bool live, int8
             // The IEEE quotient: the residual of rn(x * rn(1 / s)) is exact in one FMA because s has 8 significant
             // bits, and one more corrects the quotient (Markstein).  |x / s| < 127.3, so the clamp to [-128, 127]
             // never binds; adding 1.5 * 2^23 rounds to nearest even.
-            const float x1 = v[4 * i + j], t = __fmul_rn(x1, r);
+            const float x1 = value_of<T>(raw, 4 * i + j), t = __fmul_rn(x1, r);
             c[j] = __float_as_uint(__fadd_rn(__fmaf_rn(__fmaf_rn(-t, s, x1), r, t), 12582912.0f));
         }
         w[i] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
