@@ -71,6 +71,9 @@ struct Params {
     uint16_t* out;              // [rows_a, rows_b]
     float* partial;             // split: [splits][rows_a][ld_partial]
     int64_t ld_partial;
+    const uint16_t* columns;    // weight gradient: null, or dy, whose column sums the epilogue warps leave ...
+    int64_t ld_columns;
+    float* column_parts;        // ... here, [warps of all CTAs by their row slice][rows_a]
     const uint16_t* scales;     // codes: [contraction, rows_b / G]
     const uint8_t* zp;
     int64_t contraction;
@@ -135,6 +138,43 @@ __device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* ma
     } else {
         tma_load_2d_pair(dst, map, row, c, bar);
         tma_load_2d_pair(dst + kBoxBytes, map, row + 64, c, bar);
+    }
+}
+
+// How the column sums of [rows, cols] are shared out: a warp takes blocks of 64 columns; with fewer than eight blocks the
+// eight warps of a CTA take slices of the rows as well.
+struct ColumnShare {
+    int blocks, slices;   // column blocks; row slices per CTA
+    __host__ __device__ explicit ColumnShare(int64_t cols) : blocks(int((cols + 63) / 64)), slices(blocks >= 8 ? 1 : 8 / blocks) {}
+};
+
+// Column sums of one warp: 64 columns (8 lanes of 16 bytes a row), every parts-th run of 16 rows, fp32.
+__device__ __forceinline__ void sum_columns(const uint16_t* __restrict__ x, int64_t rows, int64_t cols, int64_t ld, int block, int part, int parts,
+                                            float* __restrict__ out) {
+    const int lane = threadIdx.x & 31;
+    const int64_t col = int64_t(block) * 64 + (lane & 7) * 8;
+    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (col < cols)   // ld is a multiple of 8: a whole 16-byte piece is there
+        for (int64_t row = int64_t(part) * 16 + (lane >> 3); row < rows; row += int64_t(parts) * 16) {
+            uint4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[j] = row + 4 * j < rows ? __ldg(reinterpret_cast<const uint4*>(x + (row + 4 * j) * ld + col)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[2 * i] += __uint_as_float(w[i] << 16);
+                    s[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+                }
+            }
+        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        s[i] += __shfl_xor_sync(0xffffffffu, s[i], 8);
+        s[i] += __shfl_xor_sync(0xffffffffu, s[i], 16);
+        if (lane < 8 && col + i < cols) out[int64_t(part) * cols + col + i] = s[i];
     }
 }
 
@@ -271,6 +311,17 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         const int group = (warp - kFirstEpilogueWarp) >> 2;   // the accumulator of the tile
         const StoreMode mode = store_mode(p.out, p.rows_b, p.bias);
         uint32_t* stage = reinterpret_cast<uint32_t*>(smem_e + (C::kStore ? (warp - kFirstEpilogueWarp) * kStoreStageBytes : 0));
+        if constexpr (C::kDeq) {
+            // bias gradient: these warps have nothing to do until the first tile is complete, and memory has time to spare
+            if (p.columns) {
+                const ColumnShare share(p.rows_a);
+                const int w = warp - kFirstEpilogueWarp;
+                if (w / share.blocks < share.slices)
+                    for (int block = w % share.blocks; block < share.blocks; block += 8)
+                        sum_columns(p.columns, p.contraction, p.rows_a, p.ld_columns, block, int(blockIdx.x) * share.slices + w / share.blocks,
+                                    int(gridDim.x) * share.slices, p.column_parts);
+            }
+        }
         int local = 0;
         bool ok = true;
         for (int item = first; ok && item < p.items; item += step, ++local) {
@@ -387,89 +438,72 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     }
 }
 
-// out[a, b] = bf16(sum over the splits, in order, + bias[b]); four columns per thread.
-__global__ void __launch_bounds__(256) add_parts_kernel(const float* __restrict__ partial, int splits, int64_t rows, int64_t cols, int64_t ld,
-                                                        const uint16_t* __restrict__ bias, uint16_t* __restrict__ out) {
-    const int64_t quads = ld / 4, total = rows * quads;
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+// Sums what the kernels above left in parts, in a fixed order.  Blocks [0, column_blocks): 32 column sums each, eight warps take
+// every eighth part.  The others: out[a, b] = bf16(sum over the splits + bias[b]), four columns per thread.
+struct Parts {
+    const float* partial;       // [splits][rows][ld]
+    int splits;
+    int64_t rows, cols, ld;
+    const uint16_t* bias;
+    uint16_t* out;
+    const float* columns;       // [column_parts][num_columns]
+    int column_parts, column_blocks;
+    int64_t num_columns;
+    uint16_t* column_out;
+};
+__global__ void __launch_bounds__(256) add_parts_kernel(const Parts p) {
+    if (int(blockIdx.x) < p.column_blocks) {
+        __shared__ float acc[8][32];
+        const int r = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        const int64_t col = int64_t(blockIdx.x) * 32 + lane;
+        float sum = 0.0f;
+        if (col < p.num_columns) {
+#pragma unroll 4
+            for (int i = r; i < p.column_parts; i += 8) sum += p.columns[int64_t(i) * p.num_columns + col];
+        }
+        acc[r][lane] = sum;
+        __syncthreads();
+        if (r == 0 && col < p.num_columns) {
+#pragma unroll
+            for (int i = 1; i < 8; ++i) sum += acc[i][lane];
+            p.column_out[col] = f32_to_bf16_bits(sum);
+        }
+        return;
+    }
+    const int64_t quads = p.ld / 4, total = p.rows * quads, step = int64_t(gridDim.x - p.column_blocks) * 256;
+    for (int64_t i = int64_t(blockIdx.x - p.column_blocks) * 256 + threadIdx.x; i < total; i += step) {
         const int64_t row = i / quads, col = (i - row * quads) * 4;
-        if (col >= cols) continue;
-        float4 sum = __ldcs(reinterpret_cast<const float4*>(partial + row * ld + col));
-        for (int s = 1; s < splits; ++s) {
-            const float4 v = __ldcs(reinterpret_cast<const float4*>(partial + (int64_t(s) * rows + row) * ld + col));
+        if (col >= p.cols) continue;
+        float4 sum = __ldcs(reinterpret_cast<const float4*>(p.partial + row * p.ld + col));
+#pragma unroll 4
+        for (int s = 1; s < p.splits; ++s) {
+            const float4 v = __ldcs(reinterpret_cast<const float4*>(p.partial + (int64_t(s) * p.rows + row) * p.ld + col));
             sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
         }
         const float f[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (col + j < cols) {
-                const float b = bias ? __uint_as_float(uint32_t(bias[col + j]) << 16) : 0.0f;
-                out[row * cols + col + j] = f32_to_bf16_bits(f[j] + b);
+            if (col + j < p.cols) {
+                const float b = p.bias ? __uint_as_float(uint32_t(p.bias[col + j]) << 16) : 0.0f;
+                p.out[row * p.cols + col + j] = f32_to_bf16_bits(f[j] + b);
             }
     }
 }
 
-// Column sums of dy, bound by reading it once: block (x, y) takes 64 columns (8 lanes of 16 bytes a row) of every
-// gridDim.y-th run of 128 rows, four rows a thread ahead.  One part: the sums are the result; else they are left as fp32.
-__global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __restrict__ dy, int64_t rows, int64_t cols, int64_t ld,
-                                                          float* __restrict__ partial, uint16_t* __restrict__ out) {
-    __shared__ float acc[32][65];
-    const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8;
-    const int64_t col = int64_t(blockIdx.x) * 64 + c;
-    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (col < cols)   // ld is a multiple of 8: a whole 16-byte piece is there
-        for (int64_t row = int64_t(blockIdx.y) * 128 + r; row < rows; row += int64_t(gridDim.y) * 128) {
-            uint4 v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                v[j] = row + 32 * j < rows ? __ldg(reinterpret_cast<const uint4*>(dy + (row + 32 * j) * ld + col)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[2 * i] += __uint_as_float(w[i] << 16);
-                    s[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
-                }
-            }
-        }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[r][c + i] = s[i];
-    __syncthreads();
-    const int64_t out_col = int64_t(blockIdx.x) * 64 + threadIdx.x;
-    if (threadIdx.x >= 64 || out_col >= cols) return;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) sum += acc[i][threadIdx.x];
-    if (gridDim.y == 1) out[out_col] = f32_to_bf16_bits(sum);
-    else partial[int64_t(blockIdx.y) * cols + out_col] = sum;
-}
-
-// A block adds the parts of 32 columns: eight warps take every eighth part, in a fixed order.
-__global__ void __launch_bounds__(256) add_column_sums_kernel(const float* __restrict__ partial, int parts, int64_t cols, uint16_t* __restrict__ out) {
-    __shared__ float acc[8][32];
-    const int r = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t col = int64_t(blockIdx.x) * 32 + lane;
-    float sum = 0.0f;
-    if (col < cols) {
-#pragma unroll 4
-        for (int i = r; i < parts; i += 8) sum += partial[int64_t(i) * cols + col];
-    }
-    acc[r][lane] = sum;
-    __syncthreads();
-    if (r == 0 && col < cols) {
-#pragma unroll
-        for (int i = 1; i < 8; ++i) sum += acc[i][lane];
-        out[col] = f32_to_bf16_bits(sum);
-    }
+// Column sums where no weight gradient is wanted: a warp per block of columns and part.
+__global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __restrict__ dy, int64_t rows, int64_t cols, int64_t ld, int parts,
+                                                          float* __restrict__ out) {
+    const ColumnShare share(cols);
+    const int64_t unit = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (unit < int64_t(share.blocks) * parts) sum_columns(dy, rows, cols, ld, int(unit % share.blocks), int(unit / share.blocks), parts, out);
 }
 
 // ------------------------------------------------------------------------ host
 
 struct Plan {
-    int64_t tiles_a, tiles_b, num_kb;
-    int splits, kb_per_split;
-    int64_t ld_partial;
+    int64_t tiles_a = 0, tiles_b = 0, num_kb = 0;
+    int splits = 1, kb_per_split = 0;
+    int64_t ld_partial = 0;
     int64_t partial_bytes(int64_t rows_a) const { return splits > 1 ? int64_t(splits) * rows_a * ld_partial * 4 : 0; }
 };
 
@@ -493,17 +527,39 @@ int64_t weight_partial_bytes(int64_t M, int64_t N, int64_t K) {
     return (make_plan(N, K, M, Config<kCodes>::kTileA).partial_bytes(N) + 31) / 32 * 32;
 }
 
-// Parts of the column sums: enough blocks for several per SM, 2048 rows or fewer in one launch of one part.
-int column_parts(int64_t rows, int64_t cols) {
-    if (rows <= 2048) return 1;
-    const int64_t across = (cols + 63) / 64, most = (rows + 511) / 512;
-    int64_t parts = (6 * int64_t(tcb::sm_count()) + across - 1) / across;
-    if (parts > most) parts = most;
-    return int(parts < 1 ? 1 : parts);
-}
-int64_t column_bytes(int64_t rows, int64_t cols) {
-    const int64_t parts = column_parts(rows, cols);
-    return parts > 1 ? parts * cols * 4 : 0;
+// Parts of the column sums: at most one per CTA (a GPU has no more than one CTA per SM of these kernels) and row slice.
+int64_t column_bytes(int64_t cols) { return int64_t(tcb::sm_count()) * ColumnShare(cols).slices * cols * 4; }
+
+// Workspace of the backward pass: split sums of a product, then the parts of the column sums.
+struct Columns {
+    const uint16_t* dy = nullptr;
+    int64_t ld = 0;
+    float* parts = nullptr;
+    uint16_t* out = nullptr;
+};
+
+int launch_add(const Plan& plan, const float* partial, int64_t rows, int64_t cols, const uint16_t* bias, uint16_t* out, const Columns& columns,
+               int column_parts, int64_t num_columns, cudaStream_t st) {
+    Parts a;
+    a.partial = partial;
+    a.splits = plan.splits;
+    a.rows = plan.splits > 1 ? rows : 0;
+    a.cols = cols;
+    a.ld = plan.ld_partial;
+    a.bias = bias;
+    a.out = out;
+    a.columns = columns.parts;
+    a.column_parts = column_parts;
+    a.column_blocks = columns.out ? int((num_columns + 31) / 32) : 0;
+    a.num_columns = num_columns;
+    a.column_out = columns.out;
+    const int64_t most = int64_t(tcb::sm_count()) * 8;
+    int64_t blocks = (a.rows * (plan.ld_partial / 4) + 255) / 256;
+    if (blocks > most) blocks = most;
+    if (blocks + a.column_blocks == 0) return TCB_OK;
+    add_parts_kernel<<<unsigned(blocks + a.column_blocks), 256, 0, st>>>(a);
+    TCB_CUDA_TRY(cudaGetLastError());
+    return TCB_OK;
 }
 
 // A tensor map over a row-major [outer, inner] array with rows of `ld` elements.
@@ -535,7 +591,7 @@ int operand_map(const char* who, CUtensorMap* map, const Operand& o) {
 
 template <Source A, Source B, int LOG2_G, bool HAS_ZP>
 int launch(const char* who, const Operand& a, const Operand& b, const uint16_t* scales, const uint8_t* zp, const uint16_t* bias, uint16_t* out,
-           void* workspace, int64_t workspace_bytes, cudaStream_t st) {
+           void* workspace, int64_t workspace_bytes, cudaStream_t st, const Columns& columns = Columns()) {
     const Plan plan = make_plan(a.rows, b.rows, a.contraction, Config<B>::kTileA);
     if (plan.tiles_a * plan.tiles_b * plan.splits > (int64_t(1) << 30)) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: too many output tiles", who);
     if (plan.partial_bytes(a.rows) > workspace_bytes)
@@ -560,6 +616,9 @@ int launch(const char* who, const Operand& a, const Operand& b, const uint16_t* 
     p.out = out;
     p.partial = plan.splits > 1 ? static_cast<float*>(workspace) : nullptr;
     p.ld_partial = plan.ld_partial;
+    p.columns = columns.dy;
+    p.ld_columns = columns.ld;
+    p.column_parts = columns.parts;
     p.scales = scales;
     p.zp = zp;
     p.contraction = a.contraction;
@@ -570,14 +629,10 @@ int launch(const char* who, const Operand& a, const Operand& b, const uint16_t* 
     p.kb_per_split = plan.kb_per_split;
     p.items = p.tiles * plan.splits;
     const int pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1;
-    kernel<<<2 * (p.items < pairs ? p.items : pairs), Config<B>::kThreads, Config<B>::kSmem, st>>>(map_a, map_b, p);
+    const int grid = 2 * (p.items < pairs ? p.items : pairs);
+    kernel<<<grid, Config<B>::kThreads, Config<B>::kSmem, st>>>(map_a, map_b, p);
     TCB_CUDA_TRY(cudaGetLastError());
-    if (plan.splits > 1) {
-        const int64_t blocks = (a.rows * (plan.ld_partial / 4) + 255) / 256, most = int64_t(tcb::sm_count()) * 8;
-        add_parts_kernel<<<unsigned(blocks < most ? blocks : most), 256, 0, st>>>(p.partial, plan.splits, a.rows, b.rows, plan.ld_partial, bias, out);
-        TCB_CUDA_TRY(cudaGetLastError());
-    }
-    return TCB_OK;
+    return launch_add(plan, p.partial, a.rows, b.rows, bias, out, columns, grid * ColumnShare(a.rows).slices, a.rows, st);
 }
 
 int check_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
@@ -616,7 +671,7 @@ int take_linear_status(int* status) { return take_status(g_status, status); }
 extern "C" int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K, int backward) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
     if (!backward) return make_plan(M, N, K, kPairRows).partial_bytes(M);
-    const int64_t dx = make_plan(M, K, N, kPairRows).partial_bytes(M), dw = weight_partial_bytes(M, N, K) + column_bytes(M, N);
+    const int64_t dx = make_plan(M, K, N, kPairRows).partial_bytes(M), dw = weight_partial_bytes(M, N, K) + column_bytes(N);
     return dx > dw ? dx : dw;
 }
 
@@ -657,35 +712,43 @@ extern "C" int tcb_linear_backward(const uint16_t* dy, int64_t ld_dy, const uint
     if (rc == TCB_OK && db_or_null) rc = check_operands(who, dy, dy, db_or_null, nullptr, workspace);
     if (rc != TCB_OK) return rc;
     const int64_t dw_bytes = weight_partial_bytes(M, N, K);
-    const int parts = column_parts(M, N);
-    if (db_or_null && workspace_bytes < dw_bytes + column_bytes(M, N))
+    if (db_or_null && workspace_bytes < dw_bytes + column_bytes(N))
         return tcb::fail(TCB_ERR_BAD_ARG, "%s: the workspace holds %lld bytes, %lld are needed", who, (long long)workspace_bytes,
-                         (long long)(dw_bytes + column_bytes(M, N)));
+                         (long long)(dw_bytes + column_bytes(N)));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dx_or_null) {
         rc = launch<kContraction, kRows, 0, false>(who, Operand{dy, M, N, ld_dy}, Operand{w_or_null, K, N, K}, nullptr, nullptr, nullptr, dx_or_null,
                                                    workspace, workspace_bytes, st);
         if (rc != TCB_OK) return rc;
     }
+    Columns columns;
     if (db_or_null) {
-        float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + dw_bytes);
-        column_sums_kernel<<<dim3(unsigned((N + 63) / 64), unsigned(parts)), 256, 0, st>>>(dy, M, N, ld_dy, partial, db_or_null);
-        if (parts > 1) add_column_sums_kernel<<<unsigned((N + 31) / 32), 256, 0, st>>>(partial, parts, N, db_or_null);
-        TCB_CUDA_TRY(cudaGetLastError());
+        columns.dy = dy;
+        columns.ld = ld_dy;
+        columns.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + dw_bytes);
+        columns.out = db_or_null;
     }
-    if (!dw_or_null) return TCB_OK;
+    if (!dw_or_null) {
+        if (!db_or_null) return TCB_OK;
+        const ColumnShare share(N);
+        const int64_t most = int64_t(tcb::sm_count()) * share.slices, runs = (M + 127) / 128;
+        const int parts = int(runs < most ? runs : most);
+        column_sums_kernel<<<unsigned((int64_t(share.blocks) * parts + 7) / 8), 256, 0, st>>>(dy, M, N, ld_dy, parts, columns.parts);
+        TCB_CUDA_TRY(cudaGetLastError());
+        return launch_add(Plan(), nullptr, 0, 0, nullptr, nullptr, columns, parts, N, st);
+    }
     const Operand a{dy, N, M, ld_dy}, b{q_or_null, K, M, K};
     const uint16_t* scales = scales_or_null;
     uint16_t* dw = dw_or_null;
     const uint8_t* zp = zp_or_null;
     switch (group_size) {
-    case 16: return zp ? launch<kRows, kCodes, 4, true>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st)
-                       : launch<kRows, kCodes, 4, false>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st);
-    case 32: return zp ? launch<kRows, kCodes, 5, true>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st)
-                       : launch<kRows, kCodes, 5, false>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st);
-    case 64: return zp ? launch<kRows, kCodes, 6, true>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st)
-                       : launch<kRows, kCodes, 6, false>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st);
-    default: return zp ? launch<kRows, kCodes, 7, true>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st)
-                       : launch<kRows, kCodes, 7, false>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st);
+    case 16: return zp ? launch<kRows, kCodes, 4, true>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st, columns)
+                       : launch<kRows, kCodes, 4, false>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st, columns);
+    case 32: return zp ? launch<kRows, kCodes, 5, true>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st, columns)
+                       : launch<kRows, kCodes, 5, false>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st, columns);
+    case 64: return zp ? launch<kRows, kCodes, 6, true>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st, columns)
+                       : launch<kRows, kCodes, 6, false>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st, columns);
+    default: return zp ? launch<kRows, kCodes, 7, true>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st, columns)
+                       : launch<kRows, kCodes, 7, false>(who, a, b, scales, zp, nullptr, dw, workspace, workspace_bytes, st, columns);
     }
 }

@@ -162,6 +162,17 @@ def test_shapes_strides_partial_gradients_and_expanded_dy():
     assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
 
 
+@pytest.mark.parametrize("M,N", [(1, 1), (17, 130), (5000, 100), (40000, 9), (3001, 700)])
+def test_bias_gradient_alone_and_beside_the_weight_gradient(M, N):
+    x, w, b, dy = layer(M, N, 64, M)
+    b.requires_grad_(True)
+    (alone,) = torch.autograd.grad(tc.int8_checkpoint_linear(x, w, b), [b], dy)
+    w.requires_grad_(True)
+    _, beside = torch.autograd.grad(tc.int8_checkpoint_linear(x, w, b), [w, b], dy)
+    for got in (alone, beside):
+        close(got.view(1, -1), torch.ones(1, M, dtype=torch.float64, device=DEV), dy.double())
+
+
 def test_empty_batches_and_layers():
     w, b = (torch.randn(s, device=DEV).to(torch.bfloat16).requires_grad_(True) for s in ((8, 32), (8,)))
     x = torch.empty(0, 32, dtype=torch.bfloat16, device=DEV, requires_grad=True)
