@@ -26,8 +26,8 @@
 // Where the output has too few tiles to fill the GPU the contraction is split: each part leaves fp32 sums in a workspace
 // and a second kernel adds them in a fixed order (results do not depend on timing).
 //
-// Warps per CTA: 0 TMA, 1 MMA issue (leader CTA) and TMEM, then four epilogue warps per accumulator of a tile (one per
-// lane quadrant), then eight dequantising producers (weight gradient only).
+// Warps per CTA: 0 TMA, 1 MMA issue (leader CTA) and TMEM, then eight epilogue warps, then eight dequantising producers
+// (weight gradient only).
 //
 // Waits are bounded as in the fused dequantising product; the status word is read by tcb_fused_dequant_linear_check().
 #include <type_traits>
@@ -53,7 +53,8 @@ struct Config {
     static constexpr int kGroups = kDeq ? 2 : 1;             // accumulators per tile = 128-row units of A per CTA
     static constexpr int kBuffers = 2 / kGroups;             // tiles in flight in tensor memory
     static constexpr int kTileA = kGroups * kPairRows;       // output rows per tile
-    static constexpr int kEpilogueWarps = 4 * kGroups;
+    static constexpr int kEpilogueWarps = 8;                 // per lane quadrant: one per accumulator, or two per tile
+    static constexpr int kChunkStep = 2 / kGroups;           // 32-column chunks between two of a warp
     static constexpr int kFirstProducerWarp = kFirstEpilogueWarp + kEpilogueWarps;
     static constexpr int kThreads = 32 * (kFirstProducerWarp + (kDeq ? kProducerWarps : 0));
     static constexpr int kStages = kDeq ? 4 : 6;
@@ -209,8 +210,9 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     auto leader_bar = [&](int id) { return map_to_cta(bar(id), 0); };
     const uint32_t abort_peer = map_to_cta(smem_u32(const_cast<int*>(abort_flag)), rank ^ 1);
 
-    cluster_sync_all();
     if (threadIdx.x == 0) {
+        prefetch_map(&map_a);
+        prefetch_map(&map_b);
         for (int s = 0; s < S; ++s) {
             mbar_init(bar(FULL + s), 2 + (C::kDeq ? 2 * kProducerWarps : 0));
             mbar_init(bar(EMPTY + s), 1);
@@ -228,9 +230,10 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         tmem_relinquish_pair();
     }
     tc_fence_before();
-    cluster_sync_all();
+    cluster_sync_all();   // both CTAs are resident and ready before either touches the other's shared or tensor memory
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    tcb::await_predecessor();
     const int first = int(blockIdx.x >> 1), step = int(gridDim.x >> 1);
 
     if (warp == 0) {
@@ -308,7 +311,9 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     } else if (warp < C::kFirstProducerWarp) {
         // ---------------------------------------------------------------- epilogue
         const int quad = warp & 3;                            // the TMEM lanes this warp may read
-        const int group = (warp - kFirstEpilogueWarp) >> 2;   // the accumulator of the tile
+        const int upper = (warp - kFirstEpilogueWarp) >> 2;
+        const int group = C::kGroups == 2 ? upper : 0;        // the accumulator of the tile
+        const int chunk0 = C::kGroups == 2 ? 0 : upper;       // or every second chunk of the only one
         const StoreMode mode = store_mode(p.out, p.rows_b, p.bias);
         uint32_t* stage = reinterpret_cast<uint32_t*>(smem_e + (C::kStore ? (warp - kFirstEpilogueWarp) * kStoreStageBytes : 0));
         if constexpr (C::kDeq) {
@@ -334,7 +339,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             const int64_t row0 = int64_t(t.ta) * C::kTileA + (int64_t(rank) * t.groups + group) * kTileRows + quad * 32;
             const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + uint32_t((buf + group) * kPairRows);
 #pragma unroll 1
-            for (int c = 0; c < kPairRows / 32; ++c) {
+            for (int c = chunk0; c < kPairRows / 32; c += C::kChunkStep) {
                 const int64_t col0 = int64_t(t.tb) * kPairRows + c * 32;
                 if (col0 >= p.rows_b || group >= t.groups) break;   // warp-uniform
                 uint32_t v[32];
@@ -452,6 +457,7 @@ struct Parts {
     uint16_t* column_out;
 };
 __global__ void __launch_bounds__(256) add_parts_kernel(const Parts p) {
+    tcb::await_predecessor();
     if (int(blockIdx.x) < p.column_blocks) {
         __shared__ float acc[8][32];
         const int r = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -493,6 +499,7 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const Parts p) {
 // Column sums where no weight gradient is wanted: a warp per block of columns and part.
 __global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __restrict__ dy, int64_t rows, int64_t cols, int64_t ld, int parts,
                                                           float* __restrict__ out) {
+    tcb::await_predecessor();
     const ColumnShare share(cols);
     const int64_t unit = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
     if (unit < int64_t(share.blocks) * parts) sum_columns(dy, rows, cols, ld, int(unit % share.blocks), int(unit / share.blocks), parts, out);
@@ -507,19 +514,25 @@ struct Plan {
     int64_t partial_bytes(int64_t rows_a) const { return splits > 1 ? int64_t(splits) * rows_a * ld_partial * 4 : 0; }
 };
 
-// Splits the contraction while tiles leave pairs of CTAs idle, but not into parts of fewer than 8 stages.
+// Splits the contraction where tiles leave pairs of CTAs idle and a shorter sum saves more than the second kernel costs.
+// A stage of a 256 x 256 (512 x 256) tile takes 0.27 (0.55) us, the second kernel 4 us and the partial sums' way through
+// memory at about 5 TB/s.  Measured on 1024 x 1024 x 1024 (forward): 12.4 us in two parts, 10.0 in one.
 Plan make_plan(int64_t rows_a, int64_t rows_b, int64_t contraction, int tile_a) {
     Plan p;
     p.tiles_a = (rows_a + tile_a - 1) / tile_a;
     p.tiles_b = (rows_b + kPairRows - 1) / kPairRows;
     p.num_kb = (contraction + kBlockK - 1) / kBlockK;
-    const int64_t pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1;
-    int64_t splits = pairs / (p.tiles_a * p.tiles_b);
-    if (splits > p.num_kb / 8) splits = p.num_kb / 8;
-    if (splits < 1) splits = 1;
+    p.ld_partial = (rows_b + 7) / 8 * 8;
+    const int64_t pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1, most = pairs / (p.tiles_a * p.tiles_b);
+    const double stage = tile_a > kPairRows ? 0.55 : 0.27, part = double(rows_a) * double(p.ld_partial) * 8.0 / 5e6;
+    double best = double(p.num_kb) * stage;
+    int64_t splits = 1;
+    for (int64_t s = 2; s <= most && s <= p.num_kb; ++s) {
+        const double t = double((p.num_kb + s - 1) / s) * stage + 4.0 + double(s) * part;
+        if (t < best) best = t, splits = s;
+    }
     p.kb_per_split = int((p.num_kb + splits - 1) / splits);
     p.splits = int((p.num_kb + p.kb_per_split - 1) / p.kb_per_split);
-    p.ld_partial = (rows_b + 7) / 8 * 8;
     return p;
 }
 
@@ -557,8 +570,7 @@ int launch_add(const Plan& plan, const float* partial, int64_t rows, int64_t col
     int64_t blocks = (a.rows * (plan.ld_partial / 4) + 255) / 256;
     if (blocks > most) blocks = most;
     if (blocks + a.column_blocks == 0) return TCB_OK;
-    add_parts_kernel<<<unsigned(blocks + a.column_blocks), 256, 0, st>>>(a);
-    TCB_CUDA_TRY(cudaGetLastError());
+    TCB_CUDA_TRY(tcb::launch_overlapped(add_parts_kernel, dim3(unsigned(blocks + a.column_blocks)), dim3(256), 0, st, a));
     return TCB_OK;
 }
 
@@ -630,15 +642,14 @@ int launch(const char* who, const Operand& a, const Operand& b, const uint16_t* 
     p.items = p.tiles * plan.splits;
     const int pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1;
     const int grid = 2 * (p.items < pairs ? p.items : pairs);
-    kernel<<<grid, Config<B>::kThreads, Config<B>::kSmem, st>>>(map_a, map_b, p);
-    TCB_CUDA_TRY(cudaGetLastError());
+    TCB_CUDA_TRY(tcb::launch_overlapped(+kernel, dim3(grid), dim3(Config<B>::kThreads), Config<B>::kSmem, st, map_a, map_b, p));
     return launch_add(plan, p.partial, a.rows, b.rows, bias, out, columns, grid * ColumnShare(a.rows).slices, a.rows, st);
 }
 
 int check_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
-    const int64_t limit = (int64_t(1) << 31) - 1;
+    const int64_t limit = (int64_t(1) << 31) - 1024;   // coordinates of the last tile stay within 32 bits
     if (M < 0 || N < 0 || K < 0) return tcb::fail(TCB_ERR_BAD_ARG, "%s: negative size", who);
-    if (M > limit || N > limit || K > limit) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: dimension beyond 2^31 - 1", who);
+    if (M > limit || N > limit || K > limit) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: dimension beyond 2^31 - 1024", who);
     if (M > 0 && N > 0 && (K <= 0 || K % 8 != 0)) return tcb::fail(TCB_ERR_BAD_ARG, "%s: K = %lld must be a positive multiple of 8", who, (long long)K);
     return TCB_OK;
 }
@@ -733,8 +744,8 @@ extern "C" int tcb_linear_backward(const uint16_t* dy, int64_t ld_dy, const uint
         const ColumnShare share(N);
         const int64_t most = int64_t(tcb::sm_count()) * share.slices, runs = (M + 127) / 128;
         const int parts = int(runs < most ? runs : most);
-        column_sums_kernel<<<unsigned((int64_t(share.blocks) * parts + 7) / 8), 256, 0, st>>>(dy, M, N, ld_dy, parts, columns.parts);
-        TCB_CUDA_TRY(cudaGetLastError());
+        TCB_CUDA_TRY(tcb::launch_overlapped(column_sums_kernel, dim3(unsigned((int64_t(share.blocks) * parts + 7) / 8)), dim3(256), 0, st, dy, M, N, ld_dy,
+                                            parts, columns.parts));
         return launch_add(Plan(), nullptr, 0, 0, nullptr, nullptr, columns, parts, N, st);
     }
     const Operand a{dy, N, M, ld_dy}, b{q_or_null, K, M, K};

@@ -27,6 +27,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
 quantize_mxfp4_kernel(const T* __restrict__ x, int64_t rows, int64_t blocks_per_row, int64_t tiles_k, uint8_t* __restrict__ codes,
                       uint8_t* __restrict__ scales) {
+    tcb::await_predecessor();
     constexpr int kAhead = sizeof(T) == 2 ? 4 : 2;   // rows of a thread loaded at once (fp32: 64 registers either way)
     const int64_t tile_r = blockIdx.x / tiles_k, tile_k = blockIdx.x % tiles_k;
     const int kb = threadIdx.x & 3, r0 = threadIdx.x >> 2;
@@ -82,6 +83,7 @@ __device__ __forceinline__ void decode8(uint32_t c, __nv_bfloat162 scale, uint32
 __global__ void __launch_bounds__(kThreads)
 dequantize_mxfp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows, int64_t blocks_per_row,
                         int64_t tiles_k, uint16_t* __restrict__ out) {
+    tcb::await_predecessor();
     const int64_t tile_r = blockIdx.x / tiles_k, tile_k = blockIdx.x % tiles_k;
     const int kb = threadIdx.x & 3, r0 = threadIdx.x >> 2;
     const int64_t blk = tile_k * 4 + kb;
@@ -142,16 +144,17 @@ extern "C" int tcb_quantize_mxfp4(const void* x, int dtype, int64_t rows, int64_
     if (rc != TCB_OK || tiles == 0) return rc;
     const int64_t bpr = cols / 32, tk = (cols + kTileCols - 1) / kTileCols;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const dim3 grid(unsigned(tiles), 1, 1), block(kThreads, 1, 1);
+    cudaError_t e;
     switch (dtype) {
     case TCB_DT_BF16:
-        quantize_mxfp4_kernel<<<unsigned(tiles), kThreads, 0, st>>>(static_cast<const __nv_bfloat16*>(x), rows, bpr, tk, codes, scales);
+        e = tcb::launch_overlapped(quantize_mxfp4_kernel<__nv_bfloat16>, grid, block, 0, st, static_cast<const __nv_bfloat16*>(x), rows, bpr, tk, codes, scales);
         break;
     case TCB_DT_F16:
-        quantize_mxfp4_kernel<<<unsigned(tiles), kThreads, 0, st>>>(static_cast<const __half*>(x), rows, bpr, tk, codes, scales);
+        e = tcb::launch_overlapped(quantize_mxfp4_kernel<__half>, grid, block, 0, st, static_cast<const __half*>(x), rows, bpr, tk, codes, scales);
         break;
-    default: quantize_mxfp4_kernel<<<unsigned(tiles), kThreads, 0, st>>>(static_cast<const float*>(x), rows, bpr, tk, codes, scales);
+    default: e = tcb::launch_overlapped(quantize_mxfp4_kernel<float>, grid, block, 0, st, static_cast<const float*>(x), rows, bpr, tk, codes, scales);
     }
-    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? TCB_OK : tcb::cuda_fail(e, who);
 }
 
@@ -160,8 +163,7 @@ extern "C" int tcb_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales,
     int64_t tiles = 0;
     const int rc = check_codec(who, rows, cols, out, codes, scales, &tiles);
     if (rc != TCB_OK || tiles == 0) return rc;
-    dequantize_mxfp4_kernel<<<unsigned(tiles), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        codes, scales, rows, cols / 32, (cols + kTileCols - 1) / kTileCols, out);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = tcb::launch_overlapped(dequantize_mxfp4_kernel, dim3(unsigned(tiles)), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), codes,
+                                                 scales, rows, cols / 32, (cols + kTileCols - 1) / kTileCols, out);
     return e == cudaSuccess ? TCB_OK : tcb::cuda_fail(e, who);
 }

@@ -131,6 +131,8 @@ mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     const int my_kb = p.num_kb - kb0 < p.kb_per_cta ? p.num_kb - kb0 : p.kb_per_cta;   // at least 1
 
     if (threadIdx.x == 0) {
+        prefetch_map(&map_w);
+        prefetch_map(&map_ws);
         for (int s = 0; s < S; ++s) {
             mbar_init(bar(FULL + s), 1);
             mbar_init(bar(EMPTY + s), 1);
@@ -138,16 +140,19 @@ mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         mbar_init(bar(DONE), 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tcb::await_predecessor();
+    if (threadIdx.x == 0) {
         // the first tiles of w, before anything else
         for (int s = 0; s < S && s < my_kb; ++s) {
             mbar_arrive_expect_tx(bar(FULL + s), kStageBytes);
             tma_load_2d(ring0 + uint32_t(s) * kCodeBytes, &map_w, (kb0 + s) * 128, tile * kTileRows, bar(FULL + s));
             tma_load_2d(scale0 + uint32_t(s) * kScaleBytes, &map_ws, (kb0 + s) * 128, tile, bar(FULL + s));
         }
-    }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     quantize_rows<COLS, T>(p, int64_t(kb0) * 8, my_kb * 8, x_codes, x_scales);
     fence_proxy_async();   // the codes and scales of x become visible to the tensor core
@@ -298,13 +303,15 @@ int launch(const char* who, const Shape& s, int64_t tiles, const CUtensorMap& ma
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = s.smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
     attr[0].val.clusterDim.y = unsigned(s.parts);
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, map_w, map_ws, p);
     return e == cudaSuccess ? TCB_OK : tcb::cuda_fail(e, who);
 }

@@ -115,8 +115,11 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     auto leader_bar = [&](int id) { return map_to_cta(bar(id), 0); };
     const uint32_t abort_peer = map_to_cta(smem_u32(const_cast<int*>(abort_flag)), rank ^ 1);
 
-    cluster_sync_all();
     if (threadIdx.x == 0) {
+        prefetch_map(&map_x);
+        prefetch_map(&map_w);
+        prefetch_map(&map_xs);
+        prefetch_map(&map_ws);
         for (int s = 0; s < S; ++s) {
             mbar_init(bar(FULL + s), 2);
             mbar_init(bar(EMPTY + s), 1);
@@ -132,9 +135,10 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         tmem_relinquish_pair();
     }
     tc_fence_before();
-    cluster_sync_all();
+    cluster_sync_all();   // both CTAs are resident and ready before either touches the other's shared or tensor memory
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    tcb::await_predecessor();
     const int first = int(blockIdx.x >> 1), step = int(gridDim.x >> 1);
 
     if (warp == 0) {
@@ -286,12 +290,12 @@ extern "C" int64_t tcb_mxfp4_linear_workspace(int64_t M, int64_t N, int64_t K) {
 extern "C" int tcb_mxfp4_linear(const void* x, int dtype, const uint8_t* wq, const uint8_t* w_scales, const uint16_t* bias_or_null, uint16_t* out,
                                 int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
     const char* who = "tcb_mxfp4_linear";
-    const int64_t limit = (int64_t(1) << 31) - 1;
+    const int64_t limit = (int64_t(1) << 31) - 1024;   // coordinates of the last tile stay within 32 bits
     if (dtype < TCB_DT_BF16 || dtype > TCB_DT_F32) return tcb::fail(TCB_ERR_BAD_ARG, "%s: unknown dtype %d", who, dtype);
     if (M < 0 || N < 0 || K < 0) return tcb::fail(TCB_ERR_BAD_ARG, "%s: negative size", who);
     if (M == 0 || N == 0) return TCB_OK;
     if (K <= 0 || K % 32 != 0) return tcb::fail(TCB_ERR_BAD_ARG, "%s: K = %lld must be a positive multiple of 32", who, (long long)K);
-    if (M > limit || N > limit || K > limit) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: dimension beyond 2^31 - 1", who);
+    if (M > limit || N > limit || K > limit) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: dimension beyond 2^31 - 1024", who);
     const int64_t tiles_m = (M + kPairRows - 1) / kPairRows, tiles_n = (N + kPairRows - 1) / kPairRows;
     if (tiles_m * tiles_n > (int64_t(1) << 30)) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: too many output tiles", who);
     if (!x || !wq || !w_scales || !out) return tcb::fail(TCB_ERR_BAD_ARG, "%s: null pointer", who);
@@ -330,8 +334,7 @@ extern "C" int tcb_mxfp4_linear(const void* x, int dtype, const uint8_t* wq, con
     p.tiles = p.tiles_m * p.tiles_n;
     p.num_kb = int((K + kBlockK - 1) / kBlockK);
     const int pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1;
-    mxfp4_linear_kernel<<<2 * (p.tiles < pairs ? p.tiles : pairs), kThreads, kSmem, static_cast<cudaStream_t>(stream)>>>(map_x, map_w, map_xs,
-                                                                                                                      map_ws, p);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = tcb::launch_overlapped(mxfp4_linear_kernel, dim3(2 * (p.tiles < pairs ? p.tiles : pairs)), dim3(kThreads), kSmem,
+                                                 static_cast<cudaStream_t>(stream), map_x, map_w, map_xs, map_ws, p);
     return e == cudaSuccess ? TCB_OK : tcb::cuda_fail(e, who);
 }

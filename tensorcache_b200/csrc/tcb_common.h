@@ -31,4 +31,29 @@ inline bool core_group_size_ok(int g) { return g == 16 || g == 32 || g == 64; }
 // Number of SMs of the current device (cached per device).
 int sm_count();
 
+#ifdef __CUDACC__
+// Programmatic dependent launch: the kernel may start while its predecessor on the stream is finishing.  It must call
+// await_predecessor() before it touches global memory, and afterwards lets its own successor start.  (In that order: a
+// successor's L1 is then empty of anything that was read before this kernel's predecessor had finished.  A kernel whose
+// predecessor READS what it also reads and atomics change in between, as the claims of the row cache, is launched plainly.)
+template <typename... Args>
+cudaError_t launch_overlapped(void (*kernel)(Args...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+__device__ __forceinline__ void await_predecessor() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+#endif
+
 }  // namespace tcb

@@ -80,6 +80,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
@@ -276,8 +277,13 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
 // has made no CUDA call of its own yet (a backward pass runs on one of the autograd engine's) has no context.
 EncodeTiledFn encode_tiled_fn() {
     static std::atomic<EncodeTiledFn> cached{nullptr};
+    static thread_local int bound = -1;
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return nullptr;
+    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+    if (dev != bound) {
+        if (cudaSetDevice(dev) != cudaSuccess) return nullptr;
+        bound = dev;
+    }
     EncodeTiledFn fn = cached.load(std::memory_order_acquire);
     if (!fn) {
         void* sym = nullptr;
