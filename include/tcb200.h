@@ -257,7 +257,7 @@ TCB_API int tcb_fused_dequant_linear(const uint16_t* dense, const uint8_t* q, co
  *   workspace  tcb_linear_workspace(M, N, K, backward ? 1 : 0) bytes on the current device
  *              (NULL where that is 0), 32-byte aligned, used by the call's own work only
  * Requirements: K a positive multiple of 8, and of G in {16, 32, 64, 128} where codes are written
- * or read; x, w, dy and q 16-byte aligned; M, N arbitrary.  With M == 0 or N == 0 nothing is
+ * or read; x, w, dy, q and dw 16-byte aligned; M, N arbitrary.  With M == 0 or N == 0 nothing is
  * computed.  A contraction that is split over the GPU is added up in a fixed order.
  */
 TCB_API int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K, int backward);

@@ -435,6 +435,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     }
 
     // Neither CTA leaves while the other may still arrive on its barriers or read its shared memory.
+    __syncwarp();
     tc_fence_before();
     cluster_sync_all();
     if (warp == 1) {
@@ -719,6 +720,8 @@ extern "C" int tcb_linear_backward(const uint16_t* dy, int64_t ld_dy, const uint
     if (rc == TCB_OK && dw_or_null) {
         if (!scales_or_null) return tcb::fail(TCB_ERR_BAD_ARG, "%s: null pointer", who);
         rc = check_operands(who, dy, q_or_null, dw_or_null, scales_or_null, workspace);
+        // rows of dw are multiples of 32 bytes: aligned to 16 it is stored straight from the registers
+        if (rc == TCB_OK && (reinterpret_cast<uintptr_t>(dw_or_null) & 15)) rc = tcb::fail(TCB_ERR_ALIGNMENT, "%s: dw must be 16-byte aligned", who);
     }
     if (rc == TCB_OK && db_or_null) rc = check_operands(who, dy, dy, db_or_null, nullptr, workspace);
     if (rc != TCB_OK) return rc;

@@ -114,7 +114,7 @@ dequantize_mxfp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __rest
             uint32_t o[8];
             decode8(w[2 * k], scale, o);
             decode8(w[2 * k + 1], scale, o + 4);
-            stg_stream_v8(dst + 16 * k, o);
+            tcb::stg_stream_v8(dst + 16 * k, o);
         }
     }
 }

@@ -234,6 +234,7 @@ mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         }
     }
 
+    __syncwarp();
     if (parts > 1) {
         cluster_sync_all();   // every CTA's sums are written (or it has given up)
         const int rows_each = kTileRows / int(parts), first = int(rank) * rows_each;

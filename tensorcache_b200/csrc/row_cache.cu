@@ -32,23 +32,12 @@ struct Split {
     static constexpr int R = G % 32 == 0 ? 32 : V;                 // values per thread, read
 };
 
-// Streamed once: 32-byte accesses that leave L2 first.
-__device__ __forceinline__ void ldg_stream_v8(const void* p, uint32_t* w) {
-    asm volatile("ld.global.nc.L1::no_allocate.L2::evict_first.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                 : "l"(p));
-}
-__device__ __forceinline__ void stg_stream_v8(void* p, const uint32_t* w) {
-    asm volatile("st.global.L2::evict_first.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-}
 // BYTES contiguous bytes: 32 at a time where a unit's size keeps them aligned, else 16, else 8.
 template <int BYTES>
 __device__ __forceinline__ void load_bytes(const void* p, uint32_t* w) {
     if constexpr (BYTES % 32 == 0) {
 #pragma unroll
-        for (int i = 0; i < BYTES / 32; ++i) ldg_stream_v8(static_cast<const uint8_t*>(p) + 32 * i, w + 8 * i);
+        for (int i = 0; i < BYTES / 32; ++i) tcb::ldg_stream_v8(static_cast<const uint8_t*>(p) + 32 * i, w + 8 * i);
     } else if constexpr (BYTES % 16 == 0) {
 #pragma unroll
         for (int i = 0; i < BYTES / 16; ++i) {
@@ -68,7 +57,7 @@ template <int BYTES>
 __device__ __forceinline__ void store_bytes(void* p, const uint32_t* w) {
     if constexpr (BYTES % 32 == 0) {
 #pragma unroll
-        for (int i = 0; i < BYTES / 32; ++i) stg_stream_v8(static_cast<uint8_t*>(p) + 32 * i, w + 8 * i);
+        for (int i = 0; i < BYTES / 32; ++i) tcb::stg_stream_v8(static_cast<uint8_t*>(p) + 32 * i, w + 8 * i);
     } else if constexpr (BYTES % 16 == 0) {
 #pragma unroll
         for (int i = 0; i < BYTES / 16; ++i) __stcs(static_cast<uint4*>(p) + i, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));

@@ -10,18 +10,6 @@
 
 namespace {
 
-// Streamed once: 32-byte accesses that leave L2 first.
-__device__ __forceinline__ void ldg_stream_v8(const void* p, uint32_t* w) {
-    asm volatile("ld.global.nc.L1::no_allocate.L2::evict_first.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                 : "l"(p));
-}
-__device__ __forceinline__ void stg_stream_v8(void* p, const uint32_t* w) {
-    asm volatile("st.global.L2::evict_first.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-}
-
 // One block of 32 values.
 template <typename T>
 struct Block32 {
@@ -30,7 +18,7 @@ struct Block32 {
 
     __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-        for (int i = 0; i < kWords; i += 8) ldg_stream_v8(reinterpret_cast<const uint32_t*>(p) + i, w + i);
+        for (int i = 0; i < kWords; i += 8) tcb::ldg_stream_v8(reinterpret_cast<const uint32_t*>(p) + i, w + i);
     }
     __device__ __forceinline__ void zero() {
 #pragma unroll

@@ -144,6 +144,7 @@ def test_linear_entry_points_refuse_bad_arguments(built_lib):
     assert bwd(p, 8, p, p, p, None, None, p, None, 4, 8, 32, 24, p, 0) == _lib.ERR_GROUP_SIZE
     assert bwd(p, 8, p, p, p, None, None, p, None, 4, 8, 48, 32, p, 0) == _lib.ERR_BAD_ARG
     assert bwd(p, 8, p, p, None, None, None, p, None, 4, 8, 32, 32, p, 0) == _lib.ERR_BAD_ARG    # scales missing
+    assert bwd(p, 8, p, p, p, None, None, p + 2, None, 4, 8, 32, 32, p, 0) == _lib.ERR_ALIGNMENT  # dw
     assert bwd(p, 8, None, p, p, None, p, None, None, 4, 8, 32, 32, p, 0) == _lib.ERR_BAD_ARG    # weight missing
     assert bwd(p, 8, None, None, None, None, None, None, p, 4, 8, 32, 32, p, 4) == _lib.ERR_BAD_ARG  # workspace too small
     assert L.tcb_linear_workspace(0, 8, 32, 1) == 0 and L.tcb_linear_workspace(4, 8, 32, 0) == 0
