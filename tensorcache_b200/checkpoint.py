@@ -61,20 +61,20 @@ def _backward(dy: torch.Tensor, sizes, weight, q, scales, zp, group_size: int, n
     in ``q``, which is one buffer then."""
     M, N, K = sizes
     dev = dy.device
-    bf16 = torch.bfloat16
     with _lib.on_device(dev):
-        dy = dy.reshape(M, N)
+        if dy.dim() != 2:
+            dy = dy.reshape(M, N)
         if N % 8 == 0:
             dy, ld = _operand(dy), N
         else:       # rows of dy must start on 16-byte boundaries
             ld = -(-N // 8) * 8
-            padded = torch.zeros((M, ld), dtype=bf16, device=dev)
+            padded = dy.new_zeros((M, ld))
             padded[:, :N] = dy
             dy = padded
-        make = torch.empty if M and N else torch.zeros
-        dx = make((M, K), dtype=bf16, device=dev) if need_dx else None
-        dw = make((N, K), dtype=bf16, device=dev) if need_dw else None
-        db = make(N, dtype=bf16, device=dev) if need_db else None
+        make = dy.new_empty if M and N else dy.new_zeros
+        dx = make((M, K)) if need_dx else None
+        dw = make((N, K)) if need_dw else None
+        db = make(N) if need_db else None
         if M and N and (need_dx or need_dw or need_db):
             ws, nbytes = _workspace(M, N, K, 1, dev)
             w = _operand(weight) if need_dx else None
@@ -94,10 +94,10 @@ class _CheckpointLinear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, group_size):
         N, K = weight.shape
         dev = x.device
-        x2 = _operand(x.reshape(-1, K))
+        x2 = _operand(x if x.dim() == 2 else x.reshape(-1, K))
         M = x2.shape[0]
-        y = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
-        need_dx, need_dw = ctx.needs_input_grad[:2]
+        y = x2.new_empty((M, N))
+        need_dx, need_dw, _, _ = ctx.needs_input_grad
         # codes [M, K], then scales [M, K / G]: one buffer (M K is a multiple of 16, so the scales are aligned)
         kept = torch.empty(M * K + 2 * (M * K // group_size), dtype=torch.uint8, device=dev) if need_dw else None
         if M and N:
@@ -118,7 +118,7 @@ class _CheckpointLinear(torch.autograd.Function):
         kept, weight = ctx.saved_tensors
         need_dx, need_dw, need_db, _ = ctx.needs_input_grad
         dx, dw, db = _backward(dy, ctx.sizes, weight, kept, None, None, ctx.group_size, need_dx, need_dw, need_db)
-        return dx.view(ctx.x_shape) if need_dx else None, dw, db, None
+        return dx.view(ctx.x_shape) if need_dx and len(ctx.x_shape) != 2 else dx, dw, db, None
 
 
 class _FusedDequantLinear(torch.autograd.Function):

@@ -260,6 +260,12 @@ mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 }
 
 // Shape of a launch; stages == 0: this kernel does not take the sizes.
+//
+// Rules and what they were measured on (us, consecutive calls on different weights; rows of x x rows of w x 4096):
+//   few rows against the tiles of 256 x 256 with their own quantisation
+//                                   1 x 14336: 9.1 / 14.9   16 x 14336: 11.9 / 12.9   32 x 4096: 7.3 / 11.0   32 x 14336: 14.6 / 12.9
+//     the last because every CTA quantises all of its K for every row: above 16 rows only where that is at most 8 stages
+//   K split over a cluster or not   1 x 4096: 4.6 / 7.0     1 x 1024: 3.7 / 6.8; with two CTAs an SM 1 x 14336: 8.2, 1 x 4096: 4.9
 struct Shape {
     int cols, parts, kb_per_cta, stages;
     uint32_t smem;
@@ -276,6 +282,7 @@ Shape few_rows_shape(int64_t M, int64_t N, int64_t K) {
         s.parts /= 2;
         per = (num_kb + s.parts - 1) / s.parts;
     }
+    if (M > 16 && per > 8) return s;
     s.kb_per_cta = int(per);
     const uint32_t fixed = uint32_t(per) * (s.cols * 128 + 1024) + 1024 /* alignment */ + 256 /* barriers */;
     // a deep ring where every CTA has an SM to itself, else one that leaves room for a second CTA

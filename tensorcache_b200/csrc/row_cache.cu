@@ -23,7 +23,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int64_t kScanRows = 1024;
+constexpr int64_t kScanRows = 1024;   // rows of 768 bf16 values, us, scan / claim: 1: 1.8 / 4.1, 1024: 3.6 / 4.8, 2048: 5.8 / 5.2, 16384: 57 / 10.5
 
 template <int G>
 struct Split {
@@ -178,7 +178,8 @@ write_rows_scan_kernel(const T* __restrict__ x, const int64_t* __restrict__ indi
     }
 }
 
-// Row and unit of a position in the list of all rows' units; Index is 32 bits wide where that suffices (the division).
+// Row and unit of a position in the list of all rows' units; Index is 32 bits wide where that suffices: the division costs
+// 57,088 rows of 768 written 29.1 us instead of 30.2.
 template <typename Index>
 struct Place {
     Index t, k;
