@@ -32,10 +32,10 @@ inline bool core_group_size_ok(int g) { return g == 16 || g == 32 || g == 64; }
 int sm_count();
 
 #ifdef __CUDACC__
-// Programmatic dependent launch: the kernel may start while its predecessor on the stream is finishing.  It must call
+// Programmatic dependent launch: the kernel may start while its predecessor on the stream is finishing.  It calls
 // await_predecessor() before it touches global memory, and afterwards lets its own successor start.  (In that order: a
-// successor's L1 is then empty of anything that was read before this kernel's predecessor had finished.  A kernel whose
-// predecessor READS what it also reads and atomics change in between, as the claims of the row cache, is launched plainly.)
+// successor's L1 is then empty of anything that was read before this kernel's predecessor had finished.  What a predecessor
+// both reads and changes must be read past L1.)
 template <typename... Args>
 cudaError_t launch_overlapped(void (*kernel)(Args...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
