@@ -5,7 +5,10 @@ Drop-in for the reference's API on that path -- ``compress`` / ``decompress``,
 ``quantize_int8_g32`` / ``quantize_int8_adaptive`` / ``dequantize_int8_g32``,
 ``FusedDequantLinear``, ``ZeroCopyTensorStreamer``, ``FeatureCacheWriter`` /
 ``FeatureCacheDataset`` -- on hand-written sm_100a CUDA kernels behind a C ABI
-(``include/tcb200.h``, ``libtcb200.so``).  There is no Triton, no backend switch
+(``include/tcb200.h``, ``libtcb200.so``).  Beside it stand low-bit operators the reference does
+not have: the MXFP4 codec and product (``quantize_mxfp4``, ``dequantize_mxfp4``, ``mxfp4_matmul``),
+linear layers that train with their input kept in 8 bits (``int8_checkpoint_linear``,
+``fused_dequant_linear``) and the device-resident ``DeviceFeatureCache``.  There is no Triton, no backend switch
 and no CPU implementation: without the built library or a CUDA device the
 compute calls raise.
 """
