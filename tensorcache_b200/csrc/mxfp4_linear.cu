@@ -130,12 +130,13 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    cluster_sync_all();   // both CTAs of the pair are resident before either touches the other's shared or tensor memory
     if (warp == 1) {
         tmem_alloc_pair(smem_u32(tmem_slot), 512);
         tmem_relinquish_pair();
     }
     tc_fence_before();
-    cluster_sync_all();   // both CTAs are resident and ready before either touches the other's shared or tensor memory
+    cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     tcb::await_predecessor();
