@@ -260,6 +260,80 @@ def test_calls_from_threads_that_have_made_no_cuda_call():
     assert not errors and all(torch.equal(a, c) for a, c in zip(want, got))
 
 
+def test_step_on_another_stream():
+    """Forward and backward on a side stream, with work of the default stream ahead of it and behind it."""
+    x, w, b, dy = layer(700, 136, 256, 4)
+    x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)
+    want = torch.autograd.grad(tc.int8_checkpoint_linear(x, w, b), [x, w, b], dy)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        big = torch.randn(4096, 4096, device=DEV) @ torch.randn(4096, 4096, device=DEV)     # the side stream runs beside this
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = torch.autograd.grad(tc.int8_checkpoint_linear(x, w, b), [x, w, b], dy)
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, c) for a, c in zip(want, got)) and big.shape == (4096, 4096)
+
+
+def test_capture_with_forks_joins_copies_and_fills_between_the_kernels():
+    """Kernels that may start under their predecessor, captured where that predecessor is a copy, a fill or a join of two
+    streams."""
+    x, w, b, dy = layer(300, 64, 128, 6)
+    wq, ws, _ = tc.quantize_mxfp4(w)
+    base, kept = x.clone(), torch.empty_like(x)
+
+    def run(side):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            doubled = x * 2
+            other = tc.mxfp4_matmul(doubled, wq, ws, b)
+        kept.zero_()
+        a = tc.int8_checkpoint_linear(x, w, b)
+        main.wait_stream(side)
+        c = tc.mxfp4_matmul(doubled, wq, ws, b)
+        kept.copy_(doubled)
+        d = tc.int8_checkpoint_linear(kept, w)
+        kept.fill_(1)
+        e = tc.dequantize_mxfp4(*tc.quantize_mxfp4(kept))
+        return other, a, c, d, e
+
+    side = torch.cuda.Stream()
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        run(side)
+    torch.cuda.current_stream().wait_stream(warm)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(side)
+    for scale in (1.0, 0.5, -2.0):
+        x.copy_(base * scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(g, e) for g, e in zip(got, run(side)))
+
+
+def test_values_that_are_not_finite_reach_the_output_but_not_the_weight_gradient():
+    x, w, _, dy = layer(40, 24, 64, 8)
+    x[3, 5], x[4, 6] = float("inf"), float("nan")
+    w.requires_grad_(True)
+    y = tc.int8_checkpoint_linear(x, w)
+    (dw,) = torch.autograd.grad(y, [w], dy)
+    bad = ~y.detach().isfinite().all(1)
+    assert bad.nonzero().flatten().tolist() == [3, 4]
+    close(dw, dy.double().t(), decoded(*plain.int8_encode(x, 32), 32))
+
+
+def test_gradients_of_gradients_are_refused():
+    x, w, _, _ = layer(8, 8, 32)
+    x.requires_grad_(True), w.requires_grad_(True)
+    (gx,) = torch.autograd.grad(tc.int8_checkpoint_linear(x, w).float().square().sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):
+        gx.float().sum().backward()
+
+
 def test_module_trains_in_a_stack():
     """Input gradient through two layers and a non-linearity between them, against the same stack in 64 bits on the
     bf16 intermediates (so that each product is checked on its own)."""

@@ -147,3 +147,41 @@ def test_offsets_beyond_2_31():
     many = torch.cat([torch.full((2000,), -1, device=DEV), idx.flip(0)])
     cache.write(many, torch.cat([torch.zeros(2000, width, dtype=torch.bfloat16, device=DEV), x]))
     assert torch.equal(cache.read(idx.flip(0)), tc.dequantize_int8_g32(q, s, shape))
+
+
+@pytest.mark.parametrize("new", [70, 1100])
+def test_rows_that_are_whole_samples(new):
+    """[446, 768] a row: several parts a row in the kernel of few rows, and more than one unit list per block in the other."""
+    rows = 1200
+    cache = tc.DeviceFeatureCache(rows, (446, 768), 32, DEV)
+    x = torch.randn(new, 446, 768, device=DEV).to(torch.bfloat16)
+    idx = torch.randperm(rows, device=DEV)[:new]
+    idx[new // 2] = idx[0]                  # row 0 of x is overwritten by a later one
+    cache.write(idx, x)
+    out = cache.read(idx)
+    assert torch.equal(out[0], out[new // 2])
+    q, s, _ = tc.quantize_int8_g32(x[1:])
+    assert torch.equal(out[1:], tc.dequantize_int8_g32(q, s, x[1:].shape))
+    untouched = torch.ones(rows, dtype=torch.bool, device=DEV)
+    untouched[idx] = False
+    assert not bool(cache.codes[untouched].any()) and not bool(cache.scales[untouched].any())
+
+
+def test_writes_and_reads_interleaved_on_one_stream():
+    """Many calls of both write kernels and reads between them without a synchronisation: every read sees the writes ahead of it."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    rows, width = 3000, 64
+    cache, model = tc.DeviceFeatureCache(rows, width, 16, DEV), Model(rows, width, 16)
+    steps, order = [], torch.arange(rows, device=DEV)
+    for i in range(24):
+        new = 2500 if i % 2 else 40
+        idx = torch.randint(0, rows, (new,), generator=g, device=DEV)
+        steps.append((idx, torch.randn(new, width, generator=g, device=DEV)))
+    torch.cuda.synchronize()
+    reads = []
+    for idx, x in steps:
+        cache.write(idx, x)
+        reads.append(cache.read(order))
+    for (idx, x), out in zip(steps, reads):
+        model.write(idx, x)
+        assert torch.equal(out.cpu(), model.read(order))
