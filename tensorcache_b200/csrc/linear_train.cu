@@ -344,23 +344,14 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             for (int c = chunk0; c < kPairRows / 32; c += C::kChunkStep) {
                 const int64_t col0 = int64_t(t.tb) * kPairRows + c * 32;
                 if (col0 >= p.rows_b || group >= t.groups) break;   // warp-uniform
+                if (p.partial) {
+                    store_32x32_f32(taddr + uint32_t(c * 32), p.partial + int64_t(t.split) * p.rows_a * p.ld_partial, p.ld_partial, row0, p.rows_a, col0);
+                    continue;
+                }
                 uint32_t v[32];
                 tmem_ld32(taddr + uint32_t(c * 32), v);
                 tmem_ld_wait();
-                if (p.partial == nullptr) {
-                    store_32x32(p.out, p.rows_b, row0, p.rows_a, col0, p.rows_b, p.bias, v, mode, stage);
-                } else if (row0 + lane < p.rows_a) {
-                    // ld_partial is a multiple of 8 and padded columns may be written
-                    float* dst = p.partial + (int64_t(t.split) * p.rows_a + row0 + lane) * p.ld_partial + col0;
-#pragma unroll
-                    for (int h = 0; h < 4; ++h)
-                        if (col0 + 8 * h < p.rows_b) {
-                            uint32_t w[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) w[i] = v[8 * h + i];
-                            st_global_v8(dst + 8 * h, w);
-                        }
-                }
+                store_32x32(p.out, p.rows_b, row0, p.rows_a, col0, p.rows_b, p.bias, v, mode, stage);
             }
             tc_fence_before();
             __syncwarp();
