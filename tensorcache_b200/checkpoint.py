@@ -20,7 +20,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .fused_linear import SUPPORTED_GROUP_SIZES, _aligned, _check_common, _launch
+from .fused_linear import SUPPORTED_GROUP_SIZES, _check_common, _launch, _operand_on
 
 
 def _check_dense(name: str, t: torch.Tensor, device: torch.device) -> None:
@@ -41,7 +41,7 @@ def _check_layer(weight: torch.Tensor, bias: Optional[torch.Tensor], K: int, dev
 
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
-    return _aligned(t.contiguous())
+    return _operand_on(t, t.device, 16)
 
 
 @lru_cache(maxsize=1024)
@@ -81,7 +81,7 @@ def _backward(dy: torch.Tensor, sizes, weight, q, scales, zp, group_size: int, n
             adr = _lib.address
             codes = sc = None
             if need_dw:
-                q = _aligned(q)
+                q = _operand(q)
                 codes = q.data_ptr()
                 sc = codes + M * K if scales is None else scales.data_ptr()
             _lib.check(_lib.lib().tcb_linear_backward(dy.data_ptr(), ld, adr(w), codes, sc, adr(zp), adr(dx), adr(dw), adr(db),

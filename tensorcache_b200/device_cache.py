@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from .codec import _DTYPES, _check_group_size
-from .fused_linear import _aligned
+from .fused_linear import _operand_on
 
 Indices = Union[torch.Tensor, Sequence[int]]
 
@@ -60,18 +60,17 @@ class DeviceFeatureCache:
         return f"DeviceFeatureCache({self.num_rows} x {self.row_shape}, G={self.group_size}, {self.device})"
 
     def _indices(self, indices: Indices) -> torch.Tensor:
-        idx = torch.as_tensor(indices)
-        if idx.dtype is not torch.int64 or idx.dim() != 1:
-            if idx.numel() == 0:
-                idx = idx.long()
-            if idx.dim() != 1 or idx.dtype not in (torch.int64, torch.int32):
+        idx = indices if isinstance(indices, torch.Tensor) else torch.as_tensor(indices)
+        if idx.dtype != torch.int64 or idx.dim() != 1:
+            if idx.dim() != 1 or idx.dtype != torch.int32 and idx.numel():
                 raise ValueError(f"indices must be one-dimensional int64 or int32, got {tuple(idx.shape)} of {idx.dtype}")
-        if idx.is_cuda:
-            if idx.device != self.device:
-                raise ValueError(f"indices are on {idx.device}, the cache is on {self.device}")
-        elif idx.numel() and int(idx.max()) >= self.num_rows:
-            raise IndexError(f"row {int(idx.max())} in a cache of {self.num_rows} rows")
-        return idx.to(device=self.device, dtype=torch.int64).contiguous()
+            idx = idx.long()
+        if not idx.is_cuda:
+            if idx.numel() and int(idx.max()) >= self.num_rows:
+                raise IndexError(f"row {int(idx.max())} in a cache of {self.num_rows} rows")
+        elif idx.device != self.device:
+            raise ValueError(f"indices are on {idx.device}, the cache is on {self.device}")
+        return _operand_on(idx, self.device, 8)
 
     def write(self, indices: Indices, x: torch.Tensor) -> None:
         """Quantises row ``t`` of ``x`` (``[n, *row_shape]`` or ``[n, width]``) into row ``indices[t]``.
@@ -83,13 +82,13 @@ class DeviceFeatureCache:
         with _lib.on_device(self.device):
             idx = self._indices(indices)
             n = idx.numel()
-            if tuple(x.shape) not in ((n, *self.row_shape), (n, self.width)):
+            if x.shape != (n, self.width) and x.shape != (n, *self.row_shape):
                 raise ValueError(f"expected {n} rows of {self.row_shape}, got {tuple(x.shape)}")
             if x.is_cuda and x.device != self.device:
                 raise ValueError(f"x is on {x.device}, the cache is on {self.device}")
             if x.dtype not in _DTYPES:
                 x = x.float()
-            xd = _aligned(x.to(self.device).contiguous(), 32)
+            xd = _operand_on(x, self.device, 32)
             _lib.check(_lib.lib().tcb_cache_write(xd.data_ptr(), _DTYPES[xd.dtype], idx.data_ptr(), n, self.codes.data_ptr(),
                                                   self.scales.data_ptr(), self.num_rows, self.width, self.group_size,
                                                   self._claims.data_ptr(), _lib.stream_of(self.device)))
@@ -101,13 +100,13 @@ class DeviceFeatureCache:
             idx = self._indices(indices)
             n = idx.numel()
             if out_buffer is None:
-                out_buffer = torch.empty((n, *self.row_shape), dtype=torch.bfloat16, device=self.device)
-            if out_buffer.numel() != n * self.width or out_buffer.dtype != torch.bfloat16:
+                out_buffer = self.scales.new_empty((n, *self.row_shape))
+            elif out_buffer.numel() != n * self.width or out_buffer.dtype != torch.bfloat16:
                 raise ValueError(f"out_buffer must be a bf16 tensor of {n} rows of {self.width} values")
-            if out_buffer.numel() == 0:
+            if n == 0 or self.width == 0:
                 return out_buffer
             direct = out_buffer.device == self.device and out_buffer.is_contiguous() and out_buffer.data_ptr() % 32 == 0
-            od = out_buffer if direct else torch.empty(n * self.width, dtype=torch.bfloat16, device=self.device)
+            od = out_buffer if direct else self.scales.new_empty(n * self.width)
             _lib.check(_lib.lib().tcb_cache_read(self.codes.data_ptr(), self.scales.data_ptr(), self.num_rows, self.width, self.group_size,
                                                  idx.data_ptr(), n, od.data_ptr(), _lib.stream_of(self.device)))
             if not direct:

@@ -35,6 +35,16 @@ def _aligned(t: Optional[torch.Tensor], nbytes: int = 16) -> Optional[torch.Tens
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _operand_on(t: torch.Tensor, device: torch.device, nbytes: int) -> torch.Tensor:
+    """``t`` contiguous on ``device`` with an aligned start: itself where it is that already (the common case is made cheap: a
+    call of ten microseconds notices every conversion that does nothing)."""
+    if t.device != device:
+        t = t.to(device)
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t if t.data_ptr() % nbytes == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def _launch(dense, q, scales, zp, bias, out, R_d, R_q, K, group_size, quant_is_rhs):
     dense, q = _aligned(dense), _aligned(q)
     dev, adr = dense.device, _lib.address

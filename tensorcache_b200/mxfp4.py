@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from .codec import _DTYPES, _compute_device
-from .fused_linear import _aligned
+from .fused_linear import _operand_on
 
 BLOCK = 32          # values that share a scale
 _TILE_ROWS = 128    # a scale tile covers 128 rows x 4 blocks
@@ -29,7 +29,7 @@ def _rows_cols(shape) -> Tuple[int, int]:
     cols = int(shape[-1])
     if cols % BLOCK != 0:
         raise ValueError(f"the last dimension ({cols}) must be a multiple of {BLOCK}")
-    return math.prod(shape[:-1]), cols
+    return int(shape[0]) if len(shape) == 2 else math.prod(shape[:-1]), cols
 
 
 def mxfp4_scale_bytes(rows: int, cols: int) -> int:
@@ -72,10 +72,10 @@ def quantize_mxfp4(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, Tuple[i
         x = x.float()
     dev = _compute_device(x)
     with _lib.on_device(dev):
-        codes = torch.empty((*x.shape[:-1], cols // 2), dtype=torch.uint8, device=dev)
-        scales = torch.empty(mxfp4_scale_bytes(rows, cols), dtype=torch.uint8, device=dev)
-        if codes.numel():
-            xd = _aligned((x if x.is_cuda else x.to(dev)).contiguous(), 32)
+        codes = torch.empty((rows, cols // 2) if x.dim() == 2 else (*x.shape[:-1], cols // 2), dtype=torch.uint8, device=dev)
+        scales = codes.new_empty(mxfp4_scale_bytes(rows, cols))
+        if rows and cols:
+            xd = _operand_on(x, dev, 32)
             _lib.check(_lib.lib().tcb_quantize_mxfp4(xd.data_ptr(), _DTYPES[x.dtype], rows, cols, codes.data_ptr(), scales.data_ptr(),
                                                      _lib.stream_of(dev)))
     if not x.is_cuda:
@@ -103,12 +103,12 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, orig_shape: Tupl
     dev = _compute_device(codes)
     if out_buffer is None:
         out_buffer = torch.empty(tuple(orig_shape), dtype=torch.bfloat16, device=codes.device)
-    if out_buffer.numel() != rows * cols or out_buffer.dtype != torch.bfloat16:
+    elif out_buffer.numel() != rows * cols or out_buffer.dtype != torch.bfloat16:
         raise ValueError("out_buffer must be a bf16 tensor of the decoded size")
-    if out_buffer.numel() == 0:
+    if rows == 0 or cols == 0:
         return out_buffer
     with _lib.on_device(dev):
-        cd, sd = _aligned(codes.contiguous().to(dev)), _aligned(scales.contiguous().to(dev))
+        cd, sd = _operand_on(codes, dev, 16), _operand_on(scales, dev, 16)
         direct = out_buffer.device == dev and out_buffer.is_contiguous() and out_buffer.data_ptr() % 32 == 0
         od = out_buffer if direct else torch.empty(rows * cols, dtype=torch.bfloat16, device=dev)
         _lib.check(_lib.lib().tcb_dequantize_mxfp4(cd.data_ptr(), sd.data_ptr(), rows, cols, od.data_ptr(), _lib.stream_of(dev)))
@@ -139,7 +139,7 @@ def mxfp4_matmul(x: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor, bias
     _check_codes(wq, w_scales, N, K)
     if x.dtype not in _DTYPES:
         raise ValueError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
-    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype != torch.bfloat16 or bias.device != x.device):
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != N or bias.dtype != torch.bfloat16 or bias.device != x.device):
         raise ValueError(f"bias must be bf16 [{N}] on {x.device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
     if wq.device != x.device:
         raise ValueError(f"x is on {x.device}, the weight on {wq.device}")
@@ -147,15 +147,16 @@ def mxfp4_matmul(x: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor, bias
         raise ValueError("mxfp4_matmul has no gradient: call it under torch.no_grad() or detach x")
     if not x.is_cuda:
         raise RuntimeError("mxfp4_matmul runs on CUDA tensors only (no CPU fallback)")
-    x2 = x.reshape(-1, K)
-    M, dev = x2.shape[0], x.device
+    dev = x.device
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    M = x2.shape[0]
     out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
     if M and N:
         with _lib.on_device(dev):
-            x2, cd, sd = _aligned(x2.contiguous(), 32), _aligned(wq.contiguous()), _aligned(w_scales.contiguous())
+            x2, cd, sd = _operand_on(x2, dev, 32), _operand_on(wq, dev, 16), _operand_on(w_scales, dev, 16)
             b = None if bias is None else bias.contiguous()
             nbytes = _workspace_bytes(M, N, K, dev.index)     # x in MXFP4; 0 for few rows
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
             _lib.check(_lib.lib().tcb_mxfp4_linear(x2.data_ptr(), _DTYPES[x2.dtype], cd.data_ptr(), sd.data_ptr(), _lib.address(b), out.data_ptr(),
                                                    M, N, K, _lib.address(ws), nbytes, _lib.stream_of(dev)))
-    return out.view(*x.shape[:-1], N)
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], N)
