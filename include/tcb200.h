@@ -254,13 +254,14 @@ TCB_API int tcb_fused_dequant_linear(const uint16_t* dense, const uint8_t* q, co
  * deq(q) is the bf16 number tcb_decompress_amo / tcb_decompress_sym gives for the codes
  * (zp != NULL: uint8 codes, else signed).  All other arrays are bf16.
  *   ld_dy      elements between rows of dy: a multiple of 8, at least N
- *   workspace  tcb_linear_workspace(M, N, K, backward ? 1 : 0) bytes on the current device
- *              (NULL where that is 0), 32-byte aligned, used by the call's own work only
+ *   workspace  tcb_linear_workspace(M, N, K, gradients) bytes on the current device (NULL where
+ *              that is 0), 32-byte aligned, used by the call's own work only; gradients: 0 for
+ *              forward, else the sum of 1 (dx), 2 (dw) and 4 (db) for those wanted
  * Requirements: K a positive multiple of 8, and of G in {16, 32, 64, 128} where codes are written
  * or read; x, w, dy, q and dw 16-byte aligned; M, N arbitrary.  With M == 0 or N == 0 nothing is
  * computed.  A contraction that is split over the GPU is added up in a fixed order.
  */
-TCB_API int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K, int backward);
+TCB_API int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K, int gradients);
 TCB_API int tcb_linear_forward(const uint16_t* x, const uint16_t* w, const uint16_t* bias_or_null, uint16_t* y,
                                uint8_t* q_or_null, uint16_t* scales_or_null, int64_t M, int64_t N, int64_t K,
                                int group_size, void* workspace, int64_t workspace_bytes, void* stream);

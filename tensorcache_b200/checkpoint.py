@@ -45,14 +45,14 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
 
 
 @lru_cache(maxsize=1024)
-def _workspace_bytes(M: int, N: int, K: int, backward: int, device_index: int) -> int:
+def _workspace_bytes(M: int, N: int, K: int, gradients: int, device_index: int) -> int:
     """Scratch bytes of a pass of these sizes (they depend on the device's number of SMs)."""
-    return _lib.lib().tcb_linear_workspace(M, N, K, backward)
+    return _lib.lib().tcb_linear_workspace(M, N, K, gradients)
 
 
-def _workspace(M: int, N: int, K: int, backward: int, device: torch.device):
+def _workspace(M: int, N: int, K: int, gradients: int, device: torch.device):
     """(buffer or None, bytes): the split sums of one call, from the caching allocator of the current stream."""
-    nbytes = _workspace_bytes(M, N, K, backward, device.index)
+    nbytes = _workspace_bytes(M, N, K, gradients, device.index)
     return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None), nbytes
 
 
@@ -76,7 +76,7 @@ def _backward(dy: torch.Tensor, sizes, weight, q, scales, zp, group_size: int, n
         dw = make((N, K)) if need_dw else None
         db = make(N) if need_db else None
         if M and N and (need_dx or need_dw or need_db):
-            ws, nbytes = _workspace(M, N, K, 1, dev)
+            ws, nbytes = _workspace(M, N, K, need_dx + 2 * need_dw + 4 * need_db, dev)
             w = _operand(weight) if need_dx else None
             adr = _lib.address
             codes = sc = None
@@ -113,12 +113,19 @@ class _CheckpointLinear(torch.autograd.Function):
         return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        kept, weight = ctx.saved_tensors
-        need_dx, need_dw, need_db, _ = ctx.needs_input_grad
-        dx, dw, db = _backward(dy, ctx.sizes, weight, kept, None, None, ctx.group_size, need_dx, need_dw, need_db)
-        return dx.view(ctx.x_shape) if need_dx and len(ctx.x_shape) != 2 else dx, dw, db, None
+        return _checkpoint_backward_once(ctx, dy) if torch.is_grad_enabled() else _checkpoint_backward(ctx, dy)
+
+
+def _checkpoint_backward(ctx, dy):
+    kept, weight = ctx.saved_tensors
+    need_dx, need_dw, need_db, _ = ctx.needs_input_grad
+    dx, dw, db = _backward(dy, ctx.sizes, weight, kept, None, None, ctx.group_size, need_dx, need_dw, need_db)
+    return dx.view(ctx.x_shape) if need_dx and len(ctx.x_shape) != 2 else dx, dw, db, None
+
+
+# with create_graph the results refuse to be differentiated; the wrapper is left out where nobody could
+_checkpoint_backward_once = once_differentiable(_checkpoint_backward)
 
 
 class _FusedDequantLinear(torch.autograd.Function):
@@ -134,12 +141,18 @@ class _FusedDequantLinear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        q, scales, zp = ctx.saved_tensors
-        need_dw, need_db = ctx.needs_input_grad[:2]
-        _, dw, db = _backward(dy, ctx.sizes, None, q, scales, zp, ctx.group_size, False, need_dw, need_db)
-        return dw, db, None, None, None, None
+        return _fused_backward_once(ctx, dy) if torch.is_grad_enabled() else _fused_backward(ctx, dy)
+
+
+def _fused_backward(ctx, dy):
+    q, scales, zp = ctx.saved_tensors
+    need_dw, need_db = ctx.needs_input_grad[:2]
+    _, dw, db = _backward(dy, ctx.sizes, None, q, scales, zp, ctx.group_size, False, need_dw, need_db)
+    return dw, db, None, None, None, None
+
+
+_fused_backward_once = once_differentiable(_fused_backward)
 
 
 def int8_checkpoint_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, group_size: int = 32) -> torch.Tensor:
@@ -173,15 +186,15 @@ def fused_dequant_linear(q: torch.Tensor, scales: torch.Tensor, weight: torch.Te
     if q.dim() == 0:
         raise ValueError("q must be [..., K]")
     K = q.shape[-1]
-    q2 = q.reshape(-1, K).contiguous() if K else q.reshape(0, 0)
+    flat = q.dim() == 2      # a view of the result would be one more node of the graph
+    q2 = (q if flat else q.reshape(-1, K) if K else q.reshape(0, 0)).contiguous()
     _check_common(q2, scales, zero_points, K, q2.shape[0], group_size)
     _check_layer(weight, bias, K, q.device)
     for name, t in (("scales", scales), ("zero_points", zero_points)):
         if t is not None and t.device != q.device:
             raise ValueError(f"{name} is on {t.device}, q is on {q.device}")
-    y = _FusedDequantLinear.apply(weight, bias, q2, scales.contiguous().view(-1), None if zero_points is None else zero_points.contiguous().view(-1),
-                                  group_size)
-    return y.view(*q.shape[:-1], weight.shape[0])
+    y = _FusedDequantLinear.apply(weight, bias, q2, scales.contiguous(), None if zero_points is None else zero_points.contiguous(), group_size)
+    return y if flat else y.view(*q.shape[:-1], weight.shape[0])
 
 
 class Int8CheckpointLinear(nn.Module):

@@ -675,11 +675,12 @@ namespace tcb {
 int take_linear_status(int* status) { return take_status(g_status, status); }
 }  // namespace tcb
 
-extern "C" int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K, int backward) {
+extern "C" int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K, int gradients) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    if (!backward) return make_plan(M, N, K, kPairRows).partial_bytes(M);
-    const int64_t dx = make_plan(M, K, N, kPairRows).partial_bytes(M), dw = weight_partial_bytes(M, N, K) + column_bytes(N);
-    return dx > dw ? dx : dw;
+    if (gradients == 0) return make_plan(M, N, K, kPairRows).partial_bytes(M);
+    const int64_t dx = gradients & 1 ? make_plan(M, K, N, kPairRows).partial_bytes(M) : 0;
+    const int64_t rest = (gradients & 2 ? weight_partial_bytes(M, N, K) : 0) + (gradients & 4 ? column_bytes(N) : 0);
+    return dx > rest ? dx : rest;
 }
 
 extern "C" int tcb_linear_forward(const uint16_t* x, const uint16_t* w, const uint16_t* bias_or_null, uint16_t* y, uint8_t* q_or_null,
@@ -720,7 +721,7 @@ extern "C" int tcb_linear_backward(const uint16_t* dy, int64_t ld_dy, const uint
     }
     if (rc == TCB_OK && db_or_null) rc = check_operands(who, dy, dy, db_or_null, nullptr, workspace);
     if (rc != TCB_OK) return rc;
-    const int64_t dw_bytes = weight_partial_bytes(M, N, K);
+    const int64_t dw_bytes = dw_or_null ? weight_partial_bytes(M, N, K) : 0;
     if (db_or_null && workspace_bytes < dw_bytes + column_bytes(N))
         return tcb::fail(TCB_ERR_BAD_ARG, "%s: the workspace holds %lld bytes, %lld are needed", who, (long long)workspace_bytes,
                          (long long)(dw_bytes + column_bytes(N)));

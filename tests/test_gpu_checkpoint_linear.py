@@ -332,6 +332,21 @@ def test_gradients_of_gradients_are_refused():
     (gx,) = torch.autograd.grad(tc.int8_checkpoint_linear(x, w).float().square().sum(), [x], create_graph=True)
     with pytest.raises(RuntimeError):
         gx.float().sum().backward()
+    q, s, _ = tc.quantize_int8_g32(x.detach())
+    (gw,) = torch.autograd.grad(tc.fused_dequant_linear(q.view(8, 32), s, w).float().square().sum(), [w], create_graph=True)
+    with pytest.raises(RuntimeError):
+        gw.float().sum().backward()
+
+
+def test_cached_codes_with_leading_dimensions():
+    x, w, b, dy = layer(24, 40, 64, 2)
+    w.requires_grad_(True), b.requires_grad_(True)
+    q, s, z, _ = tc.compress(x, "fast", 32)
+    want = tc.fused_dequant_linear(q.view(24, 64), s, w, b, zero_points=z)
+    got = tc.fused_dequant_linear(q.view(2, 3, 4, 64), s.view(2, 3, 4, 2), w, b, zero_points=z.view(2, 3, 4, 2))
+    assert torch.equal(got, want.view(2, 3, 4, 40))
+    a, c = torch.autograd.grad(want, [w, b], dy), torch.autograd.grad(got, [w, b], dy.view(2, 3, 4, 40))
+    assert all(torch.equal(u, v) for u, v in zip(a, c))
 
 
 def test_module_trains_in_a_stack():

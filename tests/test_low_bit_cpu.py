@@ -147,8 +147,8 @@ def test_linear_entry_points_refuse_bad_arguments(built_lib):
     assert bwd(p, 8, p, p, p, None, None, p + 2, None, 4, 8, 32, 32, p, 0) == _lib.ERR_ALIGNMENT  # dw
     assert bwd(p, 8, None, p, p, None, p, None, None, 4, 8, 32, 32, p, 0) == _lib.ERR_BAD_ARG    # weight missing
     assert bwd(p, 8, None, None, None, None, None, None, p, 4, 8, 32, 32, p, 4) == _lib.ERR_BAD_ARG  # workspace too small
-    assert L.tcb_linear_workspace(0, 8, 32, 1) == 0 and L.tcb_linear_workspace(4, 8, 32, 0) == 0
-    assert L.tcb_linear_workspace(4, 8, 32, 1) > 0 and L.tcb_linear_workspace(4, 8, 4096, 0) > 0
+    assert L.tcb_linear_workspace(0, 8, 32, 7) == 0 and L.tcb_linear_workspace(4, 8, 32, 0) == 0 and L.tcb_linear_workspace(4, 8, 32, 3) == 0
+    assert L.tcb_linear_workspace(4, 8, 32, 4) > 0 and L.tcb_linear_workspace(100000, 8, 32, 2) > 0 and L.tcb_linear_workspace(4, 8, 4096, 0) > 0
 
 
 def test_linear_layer_refusals():
