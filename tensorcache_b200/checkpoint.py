@@ -66,10 +66,10 @@ def _backward(dy: torch.Tensor, sizes, weight, q, scales, zp, group_size: int, n
             dy = dy.reshape(M, N)
         if N % 8 == 0:
             dy, ld = _operand(dy), N
-        else:       # rows of dy must start on 16-byte boundaries
+        else:       # rows of dy must start on 16-byte boundaries; what lies between them is never used
             ld = -(-N // 8) * 8
-            padded = dy.new_zeros((M, ld))
-            padded[:, :N] = dy
+            padded = dy.new_empty((M, ld))
+            padded.narrow(1, 0, N).copy_(dy)
             dy = padded
         make = dy.new_empty if M and N else dy.new_zeros
         dx = make((M, K)) if need_dx else None

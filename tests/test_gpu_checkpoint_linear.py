@@ -173,6 +173,21 @@ def test_bias_gradient_alone_and_beside_the_weight_gradient(M, N):
         close(got.view(1, -1), torch.ones(1, M, dtype=torch.float64, device=DEV), dy.double())
 
 
+@pytest.mark.parametrize("M,N", [(130, 13), (4097, 101)])
+def test_padding_between_rows_of_dy_is_never_used(M, N):
+    """Rows of an odd number of gradients are copied to rows of a multiple of eight; the memory in between may hold NaN."""
+    x, w, b, dy = layer(M, N, 64, M)
+    x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)
+    y = tc.int8_checkpoint_linear(x, w, b)
+    torch.cuda.synchronize()
+    for size in (M * 16, M * 104, M * 64, 64 * N, 1 << 20, 1 << 22):      # what the pass is about to take from the allocator's cache
+        torch.full((size,), float("nan"), dtype=torch.bfloat16, device=DEV)
+    gx, gw, gb = torch.autograd.grad(y, [x, w, b], dy)
+    close(gx, dy.double(), w.detach().double())
+    close(gw, dy.double().t(), decoded(*plain.int8_encode(x.detach(), 32), 32))
+    close(gb.view(1, -1), torch.ones(1, M, dtype=torch.float64, device=DEV), dy.double())
+
+
 def test_empty_batches_and_layers():
     w, b = (torch.randn(s, device=DEV).to(torch.bfloat16).requires_grad_(True) for s in ((8, 32), (8,)))
     x = torch.empty(0, 32, dtype=torch.bfloat16, device=DEV, requires_grad=True)
