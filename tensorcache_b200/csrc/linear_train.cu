@@ -19,12 +19,12 @@
 // rows are contiguous as two boxes of 64 contraction steps x 64 rows, in the same swizzle: the tensor core reads either
 // (the "major" bits of the instruction descriptor), so nothing is transposed by anyone.
 //
-// Forward and input gradient: tiles of 256 x 256 (each CTA stages 128 rows of A and 128 of B); the two 256-column
-// accumulators alternate between tiles, so a tile's epilogue runs under the next one's products.
+// Forward and input gradient: tiles of 256 x 256 (each CTA stages 128 rows of A and 128 of B), or 256 x 128 for small
+// products; the two accumulators alternate between tiles, so a tile's epilogue runs under the next one's products.
 // Weight gradient: tiles of 512 x 256, both accumulators on one tile.  Decoding 128 rows costs the producers and the
 // shared-memory pipe about as long as one 256 x 256 step of MMAs takes (measured with 256 x 256 tiles: 854 us for 16384
 // x 4096 x 4096, 330 us for the products without decoding); used against 512 rows of A it hides behind two of them.
-// A tile whose second half would lie outside runs one half only.
+// A tile whose second half would lie outside runs one half only, and so do all tiles of a small product.
 // Where the output has too few tiles to fill the GPU the contraction is split: each part leaves fp32 sums in a workspace
 // and a second kernel adds them in a fixed order (results do not depend on timing).
 //
@@ -49,23 +49,23 @@ constexpr uint32_t kMaxSmem = 232448;
 
 enum Source { kContraction, kRows, kCodes };         // how an operand lies in memory (kCodes: rows contiguous, 8-bit codes)
 
-template <Source B>
+template <Source B, int TB>
 struct Config {
+    static_assert(TB == 256 || (TB == 128 && B != kCodes), "columns of a tile");
     static constexpr bool kDeq = B == kCodes;
     static constexpr int kGroups = kDeq ? 2 : 1;             // accumulators per tile = 128-row units of A per CTA
     static constexpr int kBuffers = 2 / kGroups;             // tiles in flight in tensor memory
-    static constexpr int kTileA = kGroups * kPairRows;       // output rows per tile
+    static constexpr int kRowsB = TB / 2;                    // rows of B per CTA
     static constexpr int kEpilogueWarps = 8;                 // per lane quadrant: one per accumulator, or two per tile
-    static constexpr int kChunkStep = 2 / kGroups;           // 32-column chunks between two of a warp
     static constexpr int kFirstProducerWarp = kFirstEpilogueWarp + kEpilogueWarps;
     static constexpr int kThreads = 32 * (kFirstProducerWarp + (kDeq ? kProducerWarps : 0));
-    static constexpr int kStages = kDeq ? 4 : 6;
-    static constexpr uint32_t kBytesA = kGroups * kOperandBytes;
+    static constexpr int kStages = kDeq ? 4 : TB == 256 ? 6 : 8;
+    static constexpr uint32_t kBytesA = kGroups * kOperandBytes, kBytesB = kRowsB * kBlockK * 2;
     // store buffers of the epilogue; the weight gradient's columns are a multiple of 16 and its output aligned: none
     static constexpr uint32_t kStore = kDeq ? 0 : kEpilogueWarps * kStoreStageBytes;
-    static constexpr uint32_t kTiles = kStages * (kBytesA + kOperandBytes + (kDeq ? kCodeBytes : 0)) + kStore;
+    static constexpr uint32_t kTiles = kStages * (kBytesA + kBytesB + (kDeq ? kCodeBytes : 0)) + kStore;
     static constexpr uint32_t kSmem = kTiles + 1024 /* alignment */ + 256 /* barriers */;
-    static_assert(kSmem <= kMaxSmem, "shared memory");
+    static_assert(kSmem <= kMaxSmem && (3 * kStages + 4) * 8 + 8 <= 256, "shared memory");
 };
 
 struct Params {
@@ -81,12 +81,13 @@ struct Params {
     const uint8_t* zp;
     int64_t contraction;
     int tiles_a, tiles_b, tiles;    // tiles = tiles_a * tiles_b
+    int tile_a;                     // output rows per tile: 256, or 512 (weight gradient)
     int num_kb, kb_per_split, items;
 };
 
 struct Item {
-    int ta, tb, split, kb0, kb1;
-    int groups;   // 256-row halves of the tile that hold rows of the output
+    int row_a, tb, split, kb0, kb1;   // first output row of the tile, tile column, part and stages of the contraction
+    int groups;                       // 256-row halves of the tile that hold rows of the output
 };
 
 // Work items: the tiles of split 0, then those of split 1, ...  Tiles run in bands of 8 tile rows, down the band first,
@@ -99,11 +100,11 @@ __device__ __forceinline__ Item decode_item(const Params& p, int item) {
     const int band = t / (8 * p.tiles_b), first = band * 8;
     const int height = p.tiles_a - first < 8 ? p.tiles_a - first : 8;
     const int u = t - first * p.tiles_b;
-    r.ta = first + u % height;
+    r.row_a = (first + u % height) * p.tile_a;
     r.tb = u / height;
     r.kb0 = r.split * p.kb_per_split;
     r.kb1 = r.kb0 + p.kb_per_split < p.num_kb ? r.kb0 + p.kb_per_split : p.num_kb;
-    r.groups = GROUPS == 2 && int64_t(r.ta) * (2 * kPairRows) + kPairRows < p.rows_a ? 2 : 1;
+    r.groups = GROUPS == 2 && p.tile_a > kPairRows && int64_t(r.row_a) + kPairRows < p.rows_a ? 2 : 1;
     return r;
 }
 
@@ -133,14 +134,14 @@ __device__ __forceinline__ void umma_x4(uint32_t d_tmem, uint32_t a_lo, uint32_t
         : "memory");
 }
 
-// One CTA's part of an operand for one stage: rows [row, row + 128), contraction [c, c + 64).
-template <Source S>
+// ROWS rows of an operand for one stage: rows [row, row + ROWS), contraction [c, c + 64).
+template <Source S, int ROWS>
 __device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* map, int row, int c, uint32_t bar) {
     if constexpr (S == kContraction) {
         tma_load_2d_pair(dst, map, c, row, bar);
     } else {
-        tma_load_2d_pair(dst, map, row, c, bar);
-        tma_load_2d_pair(dst + kBoxBytes, map, row + 64, c, bar);
+#pragma unroll
+        for (int i = 0; i < ROWS / 64; ++i) tma_load_2d_pair(dst + i * kBoxBytes, map, row + 64 * i, c, bar);
     }
 }
 
@@ -181,14 +182,14 @@ __device__ __forceinline__ void sum_columns(const uint16_t* __restrict__ x, int6
     }
 }
 
-template <Source A, Source B, int LOG2_G, bool HAS_ZP>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<B>::kThreads, 1)
+template <Source A, Source B, int TB, int LOG2_G, bool HAS_ZP>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<B, TB>::kThreads, 1)
 linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
-    using C = Config<B>;
+    using C = Config<B, TB>;
     constexpr int S = C::kStages;
-    // bf16 x bf16 -> fp32, M = N = 256; bits 15 / 16: rows contiguous
+    // bf16 x bf16 -> fp32, M = 256, N = TB; bits 15 / 16: rows contiguous
     constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((A != kContraction ? 1u : 0u) << 15) |
-                                ((B != kContraction ? 1u : 0u) << 16) | (uint32_t(kPairRows >> 3) << 17) | (uint32_t(kPairRows >> 4) << 24);
+                                ((B != kContraction ? 1u : 0u) << 16) | (uint32_t(TB >> 3) << 17) | (uint32_t(kPairRows >> 4) << 24);
     // 16 of the contraction in the descriptor's 16-byte units: 32 bytes along a row, or 16 rows of 128 bytes
     constexpr uint32_t kStepA = A == kContraction ? 2 : 128, kStepB = B == kContraction ? 2 : 128;
 
@@ -196,7 +197,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* smem_a = smem;
     uint8_t* smem_b = smem_a + S * C::kBytesA;
-    uint8_t* smem_c = smem_b + S * kOperandBytes;
+    uint8_t* smem_c = smem_b + S * C::kBytesB;
     uint8_t* smem_e = smem + C::kTiles - C::kStore;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kTiles);
     // barriers: full (leader), empty, full_c (raw codes), accumulator full [2], accumulator empty [2] (leader)
@@ -248,20 +249,20 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             for (int item = first; ok && item < p.items; item += step) {
                 const Item t = decode_item<C::kGroups>(p, item);
                 const int units = t.groups;   // 128-row units of A per CTA
-                const int row_a = t.ta * C::kTileA + int(rank) * units * kTileRows, row_b = t.tb * kPairRows + int(rank) * kTileRows;
+                const int row_a = t.row_a + int(rank) * units * kTileRows, row_b = t.tb * TB + int(rank) * C::kRowsB;
                 for (int kb = t.kb0; kb < t.kb1; ++kb) {
                     ok = mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag, abort_peer, (1 << 8) | (EMPTY + s));
                     if (!ok) break;
                     const uint32_t full = leader_bar(FULL + s), dst_a = smem_u32(smem_a) + uint32_t(s) * C::kBytesA;
                     for (int u = 0; u < units; ++u)
-                        load_operand<A>(dst_a + uint32_t(u) * kOperandBytes, &map_a, row_a + u * kTileRows, kb * kBlockK, full);
+                        load_operand<A, kTileRows>(dst_a + uint32_t(u) * kOperandBytes, &map_a, row_a + u * kTileRows, kb * kBlockK, full);
                     if constexpr (C::kDeq) {
                         mbar_arrive_expect_tx(bar(FULL_C + s), kCodeBytes);
                         tma_load_2d(smem_u32(smem_c + s * kCodeBytes), &map_b, row_b, kb * kBlockK, bar(FULL_C + s));
                     } else {
-                        load_operand<B>(smem_u32(smem_b + s * kOperandBytes), &map_b, row_b, kb * kBlockK, full);
+                        load_operand<B, C::kRowsB>(smem_u32(smem_b + s * C::kBytesB), &map_b, row_b, kb * kBlockK, full);
                     }
-                    if (leader) mbar_arrive_expect_tx(bar(FULL + s), 2 * (uint32_t(units) + (C::kDeq ? 0 : 1)) * kOperandBytes);
+                    if (leader) mbar_arrive_expect_tx(bar(FULL + s), 2 * (uint32_t(units) * kOperandBytes + (C::kDeq ? 0u : C::kBytesB)));
                     else mbar_arrive_cluster(full);
                     if (++s == S) { s = 0; ph ^= 1; }
                 }
@@ -298,7 +299,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                             for (int h = 0; h < decltype(groups_tag)::value; ++h)
                                 umma_x4<kStepA, kStepB>(tmem + uint32_t((buf + h) * kPairRows),
                                                         a0 + (uint32_t(s) * C::kBytesA + uint32_t(h) * kOperandBytes) / 16,
-                                                        b0 + uint32_t(s) * (kOperandBytes / 16), kIdesc, kb > t.kb0 ? 1u : 0u);
+                                                        b0 + uint32_t(s) * (C::kBytesB / 16), kIdesc, kb > t.kb0 ? 1u : 0u);
                             umma_commit_both(bar(EMPTY + s));
                         }
                         __syncwarp();
@@ -314,9 +315,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     } else if (warp < C::kFirstProducerWarp) {
         // ---------------------------------------------------------------- epilogue
         const int quad = warp & 3;                            // the TMEM lanes this warp may read
-        const int upper = (warp - kFirstEpilogueWarp) >> 2;
-        const int group = C::kGroups == 2 ? upper : 0;        // the accumulator of the tile
-        const int chunk0 = C::kGroups == 2 ? 0 : upper;       // or every second chunk of the only one
+        const int upper = (warp - kFirstEpilogueWarp) >> 2;   // one of the two warps of a lane quadrant
         const StoreMode mode = store_mode(p.out, p.rows_b, p.bias);
         uint32_t* stage = reinterpret_cast<uint32_t*>(smem_e + (C::kStore ? (warp - kFirstEpilogueWarp) * kStoreStageBytes : 0));
         if constexpr (C::kDeq) {
@@ -340,12 +339,14 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                             mbar_wait(bar(TFULL + buf), (local / C::kBuffers) & 1, abort_flag, abort_peer, (4 << 8) | (TFULL + buf)));
             if (!ok) break;
             tc_fence_after();
-            const int64_t row0 = int64_t(t.ta) * C::kTileA + (int64_t(rank) * t.groups + group) * kTileRows + quad * 32;
+            // two accumulators: one each; one: every second chunk of its columns
+            const int group = C::kGroups == 2 && t.groups == 2 ? upper : 0, chunk0 = upper - group, step_c = t.groups == 2 ? 1 : 2;
+            const int64_t row0 = int64_t(t.row_a) + (int64_t(rank) * t.groups + group) * kTileRows + quad * 32;
             const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + uint32_t((buf + group) * kPairRows);
 #pragma unroll 1
-            for (int c = chunk0; c < kPairRows / 32; c += C::kChunkStep) {
-                const int64_t col0 = int64_t(t.tb) * kPairRows + c * 32;
-                if (col0 >= p.rows_b || group >= t.groups) break;   // warp-uniform
+            for (int c = chunk0; c < TB / 32; c += step_c) {
+                const int64_t col0 = int64_t(t.tb) * TB + c * 32;
+                if (col0 >= p.rows_b) break;   // warp-uniform
                 if (p.partial) {
                     store_32x32_f32(taddr + uint32_t(c * 32), p.partial + int64_t(t.split) * p.rows_a * p.ld_partial, p.ld_partial, row0, p.rows_a, col0);
                     continue;
@@ -378,7 +379,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             pf_end = t.kb1;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int64_t k = int64_t(t.tb) * kPairRows + int64_t(rank) * kTileRows + 16 * kq + 64 * (h0 ^ i);
+                const int64_t k = int64_t(t.tb) * TB + int64_t(rank) * C::kRowsB + 16 * kq + 64 * (h0 ^ i);
                 g[i] = k < p.rows_b ? (int64_t(pf_kb) * kBlockK + r) * gpr + (k >> LOG2_G) : INT64_MIN;
             }
         };
@@ -418,7 +419,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 if (!ok) break;
                 const uint8_t* c = smem_c + s * kCodeBytes + r * 128 + kq * 16;
                 const uint4 c0 = *reinterpret_cast<const uint4*>(c + 64 * h0), c1 = *reinterpret_cast<const uint4*>(c + 64 * (h0 ^ 1));
-                uint8_t* d = smem_b + s * kOperandBytes + r * 128;
+                uint8_t* d = smem_b + s * C::kBytesB + r * 128;
                 uint8_t *d0 = d + h0 * kBoxBytes, *d1 = d + (h0 ^ 1) * kBoxBytes;
                 convert16<HAS_ZP>(c0, sz0, d0 + piece0, d0 + piece1);
                 convert16<HAS_ZP>(c1, sz1, d1 + piece0, d1 + piece1);
@@ -504,36 +505,53 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __rest
 // ------------------------------------------------------------------------ host
 
 struct Plan {
+    int tile_a = kPairRows, tile_b = 256;
     int64_t tiles_a = 0, tiles_b = 0, num_kb = 0;
     int splits = 1, kb_per_split = 0;
     int64_t ld_partial = 0;
     int64_t partial_bytes(int64_t rows_a) const { return splits > 1 ? int64_t(splits) * rows_a * ld_partial * 4 : 0; }
 };
 
-// Splits the contraction where tiles leave pairs of CTAs idle and a shorter sum saves more than the second kernel costs.
-// A stage of a 256 x 256 (512 x 256) tile takes 0.27 (0.55) us, the second kernel 4 us and the partial sums' way through
-// memory at about 5 TB/s.  Measured on 1024 x 1024 x 1024 (forward): 12.4 us in two parts, 10.0 in one.
-Plan make_plan(int64_t rows_a, int64_t rows_b, int64_t contraction, int tile_a) {
-    Plan p;
-    p.tiles_a = (rows_a + tile_a - 1) / tile_a;
-    p.tiles_b = (rows_b + kPairRows - 1) / kPairRows;
-    p.num_kb = (contraction + kBlockK - 1) / kBlockK;
-    p.ld_partial = (rows_b + 7) / 8 * 8;
-    const int64_t pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1, most = pairs / (p.tiles_a * p.tiles_b);
-    const double stage = tile_a > kPairRows ? 0.55 : 0.27, part = double(rows_a) * double(p.ld_partial) * 8.0 / 5e6;
-    double best = double(p.num_kb) * stage;
-    int64_t splits = 1;
-    for (int64_t s = 2; s <= most && s <= p.num_kb; ++s) {
-        const double t = double((p.num_kb + s - 1) / s) * stage + 4.0 + double(s) * part;
-        if (t < best) best = t, splits = s;
+// Tiles and split of a product (codes: the weight gradient), by the estimated time in us of the longest pair of CTAs:
+//     stages x time of a stage + end of a tile + (split: 4 for the second kernel and the partial sums' way through memory at 5 TB/s)
+// A stage takes 0.27 (256 x 256), 0.25 (256 x 128; it saves little once many pairs load), 0.74 (512 x 256 from codes) or 0.7 (256 x 256 from
+// codes: the producers are what it waits for).  Results leave an SM at 26 bytes a clock, plus 1 us until the last have arrived.  Halved
+// tiles come into question where all of them run at once.  Measured, us, halved or not / whole tiles: 446 x 768 x 768 forward 6.7 / 8.5,
+// weight gradient 8.6 / 11.9; 1 x 4096 x 4096 forward in two halved parts 17.9, in four whole ones 12.7; step on 57,088 x 768 codes
+// for 1000 outputs with a halved weight gradient 224, a whole one 202; 1024 x 1024 x 1024 forward split in two 12.4, not split 10.0.
+Plan make_plan(int64_t rows_a, int64_t rows_b, int64_t contraction, bool codes) {
+    const int64_t pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1, num_kb = (contraction + kBlockK - 1) / kBlockK;
+    const int64_t ld_partial = (rows_b + 7) / 8 * 8;
+    const double part = double(rows_a) * double(ld_partial) * 8.0 / 5e6;
+    Plan best;
+    double best_time = 0.0;
+    for (int halved = 0; halved < 2; ++halved) {
+        Plan p;
+        p.tile_a = codes && !halved ? 512 : 256;
+        p.tile_b = !codes && halved ? 128 : 256;
+        p.tiles_a = (rows_a + p.tile_a - 1) / p.tile_a;
+        p.tiles_b = (rows_b + p.tile_b - 1) / p.tile_b;
+        p.num_kb = num_kb;
+        p.ld_partial = ld_partial;
+        const int64_t tiles = p.tiles_a * p.tiles_b;
+        if (halved && tiles > pairs) break;
+        const double stage = codes ? (halved ? 0.7 : 0.74) : (halved ? 0.25 : 0.27);
+        const double store = double(p.tile_a / 2) * p.tile_b / 49400.0;   // us per byte of a result
+        for (int64_t s = 1; s == 1 || (s <= pairs / tiles && s <= num_kb); ++s) {
+            const double t = double((num_kb + s - 1) / s) * stage + 1.0 + store * (s > 1 ? 4.0 : 2.0) + (s > 1 ? 4.0 + double(s) * part : 0.0);
+            if ((halved == 0 && s == 1) || t < best_time) {
+                best_time = t;
+                best = p;
+                best.kb_per_split = int((num_kb + s - 1) / s);
+                best.splits = int((num_kb + best.kb_per_split - 1) / best.kb_per_split);
+            }
+        }
     }
-    p.kb_per_split = int((p.num_kb + splits - 1) / splits);
-    p.splits = int((p.num_kb + p.kb_per_split - 1) / p.kb_per_split);
-    return p;
+    return best;
 }
 
 int64_t weight_partial_bytes(int64_t M, int64_t N, int64_t K) {
-    return (make_plan(N, K, M, Config<kCodes>::kTileA).partial_bytes(N) + 31) / 32 * 32;
+    return (make_plan(N, K, M, true).partial_bytes(N) + 31) / 32 * 32;
 }
 
 // Parts of the column sums: at most one per CTA (a GPU has no more than one CTA per SM of these kernels) and row slice.
@@ -590,33 +608,43 @@ struct Operand {
     int64_t rows, contraction, ld;
 };
 
+// `rows`: rows of the operand a CTA stages.
 template <Source S>
-int operand_map(const char* who, CUtensorMap* map, const Operand& o) {
-    if (S == kContraction) return encode_map(who, map, false, o.base, o.contraction, o.rows, o.ld, kBlockK, kTileRows);
+int operand_map(const char* who, CUtensorMap* map, const Operand& o, int rows) {
+    if (S == kContraction) return encode_map(who, map, false, o.base, o.contraction, o.rows, o.ld, kBlockK, rows);
     if (S == kRows) return encode_map(who, map, false, o.base, o.rows, o.contraction, o.ld, 64, kBlockK);
-    return encode_map(who, map, true, o.base, o.rows, o.contraction, o.ld, kTileRows, kBlockK);
+    return encode_map(who, map, true, o.base, o.rows, o.contraction, o.ld, rows, kBlockK);
+}
+
+template <Source A, Source B, int TB, int LOG2_G, bool HAS_ZP>
+int launch_tiles(const char* who, const Operand& a, const Operand& b, Params& p, cudaStream_t st, int* grid) {
+    using C = Config<B, TB>;
+    CUtensorMap map_a, map_b;
+    int rc = operand_map<A>(who, &map_a, a, kTileRows);
+    if (rc == TCB_OK) rc = operand_map<B>(who, &map_b, b, C::kRowsB);
+    if (rc != TCB_OK) return rc;
+    const auto kernel = linear_kernel<A, B, TB, LOG2_G, HAS_ZP>;
+    static std::atomic<bool> attr_set[64] = {};
+    int dev = 0;
+    TCB_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
+        TCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(C::kSmem)));
+        if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
+    }
+    const int pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1;
+    *grid = 2 * (p.items < pairs ? p.items : pairs);
+    TCB_CUDA_TRY(tcb::launch_overlapped(+kernel, dim3(*grid), dim3(C::kThreads), C::kSmem, st, map_a, map_b, p));
+    return TCB_OK;
 }
 
 template <Source A, Source B, int LOG2_G, bool HAS_ZP>
 int launch(const char* who, const Operand& a, const Operand& b, const uint16_t* scales, const uint8_t* zp, const uint16_t* bias, uint16_t* out,
            void* workspace, int64_t workspace_bytes, cudaStream_t st, const Columns& columns = Columns()) {
-    const Plan plan = make_plan(a.rows, b.rows, a.contraction, Config<B>::kTileA);
+    const Plan plan = make_plan(a.rows, b.rows, a.contraction, B == kCodes);
     if (plan.tiles_a * plan.tiles_b * plan.splits > (int64_t(1) << 30)) return tcb::fail(TCB_ERR_TOO_LARGE, "%s: too many output tiles", who);
     if (plan.partial_bytes(a.rows) > workspace_bytes)
         return tcb::fail(TCB_ERR_BAD_ARG, "%s: the workspace holds %lld bytes, %lld are needed", who, (long long)workspace_bytes,
                          (long long)plan.partial_bytes(a.rows));
-    CUtensorMap map_a, map_b;
-    int rc = operand_map<A>(who, &map_a, a);
-    if (rc == TCB_OK) rc = operand_map<B>(who, &map_b, b);
-    if (rc != TCB_OK) return rc;
-    const auto kernel = linear_kernel<A, B, LOG2_G, HAS_ZP>;
-    static std::atomic<bool> attr_set[64] = {};
-    int dev = 0;
-    TCB_CUDA_TRY(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
-        TCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Config<B>::kSmem)));
-        if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
-    }
     Params p;
     p.rows_a = a.rows;
     p.rows_b = b.rows;
@@ -633,12 +661,18 @@ int launch(const char* who, const Operand& a, const Operand& b, const uint16_t* 
     p.tiles_a = int(plan.tiles_a);
     p.tiles_b = int(plan.tiles_b);
     p.tiles = p.tiles_a * p.tiles_b;
+    p.tile_a = plan.tile_a;
     p.num_kb = int(plan.num_kb);
     p.kb_per_split = plan.kb_per_split;
     p.items = p.tiles * plan.splits;
-    const int pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1;
-    const int grid = 2 * (p.items < pairs ? p.items : pairs);
-    TCB_CUDA_TRY(tcb::launch_overlapped(+kernel, dim3(grid), dim3(Config<B>::kThreads), Config<B>::kSmem, st, map_a, map_b, p));
+    int rc = TCB_OK, grid = 0;
+    if constexpr (B == kCodes) {
+        rc = launch_tiles<A, B, 256, LOG2_G, HAS_ZP>(who, a, b, p, st, &grid);
+    } else {
+        rc = plan.tile_b == 128 ? launch_tiles<A, B, 128, LOG2_G, HAS_ZP>(who, a, b, p, st, &grid)
+                                : launch_tiles<A, B, 256, LOG2_G, HAS_ZP>(who, a, b, p, st, &grid);
+    }
+    if (rc != TCB_OK) return rc;
     return launch_add(plan, p.partial, a.rows, b.rows, bias, out, columns, grid * ColumnShare(a.rows).slices, a.rows, st);
 }
 
@@ -677,8 +711,8 @@ int take_linear_status(int* status) { return take_status(g_status, status); }
 
 extern "C" int64_t tcb_linear_workspace(int64_t M, int64_t N, int64_t K, int gradients) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    if (gradients == 0) return make_plan(M, N, K, kPairRows).partial_bytes(M);
-    const int64_t dx = gradients & 1 ? make_plan(M, K, N, kPairRows).partial_bytes(M) : 0;
+    if (gradients == 0) return make_plan(M, N, K, false).partial_bytes(M);
+    const int64_t dx = gradients & 1 ? make_plan(M, K, N, false).partial_bytes(M) : 0;
     const int64_t rest = (gradients & 2 ? weight_partial_bytes(M, N, K) : 0) + (gradients & 4 ? column_bytes(N) : 0);
     return dx > rest ? dx : rest;
 }
