@@ -15,8 +15,12 @@
 // columns) behind.  The accumulators alternate between tiles and share columns [208, 256): the epilogue reads those
 // first and hands them over, so the next tile starts while most of the previous one is still being stored.
 //
+// Small products run on tiles of 256 x 128 instead: eight stages of 26 KB, two accumulators side by side.
+//
 // Warps per CTA: 0 TMA, 1 MMA issue (leader CTA) and tensor memory, 2-9 epilogue (two per lane quadrant).
 // Waits are bounded as in the fused dequantising product; the status word is read by tcb_fused_dequant_linear_check().
+#include <type_traits>
+
 #include "tcb_tcgen05.h"
 
 namespace tcb {
@@ -29,16 +33,24 @@ namespace {
 
 constexpr int kTileRows = 128, kPairRows = 256;
 constexpr int kBlockK = 256;                       // values of K per stage
-constexpr int kStages = 6;
-constexpr uint32_t kOperandBytes = 128 * 128;      // 16 KB of codes: one operand, one CTA, one stage
+constexpr uint32_t kOperandBytes = 128 * 128;      // 16 KB: codes of x, one CTA, one stage
 constexpr uint32_t kScaleBytesA = 1024;            // 128 rows x 8 blocks
-constexpr uint32_t kScaleBytesB = 2048;            // 256 rows x 8 blocks
-constexpr uint32_t kStageBytes = 2 * kOperandBytes + kScaleBytesA + kScaleBytesB;
 constexpr int kEpilogueWarps = 8, kFirstEpilogueWarp = 2;
 constexpr int kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);
-constexpr uint32_t kSmemTiles = kStages * kStageBytes + kEpilogueWarps * kStoreStageBytes;
-constexpr uint32_t kSmem = kSmemTiles + 1024 /* alignment */ + 256 /* barriers */;
-constexpr uint32_t kAcc1 = 208, kScaleCols = 464;  // tensor-memory columns
+constexpr uint32_t kScaleCols = 464;               // first tensor-memory column of the scales
+
+// TB: columns of a tile (rows of w).
+template <int TB>
+struct Config {
+    static constexpr int kStages = TB == 256 ? 6 : 8;
+    static constexpr uint32_t kBytesB = TB / 2 * 128, kScaleBytesB = TB * 8;
+    static constexpr uint32_t kStageBytes = kOperandBytes + kBytesB + kScaleBytesA + kScaleBytesB;
+    static constexpr uint32_t kSmemTiles = kStages * kStageBytes + kEpilogueWarps * kStoreStageBytes;
+    static constexpr uint32_t kSmem = kSmemTiles + 1024 /* alignment */ + 256 /* barriers */;
+    static constexpr uint32_t kAcc1 = TB == 256 ? 208 : 128;   // second accumulator
+    static constexpr uint32_t kColsB = TB / 32;                // columns of w's scales per 128 of K
+    static_assert(kSmem <= 232448 && (2 * kStages + 3) * 8 + 8 <= 256 && kStageBytes % 1024 == 0, "shared memory");
+};
 
 struct Params {
     int64_t M, N;
@@ -47,13 +59,15 @@ struct Params {
     int tiles_m, tiles_n, tiles, num_kb;
 };
 
-// x, w: E2M1; scales: E8M0; M = N = 256; K = 64.  sf: which half of a 32-bit word of scales (0 or 2).
+// x, w: E2M1; scales: E8M0; M = 256, N = TB; K = 64.  sf: which half of a 32-bit word of scales (0 or 2).
+template <int TB>
 __device__ __forceinline__ constexpr uint32_t inst_desc(uint32_t sf) {
-    return (sf << 4) | (1u << 7) | (1u << 10) | (uint32_t(kPairRows >> 3) << 17) | (1u << 23) | (uint32_t(kPairRows >> 7) << 27) | (sf << 29);
+    return (sf << 4) | (1u << 7) | (1u << 10) | (uint32_t(TB >> 3) << 17) | (1u << 23) | (uint32_t(kPairRows >> 7) << 27) | (sf << 29);
 }
 
-// The four MMAs of a stage (64 of K = 32 bytes of codes each); the scales of MMAs 2 and 3 sit four (x) and eight (w)
+// The four MMAs of a stage (64 of K = 32 bytes of codes each); the scales of MMAs 2 and 3 sit four (x) and TB / 32 (w)
 // columns after those of 0 and 1, within a column the odd ones use the upper half.
+template <int TB>
 __device__ __forceinline__ void umma_mxf4_x4(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t sfa, uint32_t sfb, uint32_t accumulate_first) {
     asm volatile(
         "{\n\t.reg .pred p, t;\n\t.reg .b64 a, b;\n\t.reg .b32 al, bl, sa, sb;\n\t"
@@ -64,11 +78,11 @@ __device__ __forceinline__ void umma_mxf4_x4(uint32_t d_tmem, uint32_t a_lo, uin
         "add.u32 al, %1, 2;\n\tadd.u32 bl, %2, 2;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
         "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %5, [%6], [%7], t;\n\t"
         "add.u32 al, %1, 4;\n\tadd.u32 bl, %2, 4;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
-        "add.u32 sa, %6, 4;\n\tadd.u32 sb, %7, 8;\n\t"
+        "add.u32 sa, %6, 4;\n\tadd.u32 sb, %7, %9;\n\t"
         "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [sa], [sb], t;\n\t"
         "add.u32 al, %1, 6;\n\tadd.u32 bl, %2, 6;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
         "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %5, [sa], [sb], t;\n\t}" ::"r"(d_tmem),
-        "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(inst_desc(0)), "r"(inst_desc(2)), "r"(sfa), "r"(sfb), "r"(accumulate_first)
+        "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(inst_desc<TB>(0)), "r"(inst_desc<TB>(2)), "r"(sfa), "r"(sfb), "r"(accumulate_first), "n"(TB / 32)
         : "memory");
 }
 
@@ -94,14 +108,17 @@ __device__ __forceinline__ Tile decode_tile(const Params& p, int t) {
     return {first + u % height, u / height};
 }
 
+template <int TB>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                     const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_ws, const Params p) {
-    constexpr int S = kStages;
+    using C = Config<TB>;
+    constexpr int S = C::kStages;
+    constexpr uint32_t kStageBytes = C::kStageBytes;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     // stages (codes of x, codes of w, scales of x, scales of w, 1024-byte aligned each), store buffers, barriers
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemTiles);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kSmemTiles);
     // barriers: full (leader), empty, accumulator full [2], shared columns free (leader)
     constexpr int FULL = 0, EMPTY = S, TFULL = 2 * S, TFREE = 2 * S + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 3);
@@ -155,9 +172,9 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                     if (!ok) break;
                     const uint32_t full = leader_bar(FULL + s), dst = smem0 + uint32_t(s) * kStageBytes;
                     tma_load_2d_pair(dst, &map_x, kb * 128, t.m * kPairRows + int(rank) * kTileRows, full);
-                    tma_load_2d_pair(dst + kOperandBytes, &map_w, kb * 128, t.n * kPairRows + int(rank) * kTileRows, full);
-                    tma_load_2d_pair(dst + 2 * kOperandBytes, &map_xs, kb * 128, t.m * 2 + int(rank), full);
-                    tma_load_2d_pair(dst + 2 * kOperandBytes + kScaleBytesA, &map_ws, kb * 128, t.n * 2, full);
+                    tma_load_2d_pair(dst + kOperandBytes, &map_w, kb * 128, t.n * TB + int(rank) * (TB / 2), full);
+                    tma_load_2d_pair(dst + kOperandBytes + C::kBytesB, &map_xs, kb * 128, t.m * 2 + int(rank), full);
+                    tma_load_2d_pair(dst + kOperandBytes + C::kBytesB + kScaleBytesA, &map_ws, kb * 128, t.n * (TB / 128), full);
                     if (leader) mbar_arrive_expect_tx(bar(FULL + s), 2 * kStageBytes);
                     else mbar_arrive_cluster(full);
                     if (++s == S) { s = 0; ph ^= 1; }
@@ -181,22 +198,23 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                 ok = __all_sync(0xffffffffu, mbar_wait(bar(TFREE), (local & 1) ^ 1, abort_flag, abort_peer, (2 << 8) | TFREE));
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t d = tmem + ((local & 1) ? kAcc1 : 0u);
+                const uint32_t d = tmem + ((local & 1) ? C::kAcc1 : 0u);
                 for (int kb = 0; kb < p.num_kb; ++kb) {
                     ok = __all_sync(0xffffffffu, mbar_wait(bar(FULL + s), ph, abort_flag, abort_peer, (2 << 8) | (FULL + s)));
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t src = smem0 + uint32_t(s) * kStageBytes;
-                    const uint32_t sa = src + 2 * kOperandBytes, sb = sa + kScaleBytesA;
-                    const uint32_t ta = tmem + kScaleCols + 24u * set, tb = ta + 8u;
+                    const uint32_t sa = src + kOperandBytes + C::kBytesB, sb = sa + kScaleBytesA;
+                    const uint32_t ta = tmem + kScaleCols + (8u + 2 * C::kColsB) * set, tb = ta + 8u;
                     if (elected) {
 #pragma unroll
                         for (uint32_t c = 0; c < 2; ++c) {   // 128 of K: four scales a row
                             copy_scales(ta + 4 * c, sa + 512 * c);
-                            copy_scales(tb + 8 * c, sb + 512 * c);               // rows 0..127 of the tile of w
-                            copy_scales(tb + 8 * c + 4, sb + 1024 + 512 * c);    // rows 128..255
+#pragma unroll
+                            for (uint32_t j = 0; j < TB / 128; ++j)   // 128 rows of w
+                                copy_scales(tb + C::kColsB * c + 4 * j, sb + 1024 * j + 512 * c);
                         }
-                        umma_mxf4_x4(d, smem_desc_lo(src), smem_desc_lo(src + kOperandBytes), ta, tb, kb > 0 ? 1u : 0u);
+                        umma_mxf4_x4<TB>(d, smem_desc_lo(src), smem_desc_lo(src + kOperandBytes), ta, tb, kb > 0 ? 1u : 0u);
                         umma_commit_both(bar(EMPTY + s));
                     }
                     __syncwarp();
@@ -221,12 +239,12 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             if (!ok) break;
             tc_fence_after();
             const int64_t row0 = int64_t(t.m) * kPairRows + int64_t(rank) * kTileRows + quad * 32;
-            const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + (buf ? kAcc1 : 0u);
+            const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + (buf ? C::kAcc1 : 0u);
 #pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < TB / 64; ++i) {
                 // chunks of 32 columns; the two of shared columns come first (the last two of accumulator 0, the first two of 1)
-                const int c = buf ? 2 * i + half : 7 - 2 * i - half;
-                const int64_t col0 = int64_t(t.n) * kPairRows + c * 32;
+                const int c = buf ? 2 * i + half : TB / 32 - 1 - 2 * i - half;
+                const int64_t col0 = int64_t(t.n) * TB + c * 32;
                 uint32_t v[32];
                 tmem_ld32(taddr + uint32_t(c * 32), v);
                 tmem_ld_wait();
@@ -255,15 +273,15 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 int64_t scale_bytes(int64_t rows, int64_t K) { return (rows + 127) / 128 * ((K + 127) / 128) * 512; }
 int64_t code_bytes(int64_t rows, int64_t K) { return (rows * (K / 2) + 511) / 512 * 512; }
 
-// Codes: rows of K / 2 bytes in boxes of 128 rows x 128 bytes.  Scales: one row of the map per 128 rows of the operand,
+// Codes: rows of K / 2 bytes in boxes of `code_rows` rows x 128 bytes.  Scales: one row of the map per 128 rows of the operand,
 // in 8-byte elements, boxes of `box_rows` x 1024 bytes.  What lies outside is read as 0.
 int encode_maps(const char* who, CUtensorMap* codes_map, CUtensorMap* scales_map, const uint8_t* codes, const uint8_t* scales, int64_t rows,
-                int64_t K, int box_rows) {
+                int64_t K, int code_rows, int box_rows) {
     EncodeTiledFn encode = encode_tiled_fn();
     if (!encode) return tcb::fail(TCB_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available from the driver", who);
     const cuuint32_t estr[2] = {1, 1};
     const cuuint64_t cdims[2] = {cuuint64_t(K / 2), cuuint64_t(rows)}, cstride[1] = {cuuint64_t(K / 2)};
-    const cuuint32_t cbox[2] = {128, kTileRows};
+    const cuuint32_t cbox[2] = {128, cuuint32_t(code_rows)};
     CUresult cr = encode(codes_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), cdims, cstride, cbox, estr,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -310,33 +328,40 @@ extern "C" int tcb_mxfp4_linear(const void* x, int dtype, const uint8_t* wq, con
         return tcb::fail(TCB_ERR_BAD_ARG, "%s: the workspace is too small or not 16-byte aligned", who);
     CUtensorMap map_x, map_w, map_xs, map_ws;
     if (need == 0) {   // few rows: w in boxes of 128 rows, x quantised by the product itself
-        const int few = encode_maps(who, &map_w, &map_ws, wq, w_scales, N, K, 1);
+        const int few = encode_maps(who, &map_w, &map_ws, wq, w_scales, N, K, kTileRows, 1);
         return few != TCB_OK ? few : tcb::launch_mxfp4_few_rows(who, x, dtype, map_w, map_ws, bias_or_null, out, M, N, K, static_cast<cudaStream_t>(stream));
     }
     uint8_t* xq = static_cast<uint8_t*>(workspace);
     uint8_t* xs = xq + code_bytes(M, K);
     int rc = tcb_quantize_mxfp4(x, dtype, M, K, xq, xs, stream);
-    if (rc == TCB_OK) rc = encode_maps(who, &map_x, &map_xs, xq, xs, M, K, 1);
-    if (rc == TCB_OK) rc = encode_maps(who, &map_w, &map_ws, wq, w_scales, N, K, 2);
+    if (rc == TCB_OK) rc = encode_maps(who, &map_x, &map_xs, xq, xs, M, K, kTileRows, 1);
     if (rc != TCB_OK) return rc;
-    static std::atomic<bool> attr_set[64] = {};
-    int dev = 0;
-    TCB_CUDA_TRY(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
-        TCB_CUDA_TRY(cudaFuncSetAttribute(mxfp4_linear_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem)));
-        if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
-    }
+    // Tiles of 256 x 128 where all of them run at once: half the products and half the results to store per SM (us with the
+    // quantisation, halved / whole tiles: 446 x 1001 x 768 8.3 / 11.0, 64 x 4096 x 4096 9.8 / 10.9, 1024 x 1024 x 1024 7.6 / 8.5).
+    const int pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1;
     Params p;
     p.M = M;
     p.N = N;
     p.bias = bias_or_null;
     p.out = out;
     p.tiles_m = int(tiles_m);
-    p.tiles_n = int(tiles_n);
-    p.tiles = p.tiles_m * p.tiles_n;
     p.num_kb = int((K + kBlockK - 1) / kBlockK);
-    const int pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1;
-    const cudaError_t e = tcb::launch_overlapped(mxfp4_linear_kernel, dim3(2 * (p.tiles < pairs ? p.tiles : pairs)), dim3(kThreads), kSmem,
-                                                 static_cast<cudaStream_t>(stream), map_x, map_w, map_xs, map_ws, p);
-    return e == cudaSuccess ? TCB_OK : tcb::cuda_fail(e, who);
+    const auto run = [&](auto tag) {
+        constexpr int TB = decltype(tag)::value;
+        p.tiles_n = int((N + TB - 1) / TB);
+        p.tiles = p.tiles_m * p.tiles_n;
+        const int status = encode_maps(who, &map_w, &map_ws, wq, w_scales, N, K, TB / 2, TB / 128);
+        if (status != TCB_OK) return status;
+        static std::atomic<bool> attr_set[64] = {};
+        int dev = 0;
+        TCB_CUDA_TRY(cudaGetDevice(&dev));
+        if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
+            TCB_CUDA_TRY(cudaFuncSetAttribute(mxfp4_linear_kernel<TB>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Config<TB>::kSmem)));
+            if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
+        }
+        TCB_CUDA_TRY(tcb::launch_overlapped(mxfp4_linear_kernel<TB>, dim3(2 * (p.tiles < pairs ? p.tiles : pairs)), dim3(kThreads), Config<TB>::kSmem,
+                                            static_cast<cudaStream_t>(stream), map_x, map_w, map_xs, map_ws, p));
+        return int(TCB_OK);
+    };
+    return tiles_m * ((N + 127) / 128) <= pairs ? run(std::integral_constant<int, 128>()) : run(std::integral_constant<int, 256>());
 }
