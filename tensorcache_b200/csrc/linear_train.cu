@@ -431,7 +431,6 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     }
 
     // Neither CTA leaves while the other may still arrive on its barriers or read its shared memory.
-    __syncwarp();
     tc_fence_before();
     cluster_sync_all();
     if (warp == 1) {

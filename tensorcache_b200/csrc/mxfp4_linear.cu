@@ -259,7 +259,6 @@ mxfp4_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     }
 
     // Neither CTA leaves while the other may still arrive on its barriers or read its shared memory.
-    __syncwarp();
     tc_fence_before();
     cluster_sync_all();
     if (warp == 1) {

@@ -23,7 +23,10 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// Called by whole warps; their lanes meet first: an .aligned instruction must be reached by all of them together, and what comes
+// before it (one lane's set-up, loops whose length differs from lane to lane) may have parted them.
 __device__ __forceinline__ void cluster_sync_all() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
@@ -127,7 +130,9 @@ __device__ __forceinline__ bool elect_one() {
 // Index of this warp in the block, as a value the compiler knows to be the same in all lanes.
 __device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0); }
 
+// The lanes meet first, as above: the stores of the columns before leave out lanes whose rows lie outside the output.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    __syncwarp();
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"

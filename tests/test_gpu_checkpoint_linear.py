@@ -395,3 +395,25 @@ def test_device_cache_feeds_a_head():
     rows = cache.read(pick).double()
     close(y.detach(), rows, w.detach().double().t())
     close(dw, dy.double().t(), rows)
+
+
+@pytest.mark.parametrize("M", [1, 31, 33, 97, 161, 255])
+@pytest.mark.parametrize("N", [261, 264, 272])
+def test_last_rows_that_end_inside_a_warp(M, N):
+    """Lanes whose rows lie outside the output skip the stores of a piece (staged, 16-byte and 32-byte ones); the warp has
+    more pieces to read from tensor memory after it, in every product and in the parts of a split sum."""
+    K = 512 + 16
+    x, w, b, dy = layer(M, N, K, M + N)
+    x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)
+    y = tc.int8_checkpoint_linear(x, w, b, group_size=16)
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+    q, s = plain.int8_encode(x.detach(), 16)
+    fused = tc.fused_dequant_linear(q.to(torch.int8), s, w, b, group_size=16)
+    as_weight = tc.fused_dequant_matmul(w.detach(), q.to(torch.int8), s, group_size=16)
+    check_device_status()
+    X, W, D, Q = x.detach().double(), w.detach().double(), dy.double(), decoded(q, s, 16)
+    close(y.detach(), X, W.t(), b.detach().double())
+    close(dx, D, W)
+    close(dw, D.t(), Q)
+    close(fused.detach(), Q, W.t(), b.detach().double())
+    close(as_weight, W, Q.t())

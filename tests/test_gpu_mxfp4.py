@@ -181,6 +181,17 @@ def test_product_of_few_rows(M, N, K):
     product_close(y, plain.mx_values(*plain.mx_encode(x)), plain.mx_values(*plain.mx_encode(w)), b)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 1, 4096), (3, 127, 8192), (16, 385, 4096), (17, 250, 4096), (33, 261, 96), (97, 264, 96), (161, 272, 96),
+                                   (600, 10007, 64)])
+def test_product_whose_last_rows_and_columns_end_inside_a_warp(M, N, K):
+    """Lanes outside the output leave the loop over the parts of a split sum, or the stores of a piece, before the others."""
+    x, w, b = product_inputs(M, N, K, seed=M + N)
+    wq, ws, _ = tc.quantize_mxfp4(w)
+    y = tc.mxfp4_matmul(x, wq, ws, bias=b)
+    check_device_status()
+    product_close(y, plain.mx_values(*plain.mx_encode(x)), plain.mx_values(*plain.mx_encode(w)), b)
+
+
 def test_scales_that_pad_a_row_do_not_reach_the_sums():
     """K = 32 in a tile of 128: the other three scales of a row are padding."""
     for M in (3, 40):
