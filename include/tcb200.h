@@ -224,7 +224,9 @@ TCB_API int tcb_cache_read(const int8_t* codes, const uint16_t* scales, int64_t 
  * Fused dequantise + GEMM on the tcgen05 tensor cores:
  *     out[m, n] = bf16( sum_k dense[m, k] * deq(q)[n, k]  + bias )
  * with deq(q)[n, k] = (q[n, k] - zp[n, k / G]) * scale[n, k / G]   (zp != NULL, uint8 codes)
- *                or    int8(q[n, k])           * scale[n, k / G]   (zp == NULL, signed codes).
+ *                or    int8(q[n, k])           * scale[n, k / G]   (zp == NULL, signed codes),
+ * rounded to bf16; a value past the largest bf16 number counts as that number (the decoding
+ * functions give infinity), and an infinite scale as NaN.
  * Replaces FusedDequantLinear.forward / _fused_dequant_matmul_kernel
  * (src/tensorcache/fused_ops.py:1338-1461).
  *   dense  [R_d, K] bf16, K contiguous        q  [R_q, K] codes, K contiguous
@@ -252,7 +254,8 @@ TCB_API int tcb_fused_dequant_linear(const uint16_t* dense, const uint8_t* q, co
  *             dw [N, K] = dy [M, N]^T . deq(q) [M, K]          if dw is given (needs q, scales)
  *             db [N]    = column sums of dy                    if db is given
  * deq(q) is the bf16 number tcb_decompress_amo / tcb_decompress_sym gives for the codes
- * (zp != NULL: uint8 codes, else signed).  All other arrays are bf16.
+ * (zp != NULL: uint8 codes, else signed), or the largest bf16 number where that is infinite.
+ * All other arrays are bf16.
  *   ld_dy      elements between rows of dy: a multiple of 8, at least N
  *   workspace  tcb_linear_workspace(M, N, K, gradients) bytes on the current device (NULL where
  *              that is 0), 32-byte aligned, used by the call's own work only; gradients: 0 for

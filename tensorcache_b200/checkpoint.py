@@ -160,7 +160,8 @@ def int8_checkpoint_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional
 
     The forward product and the gradients of ``x`` and ``bias`` use the bf16 values; the gradient of ``weight`` is
     ``dy.T @ dequantize_int8_g32(quantize_int8_g32(x))``.  K is a multiple of ``group_size`` (16, 32, 64 or 128).
-    Values of ``x`` that are not finite enter the weight gradient as 0, as the codec stores them.  CUDA tensors
+    Values of ``x`` that are not finite enter the weight gradient as 0, as the codec stores them; decoded values past the largest bf16
+    number stay at it, so that a row of the lowest number adds nothing where its ``dy`` is 0.  CUDA tensors
     only; gradients of gradients are not available.  A training step can be captured in a CUDA graph under torch's own
     condition: no eager graph of the same leaves is alive during the capture (``del`` the outputs of warm-up steps).
     """

@@ -55,10 +55,8 @@
 //               tcgen05.ld -> (+bias) -> bf16 -> global (32- or 16-byte stores, or rows of 16 values)
 // No TMA multicast anywhere.
 //
-// The dequantised value is bf16((q - zp) * scale), the number the decode kernel produces:
-// the code byte is spliced into the mantissa of 2^15, one FMA with the exact constant
-// -(2^15 + zp) * scale yields (q - zp) * scale exactly in fp32 (16 x 8 significant
-// bits), and cvt.rn.bf16x2.f32 rounds two of them once.
+// The dequantised value is bf16((q - zp) * scale), the number the decode kernel produces
+// (convert16 says how, and what it does past the largest bf16 number).
 //
 // Every wait on an mbarrier is bounded by a clock budget.  When one runs out the
 // thread raises the abort flag of both CTAs of the pair and a device status word; all

@@ -6,7 +6,7 @@
 //
 // x, w, dy, y and the gradients are bf16, sums are fp32 (TMEM accumulators, fp32 partial sums) and rounded once.  The
 // kept input exists as int8 / uint8 codes and group scales only; deq(q) is the bf16 number the decode kernels
-// produce, made in shared memory by producer warps, and never goes to global memory.  (code x scale has up to 16 bits and the
+// produce (finite always: convert16), made in shared memory by producer warps, and never goes to global memory.  (code x scale has up to 16 bits and the
 // tensor cores take 8 of them: half a step of bf16 per term, 1.6e-3 of the norm of dw in all, as much as dw's own rounding.
 // Codes alone would be exact, but their scales change along the columns of a tile and cannot move to the other operand.)
 //

@@ -417,3 +417,65 @@ def test_last_rows_that_end_inside_a_warp(M, N):
     close(dw, D.t(), Q)
     close(fused.detach(), Q, W.t(), b.detach().double())
     close(as_weight, W, Q.t())
+
+
+LOWEST = torch.finfo(torch.bfloat16).min
+
+
+@pytest.mark.parametrize("M,N,K,G", [(70, 24, 96, 16), (300, 260, 512, 32), (513, 40, 256, 128)])
+def test_rows_of_the_lowest_value_that_no_gradient_reaches(M, N, K, G):
+    """Padding of the type's lowest value (and of its neighbours) is finite: with dy = 0 it adds nothing to a gradient."""
+    x, w, _, dy = layer(M, N, K, M)
+    out = torch.zeros(M, dtype=torch.bool, device=DEV)
+    out[::7] = out[-3:] = True
+    x[out] = LOWEST
+    x[0], x[7] = 3.0e38, -1.0e37
+    x[14, : K // 2], x[14, K // 2 :] = LOWEST, 0.0
+    dy[out] = 0
+    w.requires_grad_(True)
+    (dw,) = torch.autograd.grad(tc.int8_checkpoint_linear(x, w, group_size=G), [w], dy)
+    check_device_status()
+    close(dw, dy[~out].double().t(), decoded(*plain.int8_encode(x[~out], G), G))
+    q, s, _ = tc.quantize_int8_g32(x, G)
+    (dw2,) = torch.autograd.grad(tc.fused_dequant_linear(q.view(M, K), s, w, group_size=G), [w], dy)
+    assert torch.equal(dw2, dw)
+
+
+@pytest.mark.parametrize("zp", [False, True])
+@pytest.mark.parametrize("G", [16, 32, 64, 128])
+def test_groups_of_very_large_values_decode_as_elsewhere(G, zp):
+    """Scales up to 2^121: every code of the group keeps the value that the decoding functions give it, zeros among them,
+    in the forward product and in the weight gradient, and in the product with a quantised weight."""
+    M, N, K = 66, 40, 256
+    x, w, _, dy = layer(M, N, K, G)
+    w, dy = (w * 2.0 ** -20).requires_grad_(True), dy * 2.0 ** -20
+    big = torch.tensor([1e30, 1e34, 2e36, 1e37, 1e38, 3e38], device=DEV)
+    x = torch.rand(M, K, device=DEV) * 2 - 1
+    x = x * big[torch.randint(0, 6, (M, K // G, 1), device=DEV)].expand(-1, -1, G).reshape(M, K)
+    x[:, 1::3] = 0.0
+    x[:, ::G] = x[:, ::G].abs()
+    x = x.to(torch.bfloat16)
+    if zp:
+        q, s, z, shape = tc.compress(x.float().clamp(min=-1e38, max=1e38).to(torch.bfloat16), "fast", G)
+        X = tc.decompress(q, s, shape, z, G).double()
+    else:
+        (q, s, shape), z = tc.quantize_int8_g32(x, G), None
+        X = tc.dequantize_int8_g32(q, s, shape, G).double()
+    assert bool(X.isfinite().all()) and float(s.float().max()) > 2.0 ** 113      # beyond this, 2^15 scales are more than fp32 holds
+    y = tc.fused_dequant_linear(q.view(M, K), s, w, zero_points=z, group_size=G)
+    (dw,) = torch.autograd.grad(y, [w], dy)
+    check_device_status()
+    close(y.detach(), X, w.detach().double().t())
+    close(dw, dy.double().t(), X)
+    close(tc.fused_dequant_matmul(w.detach(), q.view(M, K), s, z, group_size=G), w.detach().double(), X.t())
+
+
+def test_values_past_the_largest_number_stay_at_it_and_infinite_scales_are_not_hidden():
+    """127 times a scale of 2.68e36 is finite in fp32 and not in bf16."""
+    x = torch.full((4, 32), LOWEST, dtype=torch.bfloat16, device=DEV)
+    q, s, _ = tc.quantize_int8_g32(x)
+    w = torch.full((8, 32), 2.0 ** -10, dtype=torch.bfloat16, device=DEV)
+    close(tc.fused_dequant_linear(q.view(4, 32), s, w), torch.full((4, 32), LOWEST, dtype=torch.float64, device=DEV), w.double().t())
+    s[1], s[2] = float("inf"), float("nan")
+    y = tc.fused_dequant_linear(q.view(4, 32), s, w)
+    assert y.isfinite().all(1).tolist() == [True, False, False, True]
