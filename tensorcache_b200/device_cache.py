@@ -11,6 +11,7 @@ import math
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .codec import _DTYPES, _check_group_size
@@ -25,6 +26,9 @@ class DeviceFeatureCache:
     ``codes`` (int8 ``[num_rows, width]``) and ``scales`` (bf16 ``[num_rows, width / group_size]``) are plain
     tensors that start as zeros; rows that were never written read as zeros.  The number of values of a row must be
     a multiple of ``group_size``.
+
+    To autograd a ``write`` is an in-place change of both tensors: a graph that keeps one of them (``fused_dequant_linear`` on the cache's own
+    codes) and is differentiated after the next write raises torch's error.
 
     Calls only enqueue work on the current stream of the cache's device (index tensors on the GPU are not looked
     at by the host), so they can be captured in a CUDA graph.  As with any tensor, calls on different streams need
@@ -92,6 +96,7 @@ class DeviceFeatureCache:
             _lib.check(_lib.lib().tcb_cache_write(xd.data_ptr(), _DTYPES[xd.dtype], idx.data_ptr(), n, self.codes.data_ptr(),
                                                   self.scales.data_ptr(), self.num_rows, self.width, self.group_size,
                                                   self._claims.data_ptr(), _lib.stream_of(self.device)))
+            increment_version((self.codes, self.scales))
 
     def read(self, indices: Indices, out_buffer: Optional[torch.Tensor] = None) -> torch.Tensor:
         """bf16 ``[n, *row_shape]``: row ``indices[t]`` decoded; a row that ``write`` would leave out is zeros.
@@ -103,6 +108,8 @@ class DeviceFeatureCache:
                 out_buffer = self.scales.new_empty((n, *self.row_shape))
             elif out_buffer.numel() != n * self.width or out_buffer.dtype != torch.bfloat16:
                 raise ValueError(f"out_buffer must be a bf16 tensor of {n} rows of {self.width} values")
+            else:
+                increment_version(out_buffer)   # the kernel writes through its address
             if n == 0 or self.width == 0:
                 return out_buffer
             direct = out_buffer.device == self.device and out_buffer.is_contiguous() and out_buffer.data_ptr() % 32 == 0

@@ -13,6 +13,7 @@ from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .codec import _DTYPES, _compute_device
@@ -105,6 +106,8 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, orig_shape: Tupl
         out_buffer = torch.empty(tuple(orig_shape), dtype=torch.bfloat16, device=codes.device)
     elif out_buffer.numel() != rows * cols or out_buffer.dtype != torch.bfloat16:
         raise ValueError("out_buffer must be a bf16 tensor of the decoded size")
+    else:
+        increment_version(out_buffer)   # the kernel writes through its address
     if rows == 0 or cols == 0:
         return out_buffer
     with _lib.on_device(dev):

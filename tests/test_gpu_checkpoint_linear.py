@@ -479,3 +479,45 @@ def test_values_past_the_largest_number_stay_at_it_and_infinite_scales_are_not_h
     s[1], s[2] = float("inf"), float("nan")
     y = tc.fused_dequant_linear(q.view(4, 32), s, w)
     assert y.isfinite().all(1).tolist() == [True, False, False, True]
+
+
+@pytest.mark.parametrize("new", [3, 1500])
+def test_cache_written_before_the_backward_pass_is_reported(new):
+    """The kernels write through raw addresses; the graph of a layer on the cache's own codes has to notice."""
+    cache = tc.DeviceFeatureCache(2000, 64, 32, DEV)
+    rows = torch.arange(new, device=DEV)
+    x = torch.randn(new, 64, device=DEV)
+    cache.write(rows, x)
+    w = torch.randn(8, 64, device=DEV).to(torch.bfloat16).requires_grad_(True)
+    y = tc.fused_dequant_linear(cache.codes, cache.scales, w)
+    picked = tc.fused_dequant_linear(cache.codes[rows], cache.scales[rows], w)       # copies: later writes do not matter
+    cache.read(rows)
+    torch.autograd.grad(y, [w], torch.ones_like(y), retain_graph=True)               # a read is not a change
+    cache.write(rows, x + 1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, [w], torch.ones_like(y))
+    torch.autograd.grad(picked, [w], torch.ones_like(picked))
+    scales = cache.scales.view(-1)
+    y = tc.fused_dequant_linear(cache.codes.clone(), scales, w)                      # a view of the scales alone
+    cache.write(rows, x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, [w], torch.ones_like(y))
+    with torch.inference_mode():                                                     # tensors without a version counter
+        other = tc.DeviceFeatureCache(10, 64, 32, DEV)
+        other.write([1], x[:1])
+        assert torch.equal(other.read([1], out_buffer=torch.empty(1, 64, dtype=torch.bfloat16, device=DEV)), cache.read([0]))
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+def test_buffers_decoded_into_before_the_backward_pass_are_reported(aligned):
+    buf = torch.empty(16 * 64 + 1, dtype=torch.bfloat16, device=DEV)[0 if aligned else 1:][:1024].view(16, 64)
+    x = torch.randn(16, 64, device=DEV)
+    codes, scales, shape = tc.quantize_mxfp4(x)
+    cache = tc.DeviceFeatureCache(16, 64, 32, DEV)
+    cache.write(range(16), x)
+    w = torch.randn(8, 64, device=DEV).to(torch.bfloat16).requires_grad_(True)
+    for fill in (lambda: tc.dequantize_mxfp4(codes, scales, shape, out_buffer=buf), lambda: cache.read(range(16), out_buffer=buf)):
+        y = fill() @ w.t()
+        fill()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, [w], torch.ones_like(y))
