@@ -91,13 +91,14 @@ def _backward(dy: torch.Tensor, sizes, weight, q, scales, zp, group_size: int, n
 
 class _CheckpointLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, group_size):
+    def forward(ctx, x, weight, bias, group_size, grad_mode):
         N, K = weight.shape
         dev = x.device
         x2 = _operand(x if x.dim() == 2 else x.reshape(-1, K))
         M = x2.shape[0]
         y = x2.new_empty((M, N))
-        need_dx, need_dw, _, _ = ctx.needs_input_grad
+        # needs_input_grad tells what requires a gradient even where no graph is recorded, and in here grad mode is always off
+        need_dx, need_dw = (grad_mode and need for need in ctx.needs_input_grad[:2])
         # codes [M, K], then scales [M, K / G]: one buffer (M K is a multiple of 16, so the scales are aligned)
         kept = torch.empty(M * K + 2 * (M * K // group_size), dtype=torch.uint8, device=dev) if need_dw else None
         if M and N:
@@ -119,9 +120,9 @@ class _CheckpointLinear(torch.autograd.Function):
 
 def _checkpoint_backward(ctx, dy):
     kept, weight = ctx.saved_tensors
-    need_dx, need_dw, need_db, _ = ctx.needs_input_grad
+    need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
     dx, dw, db = _backward(dy, ctx.sizes, weight, kept, None, None, ctx.group_size, need_dx, need_dw, need_db)
-    return dx.view(ctx.x_shape) if need_dx and len(ctx.x_shape) != 2 else dx, dw, db, None
+    return dx.view(ctx.x_shape) if need_dx and len(ctx.x_shape) != 2 else dx, dw, db, None, None
 
 
 # with create_graph the results refuse to be differentiated; the wrapper is left out where nobody could
@@ -158,6 +159,7 @@ _fused_backward_once = once_differentiable(_fused_backward)
 def int8_checkpoint_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, group_size: int = 32) -> torch.Tensor:
     """``x @ weight.T + bias`` (bf16 ``[..., K]`` -> ``[..., N]``) that keeps ``x`` in 8 bits for the backward pass.
 
+    Without a graph (``torch.no_grad()``, nothing that requires a gradient) no codes are made.
     The forward product and the gradients of ``x`` and ``bias`` use the bf16 values; the gradient of ``weight`` is
     ``dy.T @ dequantize_int8_g32(quantize_int8_g32(x))``.  K is a multiple of ``group_size`` (16, 32, 64 or 128).
     Values of ``x`` that are not finite enter the weight gradient as 0, as the codec stores them; decoded values past the largest bf16
@@ -176,7 +178,7 @@ def int8_checkpoint_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional
     _check_layer(weight, bias, K, x.device)
     if not x.is_cuda:
         raise RuntimeError("int8_checkpoint_linear runs on CUDA tensors only (no CPU fallback)")
-    return _CheckpointLinear.apply(x, weight, bias, group_size)
+    return _CheckpointLinear.apply(x, weight, bias, group_size, torch.is_grad_enabled())
 
 
 def fused_dequant_linear(q: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,

@@ -521,3 +521,41 @@ def test_buffers_decoded_into_before_the_backward_pass_are_reported(aligned):
         fill()
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(y, [w], torch.ones_like(y))
+
+
+@pytest.mark.parametrize("mode", ["no_grad", "inference_mode", "frozen", "reentrant"])
+def test_without_a_graph_no_codes_are_made(mode, monkeypatch):
+    """Evaluation of a trainable layer: only the product, and no memory but the output's."""
+    from torch.utils.checkpoint import checkpoint
+
+    from tensorcache_b200 import _lib
+
+    x, w, b, dy = layer(8192, 16, 1024)      # many rows, few outputs: the codes would be the larger part
+    w.requires_grad_(mode != "frozen")
+    x.requires_grad_(mode == "reentrant")
+    want = tc.int8_checkpoint_linear(x.detach(), w.detach(), b)
+    made, real = [], _lib.lib()
+
+    class Watch:
+        def __getattr__(self, name):
+            f = getattr(real, name)
+            return (lambda *a: made.append(a[4]) or f(*a)) if name == "tcb_linear_forward" else f
+
+    watch = Watch()
+    monkeypatch.setattr(_lib, "lib", lambda: watch)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    if mode == "reentrant":      # the first pass records nothing, the second one does
+        y = checkpoint(tc.int8_checkpoint_linear, x, w, b, use_reentrant=True)
+        assert made == [None]
+        y.backward(dy)
+        assert made[0] is None and made[1] is not None
+        close(x.grad, dy.double(), w.detach().double())
+        close(w.grad, dy.double().t(), decoded(*plain.int8_encode(x.detach(), 32), 32))
+    else:
+        with {"no_grad": torch.no_grad, "inference_mode": torch.inference_mode, "frozen": torch.enable_grad}[mode]():
+            y = tc.int8_checkpoint_linear(x, w, b)
+        grown = torch.cuda.max_memory_allocated() - before
+        assert made == [None] and grown < 8192 * 1024
+    assert torch.equal(y.detach(), want)
