@@ -20,7 +20,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .fused_linear import SUPPORTED_GROUP_SIZES, _check_common, _launch, _operand_on
+from .fused_linear import SUPPORTED_GROUP_SIZES, _check_common, _launch, _operand_on, _refuse_gradient
 
 
 def _check_dense(name: str, t: torch.Tensor, device: torch.device) -> None:
@@ -185,9 +185,11 @@ def fused_dequant_linear(q: torch.Tensor, scales: torch.Tensor, weight: torch.Te
                          zero_points: Optional[torch.Tensor] = None, group_size: int = 32) -> torch.Tensor:
     """``dequant(q) @ weight.T + bias`` for codes ``[..., K]`` (int8, or uint8 with zero points), differentiable in
     ``weight`` and ``bias``: ``dweight = dy.T @ dequant(q)``, straight from the codes.  The values are those of
-    ``FusedDequantLinear``, which has no gradient; K is a multiple of ``group_size`` (16, 32, 64 or 128)."""
+    ``FusedDequantLinear``, which has no gradient; K is a multiple of ``group_size`` (16, 32, 64 or 128).
+    ``scales`` that require a gradient are refused."""
     if q.dim() == 0:
         raise ValueError("q must be [..., K]")
+    _refuse_gradient("fused_dequant_linear: scales", scales)
     K = q.shape[-1]
     flat = q.dim() == 2      # a view of the result would be one more node of the graph
     q2 = (q if flat else q.reshape(-1, K) if K else q.reshape(0, 0)).contiguous()

@@ -21,6 +21,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -43,6 +44,14 @@ def _operand_on(t: torch.Tensor, device: torch.device, nbytes: int) -> torch.Ten
     if not t.is_contiguous():
         t = t.contiguous()
     return t if t.data_ptr() % nbytes == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _refuse_gradient(what: str, t: torch.Tensor) -> None:
+    """Raises where a result that knows nothing of ``t`` would drop a gradient or a forward-mode tangent without a word."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or detach it")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{what} has no gradient, and it carries a forward-mode tangent")
 
 
 def _launch(dense, q, scales, zp, bias, out, R_d, R_q, K, group_size, quant_is_rhs):

@@ -17,7 +17,7 @@ from torch.autograd.graph import increment_version
 
 from . import _lib
 from .codec import _DTYPES, _compute_device
-from .fused_linear import _operand_on
+from .fused_linear import _operand_on, _refuse_gradient
 
 BLOCK = 32          # values that share a scale
 _TILE_ROWS = 128    # a scale tile covers 128 rows x 4 blocks
@@ -132,7 +132,7 @@ def mxfp4_matmul(x: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor, bias
 
     ``x`` is bf16, fp16 or fp32 ``[..., K]`` and is quantised by the call, each row in blocks of 32; the result is bf16
     ``[..., N]``, summed in fp32 and rounded once.  The counterpart of ``fused_dequant_matmul`` for 4-bit weights, and
-    like it without a gradient: an ``x`` that requires one is refused.  CUDA tensors only.
+    like it without a gradient: an ``x`` or ``bias`` that requires one (or carries a forward-mode tangent) is refused.  CUDA tensors only.
     """
     if wq.dim() != 2 or x.dim() == 0:
         raise ValueError(f"x must be [..., K] and wq [N, K / 2], got {tuple(x.shape)} and {tuple(wq.shape)}")
@@ -146,8 +146,9 @@ def mxfp4_matmul(x: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor, bias
         raise ValueError(f"bias must be bf16 [{N}] on {x.device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
     if wq.device != x.device:
         raise ValueError(f"x is on {x.device}, the weight on {wq.device}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError("mxfp4_matmul has no gradient: call it under torch.no_grad() or detach x")
+    _refuse_gradient("mxfp4_matmul: x", x)
+    if bias is not None:
+        _refuse_gradient("mxfp4_matmul: bias", bias)
     if not x.is_cuda:
         raise RuntimeError("mxfp4_matmul runs on CUDA tensors only (no CPU fallback)")
     dev = x.device

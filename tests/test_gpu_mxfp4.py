@@ -291,3 +291,28 @@ def test_features_through_4_and_8_bits_together():
     wq, ws, _ = tc.quantize_mxfp4(trained)
     rows = cache.read(pick)
     product_close(tc.mxfp4_matmul(rows, wq, ws), plain.mx_values(*plain.mx_encode(rows)), plain.mx_values(*plain.mx_encode(trained)))
+
+
+def test_trainable_operands_without_a_gradient_are_refused_in_grad_mode_only():
+    x, w, b = product_inputs(4, 8, 64)
+    wq, ws, _ = tc.quantize_mxfp4(w)
+    want = tc.mxfp4_matmul(x, wq, ws, b)
+    bias = torch.nn.Parameter(b)
+    with pytest.raises(ValueError, match="bias has no gradient"):
+        tc.mxfp4_matmul(x, wq, ws, bias)
+    with torch.no_grad():
+        assert torch.equal(tc.mxfp4_matmul(x, wq, ws, bias), want)
+    assert torch.equal(tc.mxfp4_matmul(x, wq, ws, bias.detach()), want)
+    q, s, _ = tc.quantize_int8_g32(x)
+    s.requires_grad_(True)
+    with pytest.raises(ValueError, match="scales has no gradient"):
+        tc.fused_dequant_linear(q.view(4, 64), s, w)
+    with torch.no_grad():
+        assert torch.equal(tc.fused_dequant_linear(q.view(4, 64), s, w), tc.fused_dequant_linear(q.view(4, 64), s.detach(), w))
+    weight = torch.randn(8, 64, device=DEV).to(torch.bfloat16)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(weight, torch.ones_like(weight))
+        for call in (lambda: tc.fused_dequant_linear(q.view(4, 64), s.detach(), dual), lambda: tc.int8_checkpoint_linear(weight, dual),
+                     lambda: tc.int8_checkpoint_linear(dual, weight)):
+            with pytest.raises((NotImplementedError, RuntimeError)):
+                call()

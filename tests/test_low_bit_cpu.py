@@ -169,3 +169,26 @@ def test_linear_layer_refusals():
         tc.fused_dequant_linear(q, s[:-1], w, b)
     with pytest.raises(ValueError, match="int8"):
         tc.fused_dequant_linear(q.to(torch.uint8), s, w, b)
+
+
+def test_operands_whose_gradient_would_be_dropped_are_refused():
+    from torch.autograd import forward_ad
+
+    bf = torch.bfloat16
+    x, wq, ws = torch.zeros(4, 64), torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8)
+    b = torch.zeros(8, dtype=bf)
+    q, s, w = torch.zeros(4, 64, dtype=torch.int8), torch.zeros(8, dtype=bf), torch.zeros(8, 64, dtype=bf)
+    calls = {"x": (lambda t: tc.mxfp4_matmul(t, wq, ws, b), x), "bias": (lambda t: tc.mxfp4_matmul(x, wq, ws, bias=t), b),
+             "scales": (lambda t: tc.fused_dequant_linear(q, t, w, b), s)}
+    for name, (call, t) in calls.items():
+        wants = t.clone().requires_grad_(True)
+        with pytest.raises(ValueError, match=f"{name} has no gradient"):
+            call(wants)
+        with forward_ad.dual_level():
+            with pytest.raises(ValueError, match=f"{name} has no gradient.* tangent"):
+                call(forward_ad.make_dual(t, torch.ones_like(t)))
+            with pytest.raises(RuntimeError, match="CUDA"):      # nothing to refuse but the device
+                call(t)
+        for allowed in (wants.detach(), wants):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+                call(allowed)
