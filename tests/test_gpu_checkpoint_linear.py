@@ -559,3 +559,42 @@ def test_without_a_graph_no_codes_are_made(mode, monkeypatch):
         grown = torch.cuda.max_memory_allocated() - before
         assert made == [None] and grown < 8192 * 1024
     assert torch.equal(y.detach(), want)
+
+
+@pytest.mark.parametrize("M,N,K", [(96, 48, 64), (130, 257, 96), (4000, 24, 128)])
+@pytest.mark.parametrize("source", ["x", "sym", "amo"])
+def test_gradients_equal_differences_of_whole_numbers(M, N, K, source):
+    """Whole numbers small enough that nothing is rounded: outputs, gradients and their differences are exact, so the change
+    of the loss over a step has to EQUAL the gradient times the step -- and neither 0 nor its negative would."""
+    g = torch.Generator(device=DEV).manual_seed(M + N)
+
+    def whole(shape, keep=0.5):
+        v = torch.randint(0, 2, shape, generator=g, device=DEV) * 2 - 1
+        return (v * (torch.rand(shape, generator=g, device=DEV) < keep)).to(torch.bfloat16)
+
+    x, w, b = whole((M, K)), whole((N, K)), whole((N,))
+    x[:, ::32], w[:, ::32] = 127, 0                # scale 1 in every group; no weight where a product would be large
+    dy = whole((M, N), min(0.5, 60 / M))
+    leaves = [w, b] + ([x] if source == "x" else [])
+    for t in leaves:
+        t.requires_grad_(True)
+    q, s = x.detach().to(torch.int8), torch.ones(M * K // 32, dtype=torch.bfloat16, device=DEV)
+    z = None
+    if source == "amo":
+        z = torch.full_like(s, 128, dtype=torch.uint8)
+        q = (x.detach().int() + 128).to(torch.uint8)
+
+    def output(w, b, x=x):
+        return tc.int8_checkpoint_linear(x, w, b) if source == "x" else tc.fused_dequant_linear(q, s, w, b, zero_points=z)
+
+    y = output(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    assert torch.equal(y.detach().double(), x.detach().double() @ w.detach().double().t() + b.detach().double())
+    for i, grad in enumerate(grads):
+        moved = [t.detach() for t in leaves]
+        step = whole(moved[i].shape)
+        step[..., ::32] = 0 if moved[i].dim() == 2 else step[..., ::32]
+        moved[i] = moved[i] + step                # at most 2: exact
+        change = ((output(*moved).double() - y.detach().double()) * dy.double()).sum()
+        slope = (grad.double() * step.double()).sum()
+        assert float(change) == float(slope) and float(slope) != 0, (i, float(change), float(slope))
