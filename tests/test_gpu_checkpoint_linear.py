@@ -598,3 +598,32 @@ def test_gradients_equal_differences_of_whole_numbers(M, N, K, source):
         change = ((output(*moved).double() - y.detach().double()) * dy.double()).sum()
         slope = (grad.double() * step.double()).sum()
         assert float(change) == float(slope) and float(slope) != 0, (i, float(change), float(slope))
+
+
+@pytest.mark.parametrize("N,K", [(8, 2080), (2080, 32)])
+def test_layers_of_more_than_2_31_values(N, K):
+    """More than 2^31 inputs, or outputs: zeros but for the last rows, whose results are checked."""
+    M, tail = (1 << 20) + 3, slice(-300, None)
+    xt, w, b, dyt = layer(300, N, K, N)
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device=DEV)
+    x[tail] = xt
+    dy = torch.zeros(M, N, dtype=torch.bfloat16, device=DEV)
+    dy[tail] = dyt
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = tc.int8_checkpoint_linear(*leaves)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    check_device_status()
+    X, W, D, Q = xt.double(), w.detach().double(), dyt.double(), decoded(*plain.int8_encode(xt, 32), 32)
+    ones = torch.ones(1, 300, dtype=torch.float64, device=DEV)
+    close(y[tail].detach(), X, W.t(), b.detach().double())
+    assert bool((y[:1000] == b).all()) and not bool(dx[:1000].any())
+    close(dx[tail], D, W)
+    close(dw, D.t(), Q)
+    close(db.view(1, -1), ones, D)
+    del y, dx
+    q, s, _ = tc.quantize_int8_g32(x.detach())
+    y = tc.fused_dequant_linear(q.view(M, K), s, w, b)
+    (dw2,) = torch.autograd.grad(y, [w], dy)
+    check_device_status()
+    close(y[tail].detach(), Q, W.t(), b.detach().double())
+    assert bool((y[:1000] == b).all()) and torch.equal(dw2, dw)

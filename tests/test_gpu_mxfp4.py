@@ -192,6 +192,32 @@ def test_product_whose_last_rows_and_columns_end_inside_a_warp(M, N, K):
     product_close(y, plain.mx_values(*plain.mx_encode(x)), plain.mx_values(*plain.mx_encode(w)), b)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 19300, 4096), (2, 38001, 4128), (16, 19100, 8192), (32, 19300, 2048)])
+def test_product_of_few_rows_with_more_tiles_than_the_gpu_runs_at_once(M, N, K):
+    """Several waves of CTAs, with the short ring that a long row of x leaves room for."""
+    x, w, b = product_inputs(M, N, K, seed=N)
+    wq, ws, _ = tc.quantize_mxfp4(w)
+    y = tc.mxfp4_matmul(x, wq, ws, bias=b)
+    check_device_status()
+    product_close(y, plain.mx_values(*plain.mx_encode(x)), plain.mx_values(*plain.mx_encode(w)), b)
+
+
+@pytest.mark.parametrize("M,N,K", [((1 << 20) + 3, 40, 2080), ((1 << 20) + 3, 2080, 32), (40, (1 << 20) + 3, 4128), (3, (1 << 20) + 3, 4128)])
+def test_products_of_more_than_2_31_values(M, N, K):
+    """More than 2^31 values of x, of the result or bytes of the weight's codes: zeros but for the last rows and columns."""
+    x, w = torch.zeros(M, K, dtype=torch.bfloat16, device=DEV), torch.zeros(N, K, dtype=torch.bfloat16, device=DEV)
+    xt, wt, _ = product_inputs(min(M, 130), min(N, 150), K, seed=K)
+    x[-xt.shape[0]:], w[-wt.shape[0]:] = xt, wt
+    wq, ws, _ = tc.quantize_mxfp4(w)
+    y = tc.mxfp4_matmul(x, wq, ws)
+    check_device_status()
+    product_close(y[-xt.shape[0]:, -wt.shape[0]:], plain.mx_values(*plain.mx_encode(xt)), plain.mx_values(*plain.mx_encode(wt)))
+    if M > 130:
+        assert not bool(y[:1000].any())
+    if N > 150:
+        assert not bool(y[:, :1000].any())
+
+
 def test_scales_that_pad_a_row_do_not_reach_the_sums():
     """K = 32 in a tile of 128: the other three scales of a row are padding."""
     for M in (3, 40):
