@@ -189,8 +189,9 @@ TCB_API int tcb_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, in
 /*
  * Product of MXFP4 operands on the block-scaled tensor-core path:
  *     out[m, n] = bf16( sum_k X[m, k] W[n, k] + bias[n] )          (fp32 sums)
- * with X = the MXFP4 values of x (quantised by the call, as tcb_quantize_mxfp4 does) and W the
- * values of wq [N, K / 2], w_scales (tile order; no padding byte may be 255: it would be a NaN).
+ * with X = the MXFP4 values of x (quantised by the call, as tcb_quantize_mxfp4 does: values that
+ * are not finite count as 0 and do not show in out) and W the values of wq [N, K / 2], w_scales
+ * (tile order; no padding byte may be 255: it would be a NaN).
  * No counterpart in the reference.
  *   x [M, K] of `dtype`, 32-byte aligned; wq, w_scales 16-byte aligned; bias bf16 [N] or NULL;
  *   out [M, N] bf16; workspace: tcb_mxfp4_linear_workspace(M, N, K) bytes (NULL where that

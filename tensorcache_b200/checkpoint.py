@@ -184,8 +184,8 @@ def int8_checkpoint_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional
 def fused_dequant_linear(q: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                          zero_points: Optional[torch.Tensor] = None, group_size: int = 32) -> torch.Tensor:
     """``dequant(q) @ weight.T + bias`` for codes ``[..., K]`` (int8, or uint8 with zero points), differentiable in
-    ``weight`` and ``bias``: ``dweight = dy.T @ dequant(q)``, straight from the codes.  The values are those of
-    ``FusedDequantLinear``, which has no gradient; K is a multiple of ``group_size`` (16, 32, 64 or 128).
+    ``weight`` and ``bias``: ``dweight = dy.T @ dequant(q)``, straight from the codes.  ``dequant`` rounds to bf16, as the decoding
+    functions do; the values are those of ``FusedDequantLinear``, which has no gradient.  K is a multiple of ``group_size`` (16, 32, 64 or 128).
     ``scales`` that require a gradient are refused."""
     if q.dim() == 0:
         raise ValueError("q must be [..., K]")

@@ -261,11 +261,16 @@ mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 
 // Shape of a launch; stages == 0: this kernel does not take the sizes.
 //
-// Rules and what they were measured on (us, consecutive calls on different weights; rows of x x rows of w x 4096):
-//   few rows against the tiles of 256 x 256 with their own quantisation
-//                                   1 x 14336: 9.1 / 14.9   16 x 14336: 11.9 / 12.9   32 x 4096: 7.3 / 11.0   32 x 14336: 14.6 / 12.9
-//     the last because every CTA quantises all of its K for every row: above 16 rows only where that is at most 8 stages
-//   K split over a cluster or not   1 x 4096: 4.6 / 7.0     1 x 1024: 3.7 / 6.8; with two CTAs an SM 1 x 14336: 8.2, 1 x 4096: 4.9
+// Rules and what they were measured on (us, consecutive calls on different weights in a graph; rows of x x rows of w x K):
+//   this kernel against tiles of 256 rows of x after a quantisation of their own
+//     1 x 4096 x 4096: 5.5 / 10.4    1 x 14336 x 4096: 9.6 / 15.4    1 x 4096 x 14336: 9.8 / 25.4    1 x 28672 x 8192: 29.2 / 41.7
+//     1 x 128256 x 4096: 60.7 / 71.2   16 x 14336 x 4096: 12.4 / 14.1   32 x 4096 x 4096: 7.3 / 11.0   32 x 14336 x 4096: 14.6 / 12.9
+//     the last because every CTA quantises all of its K for every row: above 16 rows only where that is at most 8 stages.  Up to 16
+//     rows always, although several waves of CTAs pay for that too: 16 x 28672 x 8192: 41.3 / 35.6, 16 x 128256 x 4096: 82.2 / 69.4
+//   K split over a cluster or not   1 x 4096 x 4096: 4.6 / 7.0     1 x 1024 x 4096: 3.7 / 6.8
+//   ring: as deep as it goes where every CTA has an SM to itself (1 x 14336 x 4096 9.1, with room for a second CTA 8.2, but 1 x 4096 x
+//     4096 4.6 / 4.9).  With more tiles than SMs it leaves room for a second CTA as long as that keeps four stages: up to 16 rows
+//     of x take 3 KB a stage of K, so up to K = 3584.  Beyond that four stages stay and one CTA runs per SM.
 struct Shape {
     int cols, parts, kb_per_cta, stages;
     uint32_t smem;
@@ -285,7 +290,6 @@ Shape few_rows_shape(int64_t M, int64_t N, int64_t K) {
     if (M > 16 && per > 8) return s;
     s.kb_per_cta = int(per);
     const uint32_t fixed = uint32_t(per) * (s.cols * 128 + 1024) + 1024 /* alignment */ + 256 /* barriers */;
-    // a deep ring where every CTA has an SM to itself, else one that leaves room for a second CTA
     const uint32_t room = tiles * s.parts <= tcb::sm_count() ? kMaxSmem : kMaxSmem / 2 - 1024;
     int stages = int(per < 12 ? per : 12);
     while (stages > 4 && fixed + stages * kStageBytes > room) --stages;

@@ -336,7 +336,9 @@ extern "C" int tcb_mxfp4_linear(const void* x, int dtype, const uint8_t* wq, con
     if (rc == TCB_OK) rc = encode_maps(who, &map_x, &map_xs, xq, xs, M, K, kTileRows, 1);
     if (rc != TCB_OK) return rc;
     // Tiles of 256 x 128 where all of them run at once: half the products and half the results to store per SM (us with the
-    // quantisation, halved / whole tiles: 446 x 1001 x 768 8.3 / 11.0, 64 x 4096 x 4096 9.8 / 10.9, 1024 x 1024 x 1024 7.6 / 8.5).
+    // quantisation, halved / whole tiles: 446 x 1001 x 768 8.4 / 11.2, 64 x 4096 x 4096 10.9 / 12.0, 512 x 4736 x 4096 12.5 / 13.6,
+    // 1024 x 1024 x 1024 7.9 / 9.2).  With more of them the second round costs more than that (64 x 10240 x 4096 16.0 / 12.9, 512 x
+    // 5120 x 4096 17.2 / 14.0, 2048 x 4096 x 4096 31.8 / 23.8; on short sums it does not matter: 1024 x 4096 x 768 9.8 / 10.1).
     const int pairs = tcb::sm_count() / 2 > 0 ? tcb::sm_count() / 2 : 1;
     Params p;
     p.M = M;

@@ -130,7 +130,8 @@ def mxfp4_matmul(x: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor, bias
     """``mxfp4(x) @ dequant(W).T (+ bias)`` on the 4-bit tensor cores, with W stored as MXFP4 (``wq`` uint8 ``[N, K / 2]``,
     ``w_scales`` in tile order, both as ``quantize_mxfp4`` returns them for ``[N, K]``).
 
-    ``x`` is bf16, fp16 or fp32 ``[..., K]`` and is quantised by the call, each row in blocks of 32; the result is bf16
+    ``x`` is bf16, fp16 or fp32 ``[..., K]`` and is quantised by the call, each row in blocks of 32 as ``quantize_mxfp4`` does it:
+    infinities and NaN count as 0 and do NOT show in the result (test ``x.isfinite()`` where that matters).  The result is bf16
     ``[..., N]``, summed in fp32 and rounded once.  The counterpart of ``fused_dequant_matmul`` for 4-bit weights, and
     like it without a gradient: an ``x`` or ``bias`` that requires one (or carries a forward-mode tangent) is refused.  CUDA tensors only.
     """
